@@ -537,6 +537,108 @@ void pf_load_state_set_completed(pf_load_state *state);          /* :173-177 */
 void pf_load_state_set_error(pf_load_state *state);              /* :180-182 */
 void pf_load_state_free(pf_load_state *state);                   /* unlinks when it created it */
 
+/* ------------------------------------------------------------------------------------------
+ * 5. KV cache held in 8 bits (no counterpart in the reference, which moves the cache's bytes as
+ *    they are).  One layer's cache is [2 (K, V)][num_blocks] records.  A record holds
+ *    kv_heads x block_size x head_dim e4m3 values (head-major) and behind them one fp32 scale for
+ *    each head, padded to 16 bytes: a value stands for itself times its head's scale.  Scales are
+ *    powers of two, the least that brings the head's largest finite magnitude in that block within 448
+ *    (exponents -110 to 120).  To the engine it is a layer of two segments of pf_kv8_record_bytes
+ *    bytes: registration, save, load and peer copy move a block together with its scales.
+ *
+ *    All calls only enqueue work on `stream` (of the device `device_id`, which need not be the
+ *    current one), allocate nothing and may be captured.  Block tables, lengths and row starts
+ *    are device memory, read when the work runs.  What cannot be checked before the launch is checked
+ *    by the kernels, which leave the offending access out and set a bit in *status.
+ * ---------------------------------------------------------------------------------------- */
+typedef struct pf_kv8_cache {
+  uint64_t data_ptr;         /* 16-byte aligned, like both strides */
+  size_t block_stride_bytes; /* at least pf_kv8_record_bytes */
+  size_t kv_stride_bytes;    /* K record -> V record of the same block */
+  size_t num_blocks;
+  uint32_t block_size;       /* tokens: 16, 32, 64 or 128 */
+  uint32_t kv_heads;         /* 1 .. 1024 */
+  uint32_t head_dim;         /* 64, 128 or 256 */
+} pf_kv8_cache;
+/* Bytes of one record, 0 when the geometry is not supported. */
+size_t pf_kv8_record_bytes(uint32_t block_size, uint32_t kv_heads, uint32_t head_dim);
+
+enum pf_kv8_dtype { PF_KV8_BF16 = 0, PF_KV8_F16 = 1 };
+
+/* Bits of *status: what a kernel found and left out. */
+#define PF_KV8_BAD_BLOCK 1u   /* a block id outside the cache: its tokens are not written / not seen */
+#define PF_KV8_BAD_LENGTH 2u  /* a length below 0, or above what the block table or the weights hold: cut */
+#define PF_KV8_BAD_ROWS 4u    /* row starts that fall, leave the tensors, or give a sequence more than max_query rows: cut */
+
+typedef struct pf_kv8_batch {
+  const int32_t *block_tables; /* [n_seqs][max_blocks], rows table_stride elements apart */
+  size_t table_stride;
+  uint32_t max_blocks;
+  uint32_t n_seqs;             /* at most PF_KV8_MAX_SEQS */
+  const int32_t *lens;         /* [n_seqs] tokens of each sequence */
+  const int32_t *starts;       /* [n_seqs + 1]: rows starts[s] .. starts[s + 1] belong to sequence s; rows behind the
+                                  last are not read and not written.  NULL: the rows are divided evenly */
+  uint32_t *status;            /* device word, or NULL */
+} pf_kv8_batch;
+#define PF_KV8_MAX_SEQS 8192
+
+/* Write new tokens: row i of sequence s becomes token lens[s] + i (lens are the lengths before the call; they are
+ * not changed).  A block that was empty gets the scale of its new rows; one that was not keeps its scale, or
+ * takes the larger one that a new row needs, its old rows rounded anew.  Rows of a block behind the last token are
+ * left as they were.  Infinities are stored as the largest value, a NaN as NaN.  Strides are in elements; the last
+ * dimension is dense.  No two sequences of a call may append into one block. */
+int pf_kv8_append(int device_id, const pf_kv8_cache *cache, const pf_kv8_batch *batch, const void *k, const void *v,
+                  int dtype, size_t n_rows, size_t k_row_stride, size_t k_head_stride, size_t v_row_stride,
+                  size_t v_head_stride, void *stream);
+
+/* Attention of n_rows query rows over the cache.  lens include the rows' own tokens: row i of a sequence with n rows
+ * is token lens - n + i and sees, with `causal`, the tokens up to itself, otherwise all.  out = sum p * V with
+ * p = exp(scale * q.K - lse) over the visible tokens; a row that sees nothing gives out = 0, lse = -infinity.
+ * weights (may be NULL) [n_seqs][kv_heads][weights_capacity]: the sum of p over the sequence's rows and the
+ * query heads of the group is added for each token, in an order that does not vary. */
+typedef struct pf_kv8_attention_args {
+  const void *q;               /* [n_rows][q_heads][head_dim], q_heads a multiple of kv_heads */
+  void *out;                   /* the same shape and type */
+  float *lse;                  /* [n_rows][q_heads] dense, or NULL */
+  float *weights;
+  size_t n_rows;
+  size_t max_query;            /* most rows of a sequence */
+  size_t q_row_stride, q_head_stride, out_row_stride, out_head_stride; /* elements */
+  size_t weights_seq_stride, weights_head_stride;                      /* elements */
+  size_t weights_capacity;
+  uint32_t q_heads;
+  int dtype;
+  int causal;
+  int clear_tail;              /* 1: rows behind the last sequence get out = 0, lse = -infinity */
+  float scale;
+} pf_kv8_attention_args;
+/* Workspace bytes for a call of these sizes (pointers are not looked at).  The workspace is device memory, 256-byte
+ * aligned, used by one call at a time. */
+int pf_kv8_attention_workspace(int device_id, const pf_kv8_cache *cache, const pf_kv8_batch *batch,
+                               const pf_kv8_attention_args *args, size_t *bytes);
+int pf_kv8_attention(int device_id, const pf_kv8_cache *cache, const pf_kv8_batch *batch,
+                     const pf_kv8_attention_args *args, void *workspace, size_t workspace_bytes, void *stream);
+
+/* Eviction by accumulated weight.  Of each sequence and KV head, min(len, keep) tokens are kept: the last `recent` and,
+ * of the others, those of largest weight (equal weights: the lower index; NaN counts as the least), in their
+ * order.  They are copied into the blocks of dst_tables, with a scale for each new block and head as pf_kv8_append
+ * gives; the source blocks are not changed and must not be among the destination's.  kept receives the
+ * source indices (-1 behind the last), new_weights the kept weights (0 behind the last, up to
+ * new_capacity >= keep), new_lens the lengths.  batch->starts is ignored. */
+typedef struct pf_kv8_evict_args {
+  const float *weights;
+  size_t weights_seq_stride, weights_head_stride, weights_capacity; /* elements */
+  const int32_t *dst_tables;   /* [n_seqs][ceil(keep / block_size)] */
+  size_t dst_table_stride;
+  size_t keep, recent;         /* recent <= keep */
+  int32_t *new_lens;           /* [n_seqs] */
+  float *new_weights;          /* [n_seqs][kv_heads][new_capacity] dense */
+  size_t new_capacity;
+  int32_t *kept;               /* [n_seqs][kv_heads][keep] dense */
+} pf_kv8_evict_args;
+int pf_kv8_evict(int device_id, const pf_kv8_cache *cache, const pf_kv8_batch *batch, const pf_kv8_evict_args *args,
+                 void *stream);
+
 #ifdef __cplusplus
 }
 #endif

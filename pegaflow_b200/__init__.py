@@ -9,3 +9,12 @@ from .backend import (HostRun, LayerXfer, PinnedPool, TransferBackend, enable_pe
                       numa_node_of_device, save_blocks_noalloc)
 from .engine import Block, Completion, PegaEngine, PyLoadState  # noqa: F401
 from .connector import InProcEngineClient, QueryLoading, QueryReady, TransferStats  # noqa: F401,E402
+
+
+def __getattr__(name):
+    # the 8-bit cache works on torch tensors; everything else here does without torch, so it is imported on first use
+    if name == "Kv8Cache":
+        from .kv8 import Kv8Cache
+
+        return Kv8Cache
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

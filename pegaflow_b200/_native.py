@@ -214,6 +214,39 @@ _sig("pf_load_state_set_error", None, vp)
 _sig("pf_load_state_free", None, vp)
 
 
+class Kv8CacheDesc(C.Structure):
+    _fields_ = [("data_ptr", u64), ("block_stride_bytes", sz), ("kv_stride_bytes", sz), ("num_blocks", sz),
+                ("block_size", u32), ("kv_heads", u32), ("head_dim", u32)]
+
+
+class Kv8Batch(C.Structure):
+    _fields_ = [("block_tables", vp), ("table_stride", sz), ("max_blocks", u32), ("n_seqs", u32), ("lens", vp),
+                ("starts", vp), ("status", vp)]
+
+
+class Kv8AttentionArgs(C.Structure):
+    _fields_ = [("q", vp), ("out", vp), ("lse", vp), ("weights", vp), ("n_rows", sz), ("max_query", sz),
+                ("q_row_stride", sz), ("q_head_stride", sz), ("out_row_stride", sz), ("out_head_stride", sz),
+                ("weights_seq_stride", sz), ("weights_head_stride", sz), ("weights_capacity", sz), ("q_heads", u32),
+                ("dtype", C.c_int), ("causal", C.c_int), ("clear_tail", C.c_int), ("scale", C.c_float)]
+
+
+class Kv8EvictArgs(C.Structure):
+    _fields_ = [("weights", vp), ("weights_seq_stride", sz), ("weights_head_stride", sz), ("weights_capacity", sz),
+                ("dst_tables", vp), ("dst_table_stride", sz), ("keep", sz), ("recent", sz), ("new_lens", vp),
+                ("new_weights", vp), ("new_capacity", sz), ("kept", vp)]
+
+
+KV8_BF16, KV8_F16 = 0, 1
+KV8_BAD_BLOCK, KV8_BAD_LENGTH, KV8_BAD_ROWS = 1, 2, 4
+KV8_MAX_SEQS = 8192
+_sig("pf_kv8_record_bytes", sz, u32, u32, u32)
+_sig("pf_kv8_append", C.c_int, C.c_int, P(Kv8CacheDesc), P(Kv8Batch), vp, vp, C.c_int, sz, sz, sz, sz, sz, vp)
+_sig("pf_kv8_attention_workspace", C.c_int, C.c_int, P(Kv8CacheDesc), P(Kv8Batch), P(Kv8AttentionArgs), P(sz))
+_sig("pf_kv8_attention", C.c_int, C.c_int, P(Kv8CacheDesc), P(Kv8Batch), P(Kv8AttentionArgs), vp, sz, vp)
+_sig("pf_kv8_evict", C.c_int, C.c_int, P(Kv8CacheDesc), P(Kv8Batch), P(Kv8EvictArgs), vp)
+
+
 class PegaFlowError(Exception):
     """Base error of the bindings (python/src/lib.rs:65-72 of the reference)."""
 

@@ -394,6 +394,7 @@ class PegaWorkerConnector:
             raise RuntimeError("No KV cache layers were selected for registration")
         names, tensors, nb, bpb, kvs, segs = [], [], [], [], [], []
         for name, t in kv_caches.items():
+            t = getattr(t, "tensor", t)          # a Kv8Cache registers the tensor that it lies in
             info = infer_kv_cache_registration(t, self.block_size, is_mla=self.is_mla)
             self.registrations[name] = info
             names.append(name)

@@ -1,0 +1,786 @@
+// Attention over the KV cache held in 8 bits (pf_kv8_attention).
+//
+//   s[i, j] = scale * 2^eK(j) * q[i] . K8[j]        out[i] = sum_j p[i, j] * 2^eV(j) * V8[j],  p = exp(s - lse)
+//
+// Few query rows per KV head (single tokens, drafted tokens): the cache is read once and each byte is used for as many
+// products as there are rows, so HBM bounds it.  The tensor cores are still what makes it fit: 8 rows x 2 products x
+// 7 TB/s are more multiply-adds than the ordinary pipes have beside the conversions.
+//
+// The products are taken transposed, S^T = K Q^T and O^T = V^T P^T, as m16n8k16 f16 matrix instructions: 16 tokens (or
+// 16 head dimensions) are the rows, 8 query rows the columns.  K and V come straight from global memory into the
+// registers that the instruction wants, with no shared memory between: the order of the contracted index is free
+// as long as both operands share it, so a lane takes 16 consecutive bytes of a row and calls them what the
+// instruction's layout asks for.  Numbers:
+//   K8, V8   every e4m3 value is an f16 value: converted without rounding, products and sums in fp32
+//   q        scaled by a power of two for each row so that its largest element lies in [2^14, 2^15), then f16:
+//            exact for f16 q, and for bf16 q but for elements 2^-28 of the row's largest and below
+//   p        rounded to f16, 2^-11 / 2 relative, from fp32 scores; p is held as 2^(9 + s - ref) with a reference that
+//            follows the running maximum by steps of at least 2^6, so that f16's range is used from 2^-24 to 2^15
+//   scales   powers of two, applied to fp32 sums of one 16-token tile (a tile lies within one block)
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+
+#include "kv8.h"
+
+namespace pf {
+namespace {
+
+constexpr int kWarps = 4, kThreads = kWarps * 32;
+constexpr int kTile = 16;                   // tokens of one warp's step
+constexpr int kUnit = kTile * kWarps;       // tokens of one CTA's step, the granularity of the split
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kNone = -1e30f;             // reference of a row that has seen nothing
+constexpr float kShift = 9.f, kSlack = 6.f;
+
+struct AttnParams {
+  Kv8View cache;
+  Kv8Batch batch;
+  const uint16_t *q;
+  uint16_t *out;
+  float *lse;
+  float *weights;
+  int64_t q_row, q_head, out_row, out_head, w_seq, w_head;
+  int w_capacity;
+  int q_heads, group, max_query, row_tiles_most;
+  int causal, clear_tail, vec_q, vec_out;
+  float scale;
+  // partial results: slot 2 c + k of CTA c (k = 0: the segment that its range starts in, 1: the one that it ends in)
+  float *part_o;    // [slots][rows][dim]
+  float2 *part_ml;  // [slots][rows]
+  int n_ctas;
+};
+
+// The work of all sequences, heads and row tiles laid end to end in units of kUnit tokens; CTA c of n takes
+// [total c / n, total (c + 1) / n).  A segment is one (sequence, head, row tile).
+struct Split {
+  uint32_t total;
+  int n_ctas;       // at most total: every CTA that takes part has work
+  __device__ Split(uint32_t total, int n) : total(total), n_ctas((int)min((uint32_t)n, total)) {}
+  __device__ uint32_t begin(int c) const { return (uint32_t)((uint64_t)total * c / n_ctas); }
+  __device__ int owner(uint32_t u) const { return (int)((((uint64_t)u + 1) * n_ctas - 1) / total); }
+};
+
+template <int kRows>
+struct Seq {
+  int row0, rows, len, row_tiles;
+  uint32_t units;   // of one segment
+  __device__ Seq(const AttnParams &p, int s) {
+    int hi;
+    p.batch.rows(s, row0, hi);
+    rows = min(hi - row0, p.max_query);
+    len = p.batch.length(s, p.cache.block_log2);
+    row_tiles = (rows * p.group + kRows - 1) / kRows;
+    units = max(1, (len + kUnit - 1) / kUnit);
+  }
+  __device__ int visible(const AttnParams &p, int row) const {   // tokens that query row `row` (of rows * group) sees
+    const int i = row / p.group;
+    return p.causal ? min(max(len - rows + i + 1, 0), len) : len;
+  }
+};
+
+// prefix[s] = units before sequence s, prefix[n_seqs] = all of them.  Every CTA of every kernel computes it for
+// itself: lens stay on the device, and no launch and no workspace is spent on it.
+// kAllTiles: units of all row tiles; otherwise of one, for every sequence that has rows.
+template <int kRows, bool kAllTiles = true>
+__device__ void scan_units(const AttnParams &p, uint32_t *prefix) {
+  __shared__ uint32_t warp_sum[32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n_warps = blockDim.x >> 5;
+  uint32_t base = 0;
+  for (int s0 = 0; s0 < p.batch.n_seqs; s0 += blockDim.x) {
+    const int s = s0 + threadIdx.x;
+    uint32_t mine = 0;
+    if (s < p.batch.n_seqs) {
+      const Seq<kRows> seq(p, s);
+      mine = seq.units * (uint32_t)(p.cache.heads * (kAllTiles ? seq.row_tiles : min(seq.row_tiles, 1)));
+    }
+    uint32_t x = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const uint32_t y = __shfl_up_sync(0xffffffffu, x, d);
+      if (lane >= d) x += y;
+    }
+    if (lane == 31) warp_sum[warp] = x;
+    __syncthreads();
+    uint32_t before = base, all = 0;
+    for (int w = 0; w < n_warps; ++w) {
+      if (w < warp) before += warp_sum[w];
+      all += warp_sum[w];
+    }
+    if (s < p.batch.n_seqs) prefix[s] = before + x - mine;
+    base += all;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) prefix[p.batch.n_seqs] = base;
+  __syncthreads();
+}
+
+__device__ __forceinline__ int find_seq(const uint32_t *prefix, int n, uint32_t u) {   // last s with prefix[s] <= u
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (prefix[mid] <= u) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t d;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(x));
+  return d;
+}
+__device__ __forceinline__ uint32_t f16x2(float lo, float hi) {
+  uint32_t d;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+  return d;
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+  float d;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(d) : "f"(x));
+  return d;
+}
+template <bool kBf16>
+__device__ __forceinline__ float widen1(uint16_t x) {
+  return kBf16 ? __uint_as_float((uint32_t)x << 16) : __half2float(__ushort_as_half(x));
+}
+template <bool kBf16>
+__device__ __forceinline__ uint32_t narrow2(float lo, float hi) {
+  if (!kBf16) return f16x2(lo, hi);
+  uint32_t d;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+  return d;
+}
+
+// Query rows as the B operand of S^T = K Q^T, for rows row_first + n, n < 8 * kNt.  Lane (g, t) holds row g's elements
+// 64 x + 16 t .. + 15 for each x, in the order in which K's lanes hold theirs.  factor = scale * log2(e) over the
+// row's power of two, for columns 2 t and 2 t + 1 of each tile: score in log2 units = product * factor * scale of K.
+template <int kDim, int kNt, bool kBf16>
+struct Queries {
+  uint32_t b[kNt][kDim / 16][2];
+  float factor[kNt][2];
+
+  template <int kRows>
+  __device__ void load(const AttnParams &p, const Seq<kRows> &seq, int head, int row_first) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+#pragma unroll
+    for (int j = 0; j < kNt; ++j) {
+      const int row = row_first + 8 * j + g;
+      float x[kDim / 4];
+      const bool live = row < seq.rows * p.group;
+      const int i = live ? row / p.group : 0, qh = head * p.group + (live ? row % p.group : 0);
+      const uint16_t *src = p.q + (int64_t)(seq.row0 + i) * p.q_row + qh * p.q_head + 16 * t;
+      float top = 0.f;
+#pragma unroll
+      for (int k = 0; k < kDim / 4; k += 8) {
+        const uint16_t *at = src + 64 * (k / 16) + k % 16;
+        uint4 w = make_uint4(0, 0, 0, 0);
+        if (live) {
+          if (p.vec_q) w = *reinterpret_cast<const uint4 *>(at);
+          else w = make_uint4(at[0] | at[1] << 16, at[2] | at[3] << 16, at[4] | at[5] << 16, at[6] | at[7] << 16);
+        }
+        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+          x[k + 2 * m] = widen1<kBf16>((uint16_t)u[m]);
+          x[k + 2 * m + 1] = widen1<kBf16>((uint16_t)(u[m] >> 16));
+          top = fmaxf(top, fmaxf(fabsf(x[k + 2 * m]), fabsf(x[k + 2 * m + 1])));
+        }
+      }
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      // 2^-e brings the row's largest element into [2^14, 2^15); a row of zeros or with an infinity stays as it is
+      int e = (int)(__float_as_uint(top) >> 23) - 127 - 14;
+      if (top == 0.f || top > 3.4e38f) e = 0;
+      e = max(e, -126);
+      const float down = exp2i(-e);
+#pragma unroll
+      for (int m = 0; m < kDim / 16; ++m) {
+        b[j][m][0] = f16x2(x[4 * m] * down, x[4 * m + 1] * down);
+        b[j][m][1] = f16x2(x[4 * m + 2] * down, x[4 * m + 3] * down);
+      }
+      const float mine = p.scale * kLog2e * exp2i(e);
+      factor[j][0] = __shfl_sync(0xffffffffu, mine, (2 * t) * 4);
+      factor[j][1] = __shfl_sync(0xffffffffu, mine, (2 * t + 1) * 4);
+    }
+  }
+};
+
+// One 16-token tile of K: lane (g, t) holds rows g and g + 8, bytes 64 x + 16 t .. + 15.
+template <int kDim>
+struct KTile {
+  uint4 w[kDim / 64][2];
+  __device__ void load(const uint8_t *tile, int row0) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const uint8_t *at = tile + (row0 + g) * kDim + 16 * t;
+#pragma unroll
+    for (int x = 0; x < kDim / 64; ++x) {
+      w[x][0] = __ldg(reinterpret_cast<const uint4 *>(at + 64 * x));
+      w[x][1] = __ldg(reinterpret_cast<const uint4 *>(at + 64 * x + 8 * kDim));
+    }
+  }
+  // c += K Q^T: c[0], c[1] = token g, columns 2 t, 2 t + 1; c[2], c[3] = token g + 8
+  template <int kNt, bool kBf16>
+  __device__ void products(const Queries<kDim, kNt, kBf16> &q, float (&c)[kNt][4]) const {
+#pragma unroll
+    for (int x = 0; x < kDim / 64; ++x) {
+      const uint32_t lo[4] = {w[x][0].x, w[x][0].y, w[x][0].z, w[x][0].w};
+      const uint32_t hi[4] = {w[x][1].x, w[x][1].y, w[x][1].z, w[x][1].w};
+#pragma unroll
+      for (int m = 0; m < 4; ++m) {
+        const uint32_t a0 = f16x2_from_e4m3<0>(lo[m]), a1 = f16x2_from_e4m3<0>(hi[m]);
+        const uint32_t a2 = f16x2_from_e4m3<1>(lo[m]), a3 = f16x2_from_e4m3<1>(hi[m]);
+#pragma unroll
+        for (int j = 0; j < kNt; ++j) mma_f16(c[j], a0, a1, a2, a3, q.b[j][4 * x + m][0], q.b[j][4 * x + m][1]);
+      }
+    }
+  }
+};
+
+// One 16-token tile of V: lane (g, t) holds tokens 2 t, 2 t + 1, 2 t + 8, 2 t + 9, bytes (kDim / 8) g .. + kDim / 8 - 1.
+template <int kDim>
+struct VTile {
+  static constexpr int kWords = kDim / 32;   // 4-byte words of one token
+  uint32_t w[4][kWords];
+  __device__ void load(const uint8_t *tile, int row0) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const uint8_t *at = tile + (row0 + 2 * t) * kDim + g * (kDim / 8);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint8_t *row = at + ((i & 1) + 8 * (i >> 1)) * kDim;
+      if constexpr (kWords == 2) {
+        const uint2 v = __ldg(reinterpret_cast<const uint2 *>(row));
+        w[i][0] = v.x, w[i][1] = v.y;
+      } else {
+#pragma unroll
+        for (int x = 0; x < kWords / 4; ++x) {
+          const uint4 v = __ldg(reinterpret_cast<const uint4 *>(row) + x);
+          w[i][4 * x] = v.x, w[i][4 * x + 1] = v.y, w[i][4 * x + 2] = v.z, w[i][4 * x + 3] = v.w;
+        }
+      }
+    }
+  }
+  __device__ bool has_nan() const {   // a byte 0x7f or 0xff
+    bool any = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int x = 0; x < kWords; ++x) any |= __vcmpeq4(w[i][x] & 0x7f7f7f7fu, 0x7f7f7f7fu) != 0;
+    return any;
+  }
+};
+
+// Rows of the score tile that lie behind the visible tokens hold what the block held before: a NaN there would
+// survive a product with p = 0.  Called for a sequence's last tile only.
+template <int kDim>
+__device__ __forceinline__ void clear_behind(VTile<kDim> &v, int first_hidden) {
+  const int t = threadIdx.x & 3;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (2 * t + (i & 1) + 8 * (i >> 1) >= first_hidden)
+#pragma unroll
+      for (int x = 0; x < VTile<kDim>::kWords; ++x) v.w[i][x] = 0;
+}
+
+// A NaN in V reaches the rows that see its token, and no other: 0 * NaN would.  Called for tiles that some row sees in part
+// and that hold a NaN: marks the outputs of the rows that see it and takes it out of the tile.
+template <int kDim, int kNt>
+__device__ __noinline__ void spread_nan(VTile<kDim> &v, float (&o)[kNt][kDim / 16][4], const int (&see)[kNt][2], int tok) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    for (int from = 0; from < 4; ++from) {
+      const int token = tok + 2 * from + (i & 1) + 8 * (i >> 1);
+#pragma unroll
+      for (int x = 0; x < VTile<kDim>::kWords; ++x) {
+        const uint32_t w = __shfl_sync(0xffffffffu, v.w[i][x], (lane & ~3) | from);
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+          if (((w >> (8 * b)) & 0x7f) == 0x7f)
+#pragma unroll
+            for (int j = 0; j < kNt; ++j)
+#pragma unroll
+              for (int k = 0; k < 2; ++k)
+                if (token < see[j][k]) o[j][2 * x + b / 2][k + 2 * (b & 1)] = __int_as_float(0x7fffffff);
+      }
+    }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int x = 0; x < VTile<kDim>::kWords; ++x)
+#pragma unroll
+      for (int b = 0; b < 4; ++b)
+        if (((v.w[i][x] >> (8 * b)) & 0x7f) == 0x7f) v.w[i][x] &= ~(0xffu << (8 * b));
+}
+
+// Where a tile of a sequence lies: nothing for one whose block id is not in the cache.
+struct TileAt {
+  const uint8_t *k, *v;
+  float k_scale, v_scale;
+  int row0;
+};
+
+template <bool kWithV>
+__device__ __forceinline__ bool locate(const AttnParams &p, int s, int head, int tok, TileAt &at) {
+  uint32_t id;
+  if (!p.batch.block(p.cache, s, tok >> p.cache.block_log2, id)) {
+    p.batch.report(PF_KV8_BAD_BLOCK);
+    at.k_scale = at.v_scale = 0.f;
+    return false;
+  }
+  at.row0 = tok & (p.cache.block_size() - 1);
+  at.k = p.cache.tile(0, id, head);
+  at.k_scale = __ldg(p.cache.scale(0, id, head));
+  if (kWithV) {
+    at.v = p.cache.tile(1, id, head);
+    at.v_scale = __ldg(p.cache.scale(1, id, head));
+  }
+  return true;
+}
+
+// CTAs that an SM holds: what the registers allow (128 of them at 128 dimensions and 8 rows).
+constexpr int ctas_of(int dim, int nt) { return dim == 256 ? 2 : dim == 128 ? (nt == 1 ? 4 : 2) : (nt == 1 ? 5 : 4); }
+
+template <int kDim, int kNt, bool kBf16>
+__global__ void __launch_bounds__(kThreads, ctas_of(kDim, kNt)) kv8_attention_rows(AttnParams p) {
+  constexpr int kRows = 8 * kNt, kMt = kDim / 16;
+  extern __shared__ __align__(16) char smem[];
+  float *sh_o = reinterpret_cast<float *>(smem);                       // [kWarps][kRows][kDim]
+  float2 *sh_ml = reinterpret_cast<float2 *>(sh_o + kWarps * kRows * kDim);   // [kWarps][kRows]
+  uint32_t *prefix = reinterpret_cast<uint32_t *>(sh_ml + kWarps * kRows);    // [n_seqs + 1]
+  scan_units<kRows>(p, prefix);
+  const int n_seqs = p.batch.n_seqs, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const Split split{prefix[n_seqs], p.n_ctas};
+  if (blockIdx.x == 0) {
+    if (p.batch.starts) p.batch.check_starts(p.max_query);
+    for (int s = threadIdx.x; s < n_seqs; s += kThreads)
+      if (p.batch.lens[s] < 0 || p.batch.lens[s] > p.batch.length(s, p.cache.block_log2)) p.batch.report(PF_KV8_BAD_LENGTH);
+  }
+  if ((int)blockIdx.x >= split.n_ctas) return;
+  uint32_t u = split.begin(blockIdx.x);
+  const uint32_t u_end = split.begin(blockIdx.x + 1);
+  bool first_segment = true;
+  while (u < u_end) {
+    const int s = find_seq(prefix, n_seqs, u);
+    const Seq<kRows> seq(p, s);
+    const uint32_t in_seq = u - prefix[s], segment = in_seq / seq.units, unit0 = in_seq % seq.units;
+    const int head = segment / seq.row_tiles, rt = segment % seq.row_tiles, row_first = rt * kRows;
+    const uint32_t units = min(seq.units - unit0, u_end - u);
+    const int live_rows = min(seq.rows * p.group - row_first, kRows);
+    const int most = seq.visible(p, row_first + live_rows - 1);         // tokens that any row of the tile sees
+    const int least = seq.visible(p, row_first);                        // tokens that all rows see
+    int see[kNt][2];
+#pragma unroll
+    for (int j = 0; j < kNt; ++j)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) see[j][k] = seq.visible(p, min(row_first + 8 * j + 2 * t + k, seq.rows * p.group - 1));
+
+    Queries<kDim, kNt, kBf16> q;
+    q.load(p, seq, head, row_first);
+    float o[kNt][kMt][4], ref[kNt][2], sum[kNt][2];
+#pragma unroll
+    for (int j = 0; j < kNt; ++j) {
+#pragma unroll
+      for (int m = 0; m < kMt; ++m) o[j][m][0] = o[j][m][1] = o[j][m][2] = o[j][m][3] = 0.f;
+      ref[j][0] = ref[j][1] = kNone;
+      sum[j][0] = sum[j][1] = 0.f;
+    }
+    const int tok_end = (int)min((int64_t)(unit0 + units) * kUnit, (int64_t)most);
+    for (int tok = (int)(unit0 * kUnit) + warp * kTile; tok < tok_end; tok += kUnit) {
+      TileAt at;
+      KTile<kDim> kt;
+      VTile<kDim> vt;
+      const bool there = locate<true>(p, s, head, tok, at);
+      if (!there) continue;
+      kt.load(at.k, at.row0);
+      vt.load(at.v, at.row0);
+      if (tok + kTile > seq.len) clear_behind(vt, seq.len - tok);
+      if (tok + kTile > least && __any_sync(0xffffffffu, vt.has_nan())) spread_nan<kDim, kNt>(vt, o, see, tok);
+      float c[kNt][4];
+#pragma unroll
+      for (int j = 0; j < kNt; ++j) c[j][0] = c[j][1] = c[j][2] = c[j][3] = 0.f;
+      kt.products(q, c);
+      bool over = false;
+#pragma unroll
+      for (int j = 0; j < kNt; ++j)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const float f = q.factor[j][k] * at.k_scale;
+          c[j][k] *= f;
+          c[j][k + 2] *= f;
+        }
+      if (tok + kTile > least) {
+#pragma unroll
+        for (int j = 0; j < kNt; ++j)
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            if (tok + g >= see[j][k]) c[j][k] = -INFINITY;
+            if (tok + g + 8 >= see[j][k]) c[j][k + 2] = -INFINITY;
+          }
+      }
+#pragma unroll
+      for (int j = 0; j < kNt; ++j)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) over |= fmaxf(c[j][k], c[j][k + 2]) > ref[j][k] + kSlack;
+      if (__any_sync(0xffffffffu, over)) {
+#pragma unroll
+        for (int j = 0; j < kNt; ++j)
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            float top = fmaxf(c[j][k], c[j][k + 2]);
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+            const float now = fmaxf(ref[j][k], top), r = exp2_fast(ref[j][k] - now);
+            ref[j][k] = now;
+            sum[j][k] *= r;
+#pragma unroll
+            for (int m = 0; m < kMt; ++m) {
+              o[j][m][k] *= r;
+              o[j][m][k + 2] *= r;
+            }
+          }
+      }
+      uint32_t pb[kNt][2];
+#pragma unroll
+      for (int j = 0; j < kNt; ++j) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) c[j][k] = exp2_fast(c[j][k] - (ref[j][k & 1] - kShift));
+        sum[j][0] += c[j][0] + c[j][2];
+        sum[j][1] += c[j][1] + c[j][3];
+        pb[j][0] = transpose8x8(f16x2(c[j][0], c[j][1]));
+        pb[j][1] = transpose8x8(f16x2(c[j][2], c[j][3]));
+      }
+#pragma unroll
+      for (int w = 0; w < VTile<kDim>::kWords; ++w) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const uint32_t sel = half ? 0x7362 : 0x5140;
+          const uint32_t ab = __byte_perm(vt.w[0][w], vt.w[1][w], sel), ce = __byte_perm(vt.w[2][w], vt.w[3][w], sel);
+          const uint32_t a0 = f16x2_from_e4m3<0>(ab), a1 = f16x2_from_e4m3<1>(ab);
+          const uint32_t a2 = f16x2_from_e4m3<0>(ce), a3 = f16x2_from_e4m3<1>(ce);
+#pragma unroll
+          for (int j = 0; j < kNt; ++j) {
+            float d[4] = {0.f, 0.f, 0.f, 0.f};
+            mma_f16(d, a0, a1, a2, a3, pb[j][0], pb[j][1]);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) o[j][2 * w + half][k] += at.v_scale * d[k];
+          }
+        }
+      }
+    }
+    // join the four warps
+#pragma unroll
+    for (int j = 0; j < kNt; ++j)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) sum[j][k] += __shfl_xor_sync(0xffffffffu, sum[j][k], d);
+        if (g == 0) sh_ml[warp * kRows + 8 * j + 2 * t + k] = make_float2(ref[j][k], sum[j][k]);
+      }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kNt; ++j)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int n = 8 * j + 2 * t + k;
+        float top = kNone;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sh_ml[w * kRows + n].x);
+        const float r = exp2_fast(ref[j][k] - top);
+        float *dst = sh_o + (warp * kRows + n) * kDim + g * (kDim / 8);
+#pragma unroll
+        for (int m = 0; m < kMt; m += 2)
+          *reinterpret_cast<float4 *>(dst + 2 * m) =
+              make_float4(o[j][m][k] * r, o[j][m][k + 2] * r, o[j][m + 1][k] * r, o[j][m + 1][k + 2] * r);
+      }
+    __syncthreads();
+    const bool whole = unit0 == 0 && units == seq.units;
+    const int slot = 2 * blockIdx.x + (first_segment ? 0 : 1);
+    for (int e = threadIdx.x; e < live_rows * (kDim / 4); e += kThreads) {
+      const int n = e / (kDim / 4), d = e % (kDim / 4) * 4;
+      float top = kNone, l = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sh_ml[w * kRows + n].x);
+      float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float2 ml = sh_ml[w * kRows + n];
+        l += ml.y * exp2_fast(ml.x - top);
+        const float4 x = *reinterpret_cast<const float4 *>(sh_o + (w * kRows + n) * kDim + d);
+        a.x += x.x, a.y += x.y, a.z += x.z, a.w += x.w;
+      }
+      if (whole) {
+        const int row = row_first + n, i = row / p.group, qh = head * p.group + row % p.group;
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        uint16_t *dst = p.out + (int64_t)(seq.row0 + i) * p.out_row + qh * p.out_head + d;
+        const uint32_t x = narrow2<kBf16>(a.x * inv, a.y * inv), y = narrow2<kBf16>(a.z * inv, a.w * inv);
+        if (p.vec_out) *reinterpret_cast<uint2 *>(dst) = make_uint2(x, y);
+        else dst[0] = (uint16_t)x, dst[1] = x >> 16, dst[2] = (uint16_t)y, dst[3] = y >> 16;
+        if (d == 0 && p.lse) p.lse[(int64_t)(seq.row0 + i) * p.q_heads + qh] = l == 0.f ? -INFINITY : (top - kShift + log2f(l)) * kLn2;
+      } else {
+        *reinterpret_cast<float4 *>(p.part_o + ((int64_t)slot * kRows + n) * kDim + d) = a;
+        if (d == 0) p.part_ml[slot * kRows + n] = make_float2(top, l);
+      }
+    }
+    __syncthreads();
+    u += units;
+    first_segment = false;
+  }
+}
+
+// Joins the parts of segments that several CTAs shared, one CTA for each (segment, row), in the order of the tokens.
+// kSpan threads hold one part's row as float4, kThreads / kSpan parts are read at a time.
+template <int kDim, int kNt, bool kBf16>
+__global__ void __launch_bounds__(kThreads) kv8_attention_join(AttnParams p) {
+  constexpr int kRows = 8 * kNt, kSpan = kDim / 4, kAtOnce = kThreads / kSpan;
+  extern __shared__ __align__(16) char smem[];
+  uint32_t *prefix = reinterpret_cast<uint32_t *>(smem);
+  __shared__ float4 sh_a[kThreads];
+  __shared__ float sh_l[kAtOnce];
+  scan_units<kRows>(p, prefix);
+  const int n_seqs = p.batch.n_seqs;
+  if (p.clear_tail) {
+    int lo, hi = 0;
+    if (n_seqs) p.batch.rows(n_seqs - 1, lo, hi);
+    for (int64_t e = (int64_t)hi * p.q_heads * kDim + blockIdx.x * kThreads + threadIdx.x;
+         e < (int64_t)p.batch.n_rows * p.q_heads * kDim; e += (int64_t)gridDim.x * kThreads) {
+      const int64_t row = e / (p.q_heads * kDim);
+      const int qh = (int)(e / kDim % p.q_heads), d = (int)(e % kDim);
+      p.out[row * p.out_row + qh * p.out_head + d] = 0;
+      if (d == 0 && p.lse) p.lse[row * p.q_heads + qh] = -INFINITY;
+    }
+  }
+  const Split split{prefix[n_seqs], p.n_ctas};
+  const int n = blockIdx.x % kRows, rt = blockIdx.x / kRows % p.row_tiles_most;
+  const int rest = blockIdx.x / kRows / p.row_tiles_most, head = rest % p.cache.heads, s = rest / p.cache.heads;
+  if (s >= n_seqs) return;
+  const Seq<kRows> seq(p, s);
+  const int row = rt * kRows + n;
+  if (row >= seq.rows * p.group) return;
+  const uint32_t u0 = prefix[s] + (uint32_t)(head * seq.row_tiles + rt) * seq.units, u1 = u0 + seq.units;
+  const int c0 = split.owner(u0), c1 = split.owner(u1 - 1);
+  if (c0 == c1) return;
+  const int part = threadIdx.x / kSpan, d = threadIdx.x % kSpan * 4;
+  float top = kNone;
+  for (int c = c0; c <= c1; ++c) top = fmaxf(top, p.part_ml[(2 * c + (c == c0 && split.begin(c) < u0 ? 1 : 0)) * kRows + n].x);
+  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+  float l = 0.f;
+  for (int c = c0 + part; c <= c1; c += kAtOnce) {
+    const int slot = 2 * c + (c == c0 && split.begin(c) < u0 ? 1 : 0);
+    const float2 ml = p.part_ml[slot * kRows + n];
+    const float r = exp2_fast(ml.x - top);
+    const float4 x = *reinterpret_cast<const float4 *>(p.part_o + ((int64_t)slot * kRows + n) * kDim + d);
+    l += ml.y * r;
+    a.x += x.x * r, a.y += x.y * r, a.z += x.z * r, a.w += x.w * r;
+  }
+  sh_a[threadIdx.x] = a;
+  if (d == 0) sh_l[part] = l;
+  __syncthreads();
+  if (part) return;
+  for (int k = 1; k < kAtOnce; ++k) {
+    const float4 x = sh_a[k * kSpan + threadIdx.x];
+    a.x += x.x, a.y += x.y, a.z += x.z, a.w += x.w;
+    l += sh_l[k];
+  }
+  const int i = row / p.group, qh = head * p.group + row % p.group;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  uint16_t *dst = p.out + (int64_t)(seq.row0 + i) * p.out_row + qh * p.out_head + d;
+  const uint32_t x = narrow2<kBf16>(a.x * inv, a.y * inv), y = narrow2<kBf16>(a.z * inv, a.w * inv);
+  dst[0] = (uint16_t)x, dst[1] = x >> 16, dst[2] = (uint16_t)y, dst[3] = y >> 16;
+  if (d == 0 && p.lse) p.lse[(int64_t)(seq.row0 + i) * p.q_heads + qh] = l == 0.f ? -INFINITY : (top - kShift + log2f(l)) * kLn2;
+}
+
+// weights[s, head, j] += sum over rows and group heads of exp(score - lse), once lse is known: the scores are taken
+// again, a warp for each 16-token tile with K in registers and the row tiles passing by.  Each element has one writer.
+template <int kDim, bool kBf16>
+__global__ void __launch_bounds__(kThreads) kv8_attention_weights(AttnParams p) {
+  constexpr int kRows = 8;
+  extern __shared__ __align__(16) char smem[];
+  uint32_t *prefix = reinterpret_cast<uint32_t *>(smem);
+  scan_units<kRows, false>(p, prefix);
+  const int n_seqs = p.batch.n_seqs, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  if (blockIdx.x == 0)
+    for (int s = threadIdx.x; s < n_seqs; s += kThreads)
+      if (p.batch.lens[s] > p.w_capacity) p.batch.report(PF_KV8_BAD_LENGTH);
+  for (uint32_t u = blockIdx.x; u < prefix[n_seqs]; u += gridDim.x) {
+    const int s = find_seq(prefix, n_seqs, u);
+    const Seq<kRows> seq(p, s);
+    const int head = (u - prefix[s]) / seq.units, tok = (u - prefix[s]) % seq.units * kUnit + warp * kTile;
+    const int end = min(seq.len, p.w_capacity);
+    if (tok >= end) continue;
+    TileAt at;
+    if (!locate<false>(p, s, head, tok, at)) continue;
+    KTile<kDim> kt;
+    kt.load(at.k, at.row0);
+    float w0 = 0.f, w1 = 0.f;
+    for (int row_first = 0; row_first < seq.rows * p.group; row_first += kRows) {
+      if (seq.visible(p, min(row_first + kRows, seq.rows * p.group) - 1) <= tok) continue;
+      Queries<kDim, 1, kBf16> q;
+      q.load(p, seq, head, row_first);
+      float c[1][4] = {{0.f, 0.f, 0.f, 0.f}};
+      kt.products(q, c);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int row = row_first + 2 * t + k;
+        if (row < seq.rows * p.group) {
+          const int i = row / p.group, qh = head * p.group + row % p.group, see = seq.visible(p, row);
+          const float f = q.factor[0][k] * at.k_scale;
+          const float base = __ldg(p.lse + (int64_t)(seq.row0 + i) * p.q_heads + qh) * kLog2e;
+          if (tok + g < see) w0 += exp2_fast(c[0][k] * f - base);
+          if (tok + g + 8 < see) w1 += exp2_fast(c[0][k + 2] * f - base);
+        }
+      }
+    }
+#pragma unroll
+    for (int d = 1; d < 4; d <<= 1) {
+      w0 += __shfl_xor_sync(0xffffffffu, w0, d);
+      w1 += __shfl_xor_sync(0xffffffffu, w1, d);
+    }
+    if (t == 0) {
+      float *dst = p.weights + s * p.w_seq + head * p.w_head + tok + g;
+      if (tok + g < end) dst[0] += w0;
+      if (tok + g + 8 < end) dst[8] += w1;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------- host
+struct Plan {
+  int nt, n_ctas;
+  size_t part_o, part_ml, lse, bytes;   // offsets in the workspace
+};
+
+size_t up256(size_t n) { return (n + 255) / 256 * 256; }
+
+Plan make_plan(int device_id, const Kv8View &c, const pf_kv8_attention_args &a) {
+  const size_t group = a.q_heads / c.heads;
+  Plan plan{};
+  const size_t rows = std::min(a.max_query, a.n_rows) * group;
+  plan.nt = rows <= 8 || c.dim == 256 ? 1 : 2;
+  const int ctas_per_sm = ctas_of(c.dim, plan.nt);
+  plan.n_ctas = kv8_sm_count(device_id) * ctas_per_sm;
+  const size_t slots = 2 * (size_t)plan.n_ctas * 8 * plan.nt;
+  plan.part_o = 0;
+  plan.part_ml = up256(slots * c.dim * 4);
+  plan.lse = plan.part_ml + up256(slots * 8);
+  plan.bytes = plan.lse + (a.weights && !a.lse ? up256(a.n_rows * a.q_heads * 4) : 0);
+  return plan;
+}
+
+void check_args(const pf_kv8_attention_args *a, const Kv8View &c, const Kv8Batch &b) {
+  if (!a) throw Error::invalid("null attention arguments");
+  if (a->dtype != PF_KV8_BF16 && a->dtype != PF_KV8_F16) throw Error::invalid(strf("unknown dtype %d", a->dtype));
+  if (a->q_heads == 0 || a->q_heads % c.heads || a->q_heads > 65536)
+    throw Error::invalid(strf("%u query heads are not a multiple of %d KV heads", a->q_heads, c.heads));
+  if (a->n_rows && b.n_seqs && a->max_query == 0) throw Error::invalid("max_query must not be 0");
+  const uint64_t rows_of_group = (uint64_t)std::min<size_t>(a->max_query, a->n_rows) * (a->q_heads / c.heads);
+  if (rows_of_group > 0x3fffffffu) throw Error::invalid("too many query rows");
+  if (!b.starts && b.n_seqs && a->max_query < (size_t)b.rows_each)
+    throw Error::invalid(strf("max_query=%zu is below the %d rows of each sequence", a->max_query, b.rows_each));
+  // units are counted in 32 bits: (segments) x (units of a segment), summed over the sequences
+  const uint64_t units = ((uint64_t)b.max_blocks << c.block_log2) / kUnit + 1;
+  const uint64_t tiles = ((uint64_t)a->n_rows * (a->q_heads / c.heads) + 7) / 8 + b.n_seqs;
+  if (units * tiles > 0xffffffffull / c.heads) throw Error::invalid("too many query rows for tables of this width: split the call");
+  if ((rows_of_group + 15) * c.heads * std::max(b.n_seqs, 1) > 0x7fffffffull)
+    throw Error::invalid("too many query rows for so many sequences: split the call");
+}
+
+template <int kDim, int kNt, bool kBf16>
+void launch(const AttnParams &p, cudaStream_t stream) {
+  const size_t scan = ((size_t)p.batch.n_seqs + 1) * 4;
+  const size_t smem = kWarps * 8 * kNt * (kDim * 4 + 8) + scan;
+  auto kernel = kv8_attention_rows<kDim, kNt, kBf16>;
+  if (smem > 48 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+    throw Error::storage("cudaFuncSetAttribute failed");
+  if (p.batch.n_seqs) {
+    kernel<<<p.n_ctas, kThreads, smem, stream>>>(p);
+    PF_KV8_LAUNCHED();
+  }
+  const size_t join = std::max<size_t>(1, (size_t)p.batch.n_seqs * p.cache.heads * p.row_tiles_most * 8 * kNt);
+  kv8_attention_join<kDim, kNt, kBf16><<<(unsigned)join, kThreads, scan, stream>>>(p);
+  PF_KV8_LAUNCHED();
+  if (p.weights) {
+    kv8_attention_weights<kDim, kBf16><<<p.n_ctas, kThreads, scan, stream>>>(p);
+    PF_KV8_LAUNCHED();
+  }
+}
+
+template <bool kBf16>
+void launch(const AttnParams &p, int nt, cudaStream_t stream) {
+  if (p.cache.dim == 64) nt == 1 ? launch<64, 1, kBf16>(p, stream) : launch<64, 2, kBf16>(p, stream);
+  else if (p.cache.dim == 128) nt == 1 ? launch<128, 1, kBf16>(p, stream) : launch<128, 2, kBf16>(p, stream);
+  else launch<256, 1, kBf16>(p, stream);
+}
+
+}  // namespace
+}  // namespace pf
+
+using namespace pf;
+
+extern "C" {
+
+int pf_kv8_attention_workspace(int device_id, const pf_kv8_cache *cache, const pf_kv8_batch *batch,
+                               const pf_kv8_attention_args *args, size_t *bytes) {
+  return guarded([&] {
+    if (!bytes) throw Error::invalid("bytes is null");
+    if (!args) throw Error::invalid("null attention arguments");
+    const Kv8View c = kv8_check_cache(cache);
+    const Kv8Batch b = kv8_check_batch(batch, args->n_rows);
+    check_args(args, c, b);
+    *bytes = make_plan(device_id, c, *args).bytes;
+  });
+}
+
+int pf_kv8_attention(int device_id, const pf_kv8_cache *cache, const pf_kv8_batch *batch,
+                     const pf_kv8_attention_args *args, void *workspace, size_t workspace_bytes, void *stream) {
+  return guarded([&] {
+    if (!args) throw Error::invalid("null attention arguments");
+    const Kv8View c = kv8_check_cache(cache);
+    const Kv8Batch b = kv8_check_batch(batch, args->n_rows);
+    const pf_kv8_attention_args &a = *args;
+    check_args(args, c, b);
+    if (a.n_rows == 0 || (b.n_seqs == 0 && !a.clear_tail)) return;
+    if (!a.q || !a.out) throw Error::invalid("null q or out");
+    if ((uintptr_t)a.q % 2 || (uintptr_t)a.out % 2) throw Error::invalid("q and out must be aligned to their elements");
+    const Plan plan = make_plan(device_id, c, a);
+    if (!workspace || workspace_bytes < plan.bytes)
+      throw Error::invalid(strf("workspace of %zu bytes, the call needs %zu", workspace ? workspace_bytes : 0, plan.bytes));
+    if ((uintptr_t)workspace % 256) throw Error::invalid("the workspace must be 256-byte aligned");
+    AttnParams p{};
+    p.cache = c;
+    p.batch = b;
+    p.q = (const uint16_t *)a.q;
+    p.out = (uint16_t *)a.out;
+    char *ws = (char *)workspace;
+    p.part_o = (float *)(ws + plan.part_o);
+    p.part_ml = (float2 *)(ws + plan.part_ml);
+    p.lse = a.lse ? a.lse : a.weights ? (float *)(ws + plan.lse) : nullptr;
+    p.weights = a.weights;
+    p.q_row = (int64_t)a.q_row_stride, p.q_head = (int64_t)a.q_head_stride;
+    p.out_row = (int64_t)a.out_row_stride, p.out_head = (int64_t)a.out_head_stride;
+    p.w_seq = (int64_t)a.weights_seq_stride, p.w_head = (int64_t)a.weights_head_stride;
+    p.w_capacity = (int)std::min<size_t>(a.weights_capacity, 0x7fffffff);
+    p.q_heads = (int)a.q_heads;
+    p.group = (int)a.q_heads / c.heads;
+    p.max_query = (int)std::min<size_t>(a.max_query, a.n_rows);
+    p.row_tiles_most = (p.max_query * p.group + 8 * plan.nt - 1) / (8 * plan.nt);
+    p.causal = a.causal != 0;
+    p.clear_tail = a.clear_tail != 0;
+    p.vec_q = (uintptr_t)a.q % 16 == 0 && (a.q_row_stride | a.q_head_stride) % 8 == 0;
+    p.vec_out = (uintptr_t)a.out % 8 == 0 && (a.out_row_stride | a.out_head_stride) % 4 == 0;
+    p.scale = a.scale;
+    p.n_ctas = plan.n_ctas;
+    DeviceGuard on_device(device_id);
+    if (a.dtype == PF_KV8_BF16) launch<true>(p, plan.nt, (cudaStream_t)stream);
+    else launch<false>(p, plan.nt, (cudaStream_t)stream);
+  });
+}
+
+}  // extern "C"

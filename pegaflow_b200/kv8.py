@@ -1,0 +1,261 @@
+"""KV cache of one layer held in 8 bits: write, attention, eviction by accumulated attention weight.
+
+``Kv8Cache.tensor`` is a uint8 tensor ``[2 (K, V), num_blocks, record]``; a record holds ``kv_heads x block_size x
+head_dim`` e4m3 values and one power-of-two fp32 scale for each head (include/pegaflow_b200.h, section 5).  It registers
+like any KV tensor whose first dimension is 2 (``PegaWorkerConnector.register_kv_caches({name: cache.tensor})``, or the
+cache itself), so that saves, loads and peer copies move half the bytes of a 16-bit cache and a block's
+scales travel with it.
+
+The calls only enqueue work, on the current torch stream of the cache's device unless ``stream`` (a cudaStream_t value)
+says otherwise, and may be captured into a CUDA graph.  Block tables, lengths and row starts are int32 tensors on
+the device.  What the host cannot check (block ids, lengths, row starts) the kernels check: they leave the access out and
+set a bit that ``check()`` raises for.  None of the calls has a backward pass.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from typing import Optional, Tuple
+
+import torch
+
+from . import _native as N
+
+_DTYPES = {torch.bfloat16: N.KV8_BF16, torch.float16: N.KV8_F16}
+_byref = C.byref
+
+
+def _refuse(text: str):
+    raise N.PegaflowInvalidArgument(3, "invalid argument: " + text)
+
+
+class Kv8Cache:
+    def __init__(self, num_blocks: int, block_size: int, kv_heads: int, head_dim: int, device="cuda"):
+        """A cache of zeros.  block_size 16, 32, 64 or 128 tokens, head_dim 64, 128 or 256."""
+        record = self.record_bytes(block_size, kv_heads, head_dim)
+        self._bind(torch.zeros((2, num_blocks, record), dtype=torch.uint8, device=device), block_size, kv_heads, head_dim)
+
+    @classmethod
+    def from_tensor(cls, tensor, block_size: int, kv_heads: int, head_dim: int) -> "Kv8Cache":
+        """The cache in an existing uint8 tensor [2, num_blocks, >= record bytes] on a GPU: dense records, at any
+        strides that are multiples of 16 bytes (a slice of a buffer that holds several layers, for example)."""
+        self = cls.__new__(cls)
+        self._bind(tensor, block_size, kv_heads, head_dim)
+        return self
+
+    @staticmethod
+    def record_bytes(block_size: int, kv_heads: int, head_dim: int) -> int:
+        """Bytes of one block of K or of V with its scales."""
+        ok = all(isinstance(x, int) and 0 < x < 1 << 31 for x in (block_size, kv_heads, head_dim))
+        n = N.lib.pf_kv8_record_bytes(block_size, kv_heads, head_dim) if ok else 0
+        if not n:
+            _refuse(f"8-bit cache: unsupported geometry block_size={block_size} kv_heads={kv_heads} head_dim={head_dim} "
+                    "(block_size 16, 32, 64 or 128; kv_heads 1 to 1024; head_dim 64, 128 or 256)")
+        return n
+
+    def _bind(self, t, block_size, kv_heads, head_dim):
+        record = self.record_bytes(block_size, kv_heads, head_dim)
+        if t.dtype != torch.uint8 or t.dim() != 3 or t.shape[0] != 2 or t.shape[2] < record or t.shape[1] == 0:
+            _refuse(f"8-bit cache: a uint8 tensor [2, num_blocks, {record}] is needed, not {t.dtype} {tuple(t.shape)}")
+        if not t.is_cuda:
+            _refuse(f"8-bit cache: the tensor is on {t.device}, not on a GPU")
+        if t.stride(2) != 1 or t.stride(0) < record or (t.shape[1] > 1 and t.stride(1) < record):
+            _refuse(f"8-bit cache: records of {record} bytes do not fit the strides {t.stride()}")
+        if t.data_ptr() % 16 or t.stride(0) % 16 or (t.shape[1] > 1 and t.stride(1) % 16):
+            _refuse("8-bit cache: address and strides must be multiples of 16 bytes")
+        self.tensor = t
+        self.block_size, self.kv_heads, self.head_dim = block_size, kv_heads, head_dim
+        self.num_blocks = t.shape[1]
+        self.device = t.device
+        self._index = t.device.index
+        block_stride = t.stride(1) if t.shape[1] > 1 else -(-record // 16) * 16
+        self._desc = N.Kv8CacheDesc(t.data_ptr(), block_stride, t.stride(0), t.shape[1], block_size, kv_heads, head_dim)
+        self._desc_ref = _byref(self._desc)
+        self._status = torch.zeros(1, dtype=torch.int32, device=t.device)
+        self._status_ptr = self._status.data_ptr()
+
+    # ------------------------------------------------------------------ what the tensor holds
+    @property
+    def values(self):
+        """View of the e4m3 values: [2, num_blocks, kv_heads, block_size, head_dim]."""
+        n = self.kv_heads * self.block_size * self.head_dim
+        return self.tensor[:, :, :n].view(torch.float8_e4m3fn).view(2, self.num_blocks, self.kv_heads, self.block_size,
+                                                                    self.head_dim)
+
+    @property
+    def scales(self):
+        """View of the scales: [2, num_blocks, kv_heads], float32."""
+        n = self.kv_heads * self.block_size * self.head_dim
+        return self.tensor[:, :, n:n + 4 * self.kv_heads].view(torch.float32)
+
+    def check(self):
+        """Raise if a call since the last check met a block id, a length or row starts that it had to leave out.  Waits
+        for the device's current stream."""
+        bits = int(self._status.item())
+        if bits:
+            self._status.zero_()
+            what = [text for bit, text in ((N.KV8_BAD_BLOCK, "a block id outside the cache"),
+                                           (N.KV8_BAD_LENGTH, "a length below 0 or above what block tables or weights hold"),
+                                           (N.KV8_BAD_ROWS, "row starts that fall, leave the tensors or exceed max_query"))
+                    if bits & bit]
+            _refuse("8-bit cache: " + "; ".join(what))
+
+    # ------------------------------------------------------------------ arguments
+    def _ints(self, name, t, dim):
+        if t.dtype != torch.int32 or t.dim() != dim or t.device != self.device:
+            _refuse(f"{name}: an int32 tensor of {dim} dimension(s) on {self.device} is needed, not {t.dtype} "
+                    f"{tuple(t.shape)} on {t.device}")
+        if t.shape[-1] > 1 and t.stride(-1) != 1:
+            _refuse(f"{name}: the last dimension must be dense")
+
+    def _batch(self, block_tables, lens, starts):
+        self._ints("block_tables", block_tables, 2)
+        self._ints("lens", lens, 1)
+        n = lens.shape[0]
+        if block_tables.shape[0] != n:
+            _refuse(f"block_tables has {block_tables.shape[0]} rows for {n} lengths")
+        ptr = None
+        if starts is not None:
+            self._ints("starts", starts, 1)
+            if starts.shape[0] != n + 1:
+                _refuse(f"starts has {starts.shape[0]} entries for {n} sequences: {n + 1} are needed")
+            ptr = starts.data_ptr()
+        return N.Kv8Batch(block_tables.data_ptr(), block_tables.stride(0), block_tables.shape[1], n, lens.data_ptr(), ptr,
+                          self._status_ptr)
+
+    def _rows(self, name, t, heads=None):
+        if t.dtype not in _DTYPES or t.dim() != 3 or t.device != self.device:
+            _refuse(f"{name}: a bfloat16 or float16 tensor [rows, heads, {self.head_dim}] on {self.device} is needed, not "
+                    f"{t.dtype} {tuple(t.shape)} on {t.device}")
+        if t.shape[2] != self.head_dim or (heads is not None and t.shape[1] != heads):
+            _refuse(f"{name}: shape {tuple(t.shape)} does not fit kv_heads={self.kv_heads}, head_dim={self.head_dim}")
+        if t.stride(2) != 1:
+            _refuse(f"{name}: the last dimension must be dense")
+        if t.requires_grad and torch.is_grad_enabled():
+            _refuse(f"{name} requires a gradient: the 8-bit cache has no backward pass")
+
+    def _stream(self, stream):
+        """(handle, the context in which memory for that stream is allocated)."""
+        if stream is None:
+            return torch.cuda.current_stream(self.device).cuda_stream
+        return stream
+
+    def _on(self, stream):
+        return torch.cuda.stream(torch.cuda.ExternalStream(stream, device=self.device))
+
+    # ------------------------------------------------------------------ operators
+    def append(self, k, v, block_tables, lens, *, starts=None, stream: Optional[int] = None) -> None:
+        """Write new tokens.  k, v: [rows, kv_heads, head_dim]; rows starts[s] .. starts[s + 1] (without starts: an equal
+        share of the rows) become tokens lens[s], lens[s] + 1, ... of sequence s.  lens holds the lengths before the call
+        and is not changed.  A block takes the scale that its largest magnitude needs; where a new row raises it,
+        the block's old rows are rounded anew."""
+        self._rows("k", k, self.kv_heads)
+        self._rows("v", v, self.kv_heads)
+        if k.dtype != v.dtype or k.shape != v.shape:
+            _refuse(f"k ({k.dtype} {tuple(k.shape)}) and v ({v.dtype} {tuple(v.shape)}) differ")
+        batch = self._batch(block_tables, lens, starts)
+        ks, vs = k.stride(), v.stride()
+        N.check(N.lib.pf_kv8_append(self._index, self._desc_ref, _byref(batch), k.data_ptr(), v.data_ptr(), _DTYPES[k.dtype],
+                                    k.shape[0], ks[0], ks[1], vs[0], vs[1], self._stream(stream)))
+
+    def attention(self, q, block_tables, lens, *, starts=None, max_query: Optional[int] = None,
+                  scale: Optional[float] = None, causal: bool = True, weights=None, lse: bool = False, out=None,
+                  stream: Optional[int] = None):
+        """Attention of q [rows, q_heads, head_dim] over the cache; returns out, or (out, lse) with ``lse=True``.
+
+        lens counts the rows' own tokens, which are in the cache already: row i of a sequence with n rows is
+        token lens - n + i and sees, unless ``causal=False``, the tokens up to itself.  A row that sees none
+        gives 0 and lse = -inf.  max_query: the most rows of any sequence (needed with starts).  scale: head_dim ** -0.5
+        unless given.  weights, float32 [sequences, kv_heads, >= longest]: each token's probability, summed over the
+        sequence's rows and the query heads of the KV head, is added in place.  Rows behind the last sequence are
+        left as they were in a given ``out``, and 0 in one that the call allocates."""
+        self._rows("q", q)
+        n_rows, q_heads, dim = q.shape
+        if q_heads == 0 or q_heads % self.kv_heads:
+            _refuse(f"{q_heads} query heads are not a multiple of {self.kv_heads} KV heads")
+        batch = self._batch(block_tables, lens, starts)
+        if max_query is None:
+            if starts is not None:
+                _refuse("max_query is needed with starts")
+            max_query = n_rows // max(1, batch.n_seqs)
+        elif max_query < 0:
+            _refuse(f"max_query={max_query}")
+        qs = q.stride()
+        a = N.Kv8AttentionArgs()
+        if weights is not None:
+            if weights.dtype != torch.float32 or weights.dim() != 3 or weights.device != self.device or \
+                    weights.shape[0] != batch.n_seqs or weights.shape[1] != self.kv_heads or \
+                    (weights.shape[2] > 1 and weights.stride(2) != 1):
+                _refuse(f"weights: a float32 tensor [{batch.n_seqs}, {self.kv_heads}, tokens] on {self.device} with a dense "
+                        f"last dimension is needed, not {weights.dtype} {tuple(weights.shape)} on {weights.device}")
+            a.weights, a.weights_capacity = weights.data_ptr(), weights.shape[2]
+            a.weights_seq_stride, a.weights_head_stride = weights.stride(0), weights.stride(1)
+        given = out is not None
+        if given:
+            self._rows("out", out)
+            if out.shape != q.shape or out.dtype != q.dtype:
+                _refuse(f"out ({out.dtype} {tuple(out.shape)}) and q ({q.dtype} {tuple(q.shape)}) differ")
+        a.q, a.n_rows, a.max_query, a.q_row_stride, a.q_head_stride = q.data_ptr(), n_rows, max_query, qs[0], qs[1]
+        a.q_heads, a.dtype, a.causal = q_heads, _DTYPES[q.dtype], int(causal)
+        a.scale = dim ** -0.5 if scale is None else scale
+        a.clear_tail = int(not given and starts is not None)
+        handle = self._stream(stream)
+        if stream is None:
+            return self._attend(a, batch, q, out, lse, handle)
+        with self._on(stream):     # what the call allocates belongs to the stream that uses it
+            return self._attend(a, batch, q, out, lse, handle)
+
+    def _attend(self, a, batch, q, out, want_lse, handle):
+        need = N.sz()
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        lse = None
+        if want_lse:
+            lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
+            a.lse = lse.data_ptr()
+        a.out = out.data_ptr()
+        a.out_row_stride, a.out_head_stride = out.stride(0), out.stride(1)
+        N.check(N.lib.pf_kv8_attention_workspace(self._index, self._desc_ref, _byref(batch), _byref(a), _byref(need)))
+        space = torch.empty(need.value, dtype=torch.uint8, device=q.device)
+        N.check(N.lib.pf_kv8_attention(self._index, self._desc_ref, _byref(batch), _byref(a), space.data_ptr(), need.value,
+                                       handle))
+        return (out, lse) if want_lse else out
+
+    def evict(self, block_tables, lens, weights, dst_tables, keep: int, *, recent: int = 0,
+              stream: Optional[int] = None) -> Tuple["torch.Tensor", "torch.Tensor", "torch.Tensor"]:
+        """Shorten every sequence to at most ``keep`` tokens by accumulated attention weight.
+
+        Of each sequence and KV head the last ``recent`` tokens are kept and, of the others, those of largest weight (equal
+        ones: the earlier token), in their order.  They are copied into the blocks of dst_tables [sequences,
+        ceil(keep / block_size)], which must not be among block_tables; the source blocks, which other sequences may
+        share, are not changed.  weights as ``attention`` accumulates them.
+
+        Returns (lens, weights, kept): int32 [sequences]; float32 like weights, 0 behind the kept tokens, so that
+        attention can go on adding; int32 [sequences, kv_heads, keep], the source token of each, -1 behind the last."""
+        batch = self._batch(block_tables, lens, None)
+        self._ints("dst_tables", dst_tables, 2)
+        n = batch.n_seqs
+        if not 0 < keep < 1 << 31 or not 0 <= recent <= keep:
+            _refuse(f"keep={keep}, recent={recent}: keep must be positive and recent at most keep")
+        if dst_tables.shape[0] != n or dst_tables.shape[1] * self.block_size < keep:
+            _refuse(f"dst_tables {tuple(dst_tables.shape)} does not hold {keep} tokens of {n} sequences")
+        if weights.dtype != torch.float32 or weights.dim() != 3 or weights.device != self.device or \
+                weights.shape[0] != n or weights.shape[1] != self.kv_heads or (weights.shape[2] > 1 and weights.stride(2) != 1):
+            _refuse(f"weights: a float32 tensor [{n}, {self.kv_heads}, tokens] on {self.device} with a dense last dimension "
+                    f"is needed, not {weights.dtype} {tuple(weights.shape)} on {weights.device}")
+        handle = self._stream(stream)
+        if stream is None:
+            return self._evict(batch, weights, dst_tables, keep, recent, handle)
+        with self._on(stream):
+            return self._evict(batch, weights, dst_tables, keep, recent, handle)
+
+    def _evict(self, batch, weights, dst_tables, keep, recent, handle):
+        n, heads, capacity = weights.shape
+        capacity = max(capacity, keep)
+        new_lens = torch.empty(n, dtype=torch.int32, device=self.device)
+        new_weights = torch.empty((n, heads, capacity), dtype=torch.float32, device=self.device)
+        kept = torch.empty((n, heads, keep), dtype=torch.int32, device=self.device)
+        a = N.Kv8EvictArgs(weights.data_ptr(), weights.stride(0), weights.stride(1), weights.shape[2], dst_tables.data_ptr(),
+                           dst_tables.stride(0), keep, recent, new_lens.data_ptr(), new_weights.data_ptr(), capacity,
+                           kept.data_ptr())
+        N.check(N.lib.pf_kv8_evict(self._index, self._desc_ref, _byref(batch), _byref(a), handle))
+        return new_lens, new_weights, kept
