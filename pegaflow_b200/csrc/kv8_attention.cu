@@ -22,7 +22,7 @@
 
 #include <algorithm>
 
-#include "kv8.h"
+#include "kv8_attention.h"
 
 namespace pf {
 namespace {
@@ -30,101 +30,7 @@ namespace {
 constexpr int kWarps = 4, kThreads = kWarps * 32;
 constexpr int kTile = 16;                   // tokens of one warp's step
 constexpr int kUnit = kTile * kWarps;       // tokens of one CTA's step, the granularity of the split
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-constexpr float kNone = -1e30f;             // reference of a row that has seen nothing
 constexpr float kShift = 9.f, kSlack = 6.f;
-
-struct AttnParams {
-  Kv8View cache;
-  Kv8Batch batch;
-  const uint16_t *q;
-  uint16_t *out;
-  float *lse;
-  float *weights;
-  int64_t q_row, q_head, out_row, out_head, w_seq, w_head;
-  int w_capacity;
-  int q_heads, group, max_query, row_tiles_most;
-  int causal, clear_tail, vec_q, vec_out;
-  float scale;
-  // partial results: slot 2 c + k of CTA c (k = 0: the segment that its range starts in, 1: the one that it ends in)
-  float *part_o;    // [slots][rows][dim]
-  float2 *part_ml;  // [slots][rows]
-  int n_ctas;
-};
-
-// The work of all sequences, heads and row tiles laid end to end in units of kUnit tokens; CTA c of n takes
-// [total c / n, total (c + 1) / n).  A segment is one (sequence, head, row tile).
-struct Split {
-  uint32_t total;
-  int n_ctas;       // at most total: every CTA that takes part has work
-  __device__ Split(uint32_t total, int n) : total(total), n_ctas((int)min((uint32_t)n, total)) {}
-  __device__ uint32_t begin(int c) const { return (uint32_t)((uint64_t)total * c / n_ctas); }
-  __device__ int owner(uint32_t u) const { return (int)((((uint64_t)u + 1) * n_ctas - 1) / total); }
-};
-
-template <int kRows>
-struct Seq {
-  int row0, rows, len, row_tiles;
-  uint32_t units;   // of one segment
-  __device__ Seq(const AttnParams &p, int s) {
-    int hi;
-    p.batch.rows(s, row0, hi);
-    rows = min(hi - row0, p.max_query);
-    len = p.batch.length(s, p.cache.block_log2);
-    row_tiles = (rows * p.group + kRows - 1) / kRows;
-    units = max(1, (len + kUnit - 1) / kUnit);
-  }
-  __device__ int visible(const AttnParams &p, int row) const {   // tokens that query row `row` (of rows * group) sees
-    const int i = row / p.group;
-    return p.causal ? min(max(len - rows + i + 1, 0), len) : len;
-  }
-};
-
-// prefix[s] = units before sequence s, prefix[n_seqs] = all of them.  Every CTA of every kernel computes it for
-// itself: lens stay on the device, and no launch and no workspace is spent on it.
-// kAllTiles: units of all row tiles; otherwise of one, for every sequence that has rows.
-template <int kRows, bool kAllTiles = true>
-__device__ void scan_units(const AttnParams &p, uint32_t *prefix) {
-  __shared__ uint32_t warp_sum[32];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n_warps = blockDim.x >> 5;
-  uint32_t base = 0;
-  for (int s0 = 0; s0 < p.batch.n_seqs; s0 += blockDim.x) {
-    const int s = s0 + threadIdx.x;
-    uint32_t mine = 0;
-    if (s < p.batch.n_seqs) {
-      const Seq<kRows> seq(p, s);
-      mine = seq.units * (uint32_t)(p.cache.heads * (kAllTiles ? seq.row_tiles : min(seq.row_tiles, 1)));
-    }
-    uint32_t x = mine;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const uint32_t y = __shfl_up_sync(0xffffffffu, x, d);
-      if (lane >= d) x += y;
-    }
-    if (lane == 31) warp_sum[warp] = x;
-    __syncthreads();
-    uint32_t before = base, all = 0;
-    for (int w = 0; w < n_warps; ++w) {
-      if (w < warp) before += warp_sum[w];
-      all += warp_sum[w];
-    }
-    if (s < p.batch.n_seqs) prefix[s] = before + x - mine;
-    base += all;
-    __syncthreads();
-  }
-  if (threadIdx.x == 0) prefix[p.batch.n_seqs] = base;
-  __syncthreads();
-}
-
-__device__ __forceinline__ int find_seq(const uint32_t *prefix, int n, uint32_t u) {   // last s with prefix[s] <= u
-  int lo = 0, hi = n;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (prefix[mid] <= u) lo = mid;
-    else hi = mid;
-  }
-  return lo;
-}
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                         uint32_t b1) {
@@ -137,28 +43,6 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(x));
   return d;
 }
-__device__ __forceinline__ uint32_t f16x2(float lo, float hi) {
-  uint32_t d;
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
-  return d;
-}
-__device__ __forceinline__ float exp2_fast(float x) {
-  float d;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(d) : "f"(x));
-  return d;
-}
-template <bool kBf16>
-__device__ __forceinline__ float widen1(uint16_t x) {
-  return kBf16 ? __uint_as_float((uint32_t)x << 16) : __half2float(__ushort_as_half(x));
-}
-template <bool kBf16>
-__device__ __forceinline__ uint32_t narrow2(float lo, float hi) {
-  if (!kBf16) return f16x2(lo, hi);
-  uint32_t d;
-  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
-  return d;
-}
-
 // Query rows as the B operand of S^T = K Q^T, for rows row_first + n, n < 8 * kNt.  Lane (g, t) holds row g's elements
 // 64 x + 16 t .. + 15 for each x, in the order in which K's lanes hold theirs.  factor = scale * log2(e) over the
 // row's power of two, for columns 2 t and 2 t + 1 of each tile: score in log2 units = product * factor * scale of K.
@@ -167,8 +51,8 @@ struct Queries {
   uint32_t b[kNt][kDim / 16][2];
   float factor[kNt][2];
 
-  template <int kRows>
-  __device__ void load(const AttnParams &p, const Seq<kRows> &seq, int head, int row_first) {
+  template <class SeqT>
+  __device__ void load(const AttnParams &p, const SeqT &seq, int head, int row_first) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 #pragma unroll
     for (int j = 0; j < kNt; ++j) {
@@ -320,30 +204,12 @@ __device__ __noinline__ void spread_nan(VTile<kDim> &v, float (&o)[kNt][kDim / 1
         if (((v.w[i][x] >> (8 * b)) & 0x7f) == 0x7f) v.w[i][x] &= ~(0xffu << (8 * b));
 }
 
-// Where a tile of a sequence lies: nothing for one whose block id is not in the cache.
-struct TileAt {
-  const uint8_t *k, *v;
-  float k_scale, v_scale;
-  int row0;
-};
-
-template <bool kWithV>
-__device__ __forceinline__ bool locate(const AttnParams &p, int s, int head, int tok, TileAt &at) {
+// A block of the sequence's table, looked up ahead of its use.
+struct Page {
   uint32_t id;
-  if (!p.batch.block(p.cache, s, tok >> p.cache.block_log2, id)) {
-    p.batch.report(PF_KV8_BAD_BLOCK);
-    at.k_scale = at.v_scale = 0.f;
-    return false;
-  }
-  at.row0 = tok & (p.cache.block_size() - 1);
-  at.k = p.cache.tile(0, id, head);
-  at.k_scale = __ldg(p.cache.scale(0, id, head));
-  if (kWithV) {
-    at.v = p.cache.tile(1, id, head);
-    at.v_scale = __ldg(p.cache.scale(1, id, head));
-  }
-  return true;
-}
+  bool there;
+  __device__ void find(const AttnParams &p, int s, int tok) { there = p.batch.block(p.cache, s, tok >> p.cache.block_log2, id); }
+};
 
 // CTAs that an SM holds: what the registers allow (128 of them at 128 dimensions and 8 rows).
 constexpr int ctas_of(int dim, int nt) { return dim == 256 ? 2 : dim == 128 ? (nt == 1 ? 4 : 2) : (nt == 1 ? 5 : 4); }
@@ -351,39 +217,53 @@ constexpr int ctas_of(int dim, int nt) { return dim == 256 ? 2 : dim == 128 ? (n
 template <int kDim, int kNt, bool kBf16>
 __global__ void __launch_bounds__(kThreads, ctas_of(kDim, kNt)) kv8_attention_rows(AttnParams p) {
   constexpr int kRows = 8 * kNt, kMt = kDim / 16;
+  using SeqT = Seq<kRows, kUnit>;
   extern __shared__ __align__(16) char smem[];
   float *sh_o = reinterpret_cast<float *>(smem);                       // [kWarps][kRows][kDim]
   float2 *sh_ml = reinterpret_cast<float2 *>(sh_o + kWarps * kRows * kDim);   // [kWarps][kRows]
   uint32_t *prefix = reinterpret_cast<uint32_t *>(sh_ml + kWarps * kRows);    // [n_seqs + 1]
-  scan_units<kRows>(p, prefix);
+  scan_units(p, prefix, [&](int s) { return SeqT(p, s).all_units(p); });
   const int n_seqs = p.batch.n_seqs, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const Split split{prefix[n_seqs], p.n_ctas};
-  if (blockIdx.x == 0) {
-    if (p.batch.starts) p.batch.check_starts(p.max_query);
-    for (int s = threadIdx.x; s < n_seqs; s += kThreads)
-      if (p.batch.lens[s] < 0 || p.batch.lens[s] > p.batch.length(s, p.cache.block_log2)) p.batch.report(PF_KV8_BAD_LENGTH);
-  }
+  const Split split(prefix[n_seqs], p.n_ctas);
+  if (blockIdx.x == 0) check_batch(p);
   if ((int)blockIdx.x >= split.n_ctas) return;
   uint32_t u = split.begin(blockIdx.x);
   const uint32_t u_end = split.begin(blockIdx.x + 1);
   bool first_segment = true;
   while (u < u_end) {
     const int s = find_seq(prefix, n_seqs, u);
-    const Seq<kRows> seq(p, s);
-    const uint32_t in_seq = u - prefix[s], segment = in_seq / seq.units, unit0 = in_seq % seq.units;
-    const int head = segment / seq.row_tiles, rt = segment % seq.row_tiles, row_first = rt * kRows;
-    const uint32_t units = min(seq.units - unit0, u_end - u);
-    const int live_rows = min(seq.rows * p.group - row_first, kRows);
+    const SeqT seq(p, s);
+    const Segment seg(p, seq, s, prefix[s], u);
+    const int head = seg.head, row_first = seg.rt * kRows;
+    const uint32_t unit0 = u - seg.begin, units = min(seg.units - unit0, u_end - u);
+    const int live_rows = min(seq.all_rows(p) - row_first, kRows);
     const int most = seq.visible(p, row_first + live_rows - 1);         // tokens that any row of the tile sees
     const int least = seq.visible(p, row_first);                        // tokens that all rows see
+    const int tok_end = (int)min((int64_t)(unit0 + units) * kUnit, (int64_t)most);
+    int tok = (int)(unit0 * kUnit) + warp * kTile;
+
+    // The pages of two steps ahead, the values of one: K of the next step is asked for when this step's products have
+    // read K's registers, V when its own have.
+    const int within = p.cache.block_size() - 1;
+    Page page{}, next{};
+    KTile<kDim> kt;
+    VTile<kDim> vt;
+    float k_scale = 0.f, v_scale = 0.f;
+    if (tok < tok_end) page.find(p, s, tok);
+    if (tok + kUnit < tok_end) next.find(p, s, tok + kUnit);
+    if (tok < tok_end && page.there) {
+      kt.load(p.cache.tile(0, page.id, head), tok & within);
+      k_scale = __ldg(p.cache.scale(0, page.id, head));
+      vt.load(p.cache.tile(1, page.id, head), tok & within);
+      v_scale = __ldg(p.cache.scale(1, page.id, head));
+    }
+    Queries<kDim, kNt, kBf16> q;
+    q.load(p, seq, head, row_first);
     int see[kNt][2];
 #pragma unroll
     for (int j = 0; j < kNt; ++j)
 #pragma unroll
-      for (int k = 0; k < 2; ++k) see[j][k] = seq.visible(p, min(row_first + 8 * j + 2 * t + k, seq.rows * p.group - 1));
-
-    Queries<kDim, kNt, kBf16> q;
-    q.load(p, seq, head, row_first);
+      for (int k = 0; k < 2; ++k) see[j][k] = seq.visible(p, min(row_first + 8 * j + 2 * t + k, seq.all_rows(p) - 1));
     float o[kNt][kMt][4], ref[kNt][2], sum[kNt][2];
 #pragma unroll
     for (int j = 0; j < kNt; ++j) {
@@ -392,87 +272,94 @@ __global__ void __launch_bounds__(kThreads, ctas_of(kDim, kNt)) kv8_attention_ro
       ref[j][0] = ref[j][1] = kNone;
       sum[j][0] = sum[j][1] = 0.f;
     }
-    const int tok_end = (int)min((int64_t)(unit0 + units) * kUnit, (int64_t)most);
-    for (int tok = (int)(unit0 * kUnit) + warp * kTile; tok < tok_end; tok += kUnit) {
-      TileAt at;
-      KTile<kDim> kt;
-      VTile<kDim> vt;
-      const bool there = locate<true>(p, s, head, tok, at);
-      if (!there) continue;
-      kt.load(at.k, at.row0);
-      vt.load(at.v, at.row0);
-      if (tok + kTile > seq.len) clear_behind(vt, seq.len - tok);
-      if (tok + kTile > least && __any_sync(0xffffffffu, vt.has_nan())) spread_nan<kDim, kNt>(vt, o, see, tok);
+    for (; tok < tok_end; tok += kUnit) {
+      const bool there = page.there, more = tok + kUnit < tok_end && next.there;
+      if (!there) p.batch.report(PF_KV8_BAD_BLOCK);
       float c[kNt][4];
 #pragma unroll
       for (int j = 0; j < kNt; ++j) c[j][0] = c[j][1] = c[j][2] = c[j][3] = 0.f;
-      kt.products(q, c);
-      bool over = false;
+      if (there) kt.products(q, c);
 #pragma unroll
       for (int j = 0; j < kNt; ++j)
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          const float f = q.factor[j][k] * at.k_scale;
+          const float f = q.factor[j][k] * k_scale;
           c[j][k] *= f;
           c[j][k + 2] *= f;
         }
-      if (tok + kTile > least) {
-#pragma unroll
-        for (int j = 0; j < kNt; ++j)
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            if (tok + g >= see[j][k]) c[j][k] = -INFINITY;
-            if (tok + g + 8 >= see[j][k]) c[j][k + 2] = -INFINITY;
-          }
+      const Page ahead = next;
+      if (more) {
+        kt.load(p.cache.tile(0, ahead.id, head), (tok + kUnit) & within);
+        k_scale = __ldg(p.cache.scale(0, ahead.id, head));
       }
+      if (tok + 2 * kUnit < tok_end) next.find(p, s, tok + 2 * kUnit);
+      page = ahead;
+      if (there) {
+        if (tok + kTile > least) {
 #pragma unroll
-      for (int j = 0; j < kNt; ++j)
+          for (int j = 0; j < kNt; ++j)
 #pragma unroll
-        for (int k = 0; k < 2; ++k) over |= fmaxf(c[j][k], c[j][k + 2]) > ref[j][k] + kSlack;
-      if (__any_sync(0xffffffffu, over)) {
+            for (int k = 0; k < 2; ++k) {
+              if (tok + g >= see[j][k]) c[j][k] = -INFINITY;
+              if (tok + g + 8 >= see[j][k]) c[j][k + 2] = -INFINITY;
+            }
+          if (tok + kTile > seq.len) clear_behind(vt, seq.len - tok);
+          if (__any_sync(0xffffffffu, vt.has_nan())) spread_nan<kDim, kNt>(vt, o, see, tok);
+        }
+        bool over = false;
 #pragma unroll
         for (int j = 0; j < kNt; ++j)
 #pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            float top = fmaxf(c[j][k], c[j][k + 2]);
+          for (int k = 0; k < 2; ++k) over |= fmaxf(c[j][k], c[j][k + 2]) > ref[j][k] + kSlack;
+        if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
-            for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-            const float now = fmaxf(ref[j][k], top), r = exp2_fast(ref[j][k] - now);
-            ref[j][k] = now;
-            sum[j][k] *= r;
+          for (int j = 0; j < kNt; ++j)
 #pragma unroll
-            for (int m = 0; m < kMt; ++m) {
-              o[j][m][k] *= r;
-              o[j][m][k + 2] *= r;
+            for (int k = 0; k < 2; ++k) {
+              float top = fmaxf(c[j][k], c[j][k + 2]);
+#pragma unroll
+              for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+              const float now = fmaxf(ref[j][k], top), r = exp2_fast(ref[j][k] - now);
+              ref[j][k] = now;
+              sum[j][k] *= r;
+#pragma unroll
+              for (int m = 0; m < kMt; ++m) {
+                o[j][m][k] *= r;
+                o[j][m][k + 2] *= r;
+              }
+            }
+        }
+        uint32_t pb[kNt][2];
+#pragma unroll
+        for (int j = 0; j < kNt; ++j) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) c[j][k] = exp2_fast(c[j][k] - (ref[j][k & 1] - kShift));
+          sum[j][0] += c[j][0] + c[j][2];
+          sum[j][1] += c[j][1] + c[j][3];
+          pb[j][0] = transpose8x8(f16x2(c[j][0], c[j][1]));
+          pb[j][1] = transpose8x8(f16x2(c[j][2], c[j][3]));
+        }
+#pragma unroll
+        for (int w = 0; w < VTile<kDim>::kWords; ++w) {
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const uint32_t sel = half ? 0x7362 : 0x5140;
+            const uint32_t ab = __byte_perm(vt.w[0][w], vt.w[1][w], sel), ce = __byte_perm(vt.w[2][w], vt.w[3][w], sel);
+            const uint32_t a0 = f16x2_from_e4m3<0>(ab), a1 = f16x2_from_e4m3<1>(ab);
+            const uint32_t a2 = f16x2_from_e4m3<0>(ce), a3 = f16x2_from_e4m3<1>(ce);
+#pragma unroll
+            for (int j = 0; j < kNt; ++j) {
+              float d[4] = {0.f, 0.f, 0.f, 0.f};
+              mma_f16(d, a0, a1, a2, a3, pb[j][0], pb[j][1]);
+#pragma unroll
+              for (int k = 0; k < 4; ++k) o[j][2 * w + half][k] += v_scale * d[k];
             }
           }
-      }
-      uint32_t pb[kNt][2];
-#pragma unroll
-      for (int j = 0; j < kNt; ++j) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) c[j][k] = exp2_fast(c[j][k] - (ref[j][k & 1] - kShift));
-        sum[j][0] += c[j][0] + c[j][2];
-        sum[j][1] += c[j][1] + c[j][3];
-        pb[j][0] = transpose8x8(f16x2(c[j][0], c[j][1]));
-        pb[j][1] = transpose8x8(f16x2(c[j][2], c[j][3]));
-      }
-#pragma unroll
-      for (int w = 0; w < VTile<kDim>::kWords; ++w) {
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const uint32_t sel = half ? 0x7362 : 0x5140;
-          const uint32_t ab = __byte_perm(vt.w[0][w], vt.w[1][w], sel), ce = __byte_perm(vt.w[2][w], vt.w[3][w], sel);
-          const uint32_t a0 = f16x2_from_e4m3<0>(ab), a1 = f16x2_from_e4m3<1>(ab);
-          const uint32_t a2 = f16x2_from_e4m3<0>(ce), a3 = f16x2_from_e4m3<1>(ce);
-#pragma unroll
-          for (int j = 0; j < kNt; ++j) {
-            float d[4] = {0.f, 0.f, 0.f, 0.f};
-            mma_f16(d, a0, a1, a2, a3, pb[j][0], pb[j][1]);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) o[j][2 * w + half][k] += at.v_scale * d[k];
-          }
         }
+      }
+      if (more) {
+        vt.load(p.cache.tile(1, ahead.id, head), (tok + kUnit) & within);
+        v_scale = __ldg(p.cache.scale(1, ahead.id, head));
       }
     }
     // join the four warps
@@ -501,7 +388,7 @@ __global__ void __launch_bounds__(kThreads, ctas_of(kDim, kNt)) kv8_attention_ro
               make_float4(o[j][m][k] * r, o[j][m][k + 2] * r, o[j][m + 1][k] * r, o[j][m + 1][k + 2] * r);
       }
     __syncthreads();
-    const bool whole = unit0 == 0 && units == seq.units;
+    const bool whole = units == seg.units;
     const int slot = 2 * blockIdx.x + (first_segment ? 0 : 1);
     for (int e = threadIdx.x; e < live_rows * (kDim / 4); e += kThreads) {
       const int n = e / (kDim / 4), d = e % (kDim / 4) * 4;
@@ -523,10 +410,10 @@ __global__ void __launch_bounds__(kThreads, ctas_of(kDim, kNt)) kv8_attention_ro
         const uint32_t x = narrow2<kBf16>(a.x * inv, a.y * inv), y = narrow2<kBf16>(a.z * inv, a.w * inv);
         if (p.vec_out) *reinterpret_cast<uint2 *>(dst) = make_uint2(x, y);
         else dst[0] = (uint16_t)x, dst[1] = x >> 16, dst[2] = (uint16_t)y, dst[3] = y >> 16;
-        if (d == 0 && p.lse) p.lse[(int64_t)(seq.row0 + i) * p.q_heads + qh] = l == 0.f ? -INFINITY : (top - kShift + log2f(l)) * kLn2;
+        if (d == 0 && p.lse) p.lse[(int64_t)(seq.row0 + i) * p.q_heads + qh] = lse_of(top - kShift, l);
       } else {
         *reinterpret_cast<float4 *>(p.part_o + ((int64_t)slot * kRows + n) * kDim + d) = a;
-        if (d == 0) p.part_ml[slot * kRows + n] = make_float2(top, l);
+        if (d == 0) p.part_ml[slot * kRows + n] = make_float2(top - kShift, l);
       }
     }
     __syncthreads();
@@ -535,125 +422,180 @@ __global__ void __launch_bounds__(kThreads, ctas_of(kDim, kNt)) kv8_attention_ro
   }
 }
 
-// Joins the parts of segments that several CTAs shared, one CTA for each (segment, row), in the order of the tokens.
-// kSpan threads hold one part's row as float4, kThreads / kSpan parts are read at a time.
-template <int kDim, int kNt, bool kBf16>
+// Joins the parts of segments that several CTAs shared, in the order of the tokens.  CTA (b, y) looks at the boundary
+// between the ranges of CTAs b and b + 1: if it is the first one within a segment, it joins rows y, y + gridDim.y, ...
+// of it.  A row of a part is kDim / 4 threads' float4; kThreads / (kDim / 4) parts are read at a time.
+template <int kDim, int kRows, int kUnits, bool kBf16>
 __global__ void __launch_bounds__(kThreads) kv8_attention_join(AttnParams p) {
-  constexpr int kRows = 8 * kNt, kSpan = kDim / 4, kAtOnce = kThreads / kSpan;
+  constexpr int kSpan = kDim / 4, kAtOnce = kThreads / kSpan;
+  using SeqT = Seq<kRows, kUnits>;
   extern __shared__ __align__(16) char smem[];
   uint32_t *prefix = reinterpret_cast<uint32_t *>(smem);
   __shared__ float4 sh_a[kThreads];
   __shared__ float sh_l[kAtOnce];
-  scan_units<kRows>(p, prefix);
   const int n_seqs = p.batch.n_seqs;
   if (p.clear_tail) {
     int lo, hi = 0;
     if (n_seqs) p.batch.rows(n_seqs - 1, lo, hi);
-    for (int64_t e = (int64_t)hi * p.q_heads * kDim + blockIdx.x * kThreads + threadIdx.x;
-         e < (int64_t)p.batch.n_rows * p.q_heads * kDim; e += (int64_t)gridDim.x * kThreads) {
+    const int64_t id = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * kThreads + threadIdx.x;
+    for (int64_t e = (int64_t)hi * p.q_heads * kDim + id; e < (int64_t)p.batch.n_rows * p.q_heads * kDim;
+         e += (int64_t)gridDim.x * gridDim.y * kThreads) {
       const int64_t row = e / (p.q_heads * kDim);
       const int qh = (int)(e / kDim % p.q_heads), d = (int)(e % kDim);
       p.out[row * p.out_row + qh * p.out_head + d] = 0;
       if (d == 0 && p.lse) p.lse[row * p.q_heads + qh] = -INFINITY;
     }
   }
-  const Split split{prefix[n_seqs], p.n_ctas};
-  const int n = blockIdx.x % kRows, rt = blockIdx.x / kRows % p.row_tiles_most;
-  const int rest = blockIdx.x / kRows / p.row_tiles_most, head = rest % p.cache.heads, s = rest / p.cache.heads;
-  if (s >= n_seqs) return;
-  const Seq<kRows> seq(p, s);
-  const int row = rt * kRows + n;
-  if (row >= seq.rows * p.group) return;
-  const uint32_t u0 = prefix[s] + (uint32_t)(head * seq.row_tiles + rt) * seq.units, u1 = u0 + seq.units;
-  const int c0 = split.owner(u0), c1 = split.owner(u1 - 1);
-  if (c0 == c1) return;
+  scan_units(p, prefix, [&](int s) { return SeqT(p, s).all_units(p); });
+  const Split split(prefix[n_seqs], p.n_ctas);
+  const int c0 = blockIdx.x;
+  if (c0 + 1 >= split.n_ctas) return;
+  const uint32_t u = split.begin(c0 + 1);
+  const int s = find_seq(prefix, n_seqs, u);
+  const SeqT seq(p, s);
+  const Segment seg(p, seq, s, prefix[s], u);
+  if (seg.begin == u || split.owner(seg.begin) != c0) return;
+  const int c1 = split.owner(seg.begin + seg.units - 1), slot0 = 2 * c0 + (split.begin(c0) < seg.begin ? 1 : 0);
   const int part = threadIdx.x / kSpan, d = threadIdx.x % kSpan * 4;
-  float top = kNone;
-  for (int c = c0; c <= c1; ++c) top = fmaxf(top, p.part_ml[(2 * c + (c == c0 && split.begin(c) < u0 ? 1 : 0)) * kRows + n].x);
-  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-  float l = 0.f;
-  for (int c = c0 + part; c <= c1; c += kAtOnce) {
-    const int slot = 2 * c + (c == c0 && split.begin(c) < u0 ? 1 : 0);
-    const float2 ml = p.part_ml[slot * kRows + n];
-    const float r = exp2_fast(ml.x - top);
-    const float4 x = *reinterpret_cast<const float4 *>(p.part_o + ((int64_t)slot * kRows + n) * kDim + d);
-    l += ml.y * r;
-    a.x += x.x * r, a.y += x.y * r, a.z += x.z * r, a.w += x.w * r;
+  const int live_rows = min(seq.all_rows(p) - seg.rt * kRows, kRows);
+  for (int n = blockIdx.y; n < live_rows; n += gridDim.y) {
+    float top = kNone;
+    for (int c = c0; c <= c1; ++c) top = fmaxf(top, p.part_ml[(c == c0 ? slot0 : 2 * c) * kRows + n].x);
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+    float l = 0.f;
+    for (int c = c0 + part; c <= c1; c += kAtOnce) {
+      const int slot = c == c0 ? slot0 : 2 * c;
+      const float2 ml = p.part_ml[slot * kRows + n];
+      const float r = exp2_fast(ml.x - top);
+      const float4 x = *reinterpret_cast<const float4 *>(p.part_o + ((int64_t)slot * kRows + n) * kDim + d);
+      l += ml.y * r;
+      a.x += x.x * r, a.y += x.y * r, a.z += x.z * r, a.w += x.w * r;
+    }
+    sh_a[threadIdx.x] = a;
+    if (d == 0) sh_l[part] = l;
+    __syncthreads();
+    if (part == 0) {
+      for (int k = 1; k < kAtOnce; ++k) {
+        const float4 x = sh_a[k * kSpan + threadIdx.x];
+        a.x += x.x, a.y += x.y, a.z += x.z, a.w += x.w;
+        l += sh_l[k];
+      }
+      const int row = seg.rt * kRows + n, i = row / p.group, qh = seg.head * p.group + row % p.group;
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      uint16_t *dst = p.out + (int64_t)(seq.row0 + i) * p.out_row + qh * p.out_head + d;
+      const uint32_t x = narrow2<kBf16>(a.x * inv, a.y * inv), y = narrow2<kBf16>(a.z * inv, a.w * inv);
+      if (p.vec_out) *reinterpret_cast<uint2 *>(dst) = make_uint2(x, y);
+      else dst[0] = (uint16_t)x, dst[1] = x >> 16, dst[2] = (uint16_t)y, dst[3] = y >> 16;
+      if (d == 0 && p.lse) p.lse[(int64_t)(seq.row0 + i) * p.q_heads + qh] = lse_of(top, l);
+    }
+    __syncthreads();
   }
-  sh_a[threadIdx.x] = a;
-  if (d == 0) sh_l[part] = l;
-  __syncthreads();
-  if (part) return;
-  for (int k = 1; k < kAtOnce; ++k) {
-    const float4 x = sh_a[k * kSpan + threadIdx.x];
-    a.x += x.x, a.y += x.y, a.z += x.z, a.w += x.w;
-    l += sh_l[k];
-  }
-  const int i = row / p.group, qh = head * p.group + row % p.group;
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  uint16_t *dst = p.out + (int64_t)(seq.row0 + i) * p.out_row + qh * p.out_head + d;
-  const uint32_t x = narrow2<kBf16>(a.x * inv, a.y * inv), y = narrow2<kBf16>(a.z * inv, a.w * inv);
-  dst[0] = (uint16_t)x, dst[1] = x >> 16, dst[2] = (uint16_t)y, dst[3] = y >> 16;
-  if (d == 0 && p.lse) p.lse[(int64_t)(seq.row0 + i) * p.q_heads + qh] = l == 0.f ? -INFINITY : (top - kShift + log2f(l)) * kLn2;
 }
 
 // weights[s, head, j] += sum over rows and group heads of exp(score - lse), once lse is known: the scores are taken
-// again, a warp for each 16-token tile with K in registers and the row tiles passing by.  Each element has one writer.
+// again, a warp for 16 tokens, or for 64 at a time where there are more than eight rows.  Each element has one writer.
 template <int kDim, bool kBf16>
 __global__ void __launch_bounds__(kThreads) kv8_attention_weights(AttnParams p) {
-  constexpr int kRows = 8;
+  constexpr int kRows = 8, kDeep = 4;
+  using SeqT = Seq<kRows, kUnit>;
   extern __shared__ __align__(16) char smem[];
   uint32_t *prefix = reinterpret_cast<uint32_t *>(smem);
-  scan_units<kRows, false>(p, prefix);
+  auto units_of = [&](const SeqT &seq) {   // of one head; none for a sequence without rows
+    const int tokens = min(seq.len, p.w_capacity);
+    return seq.rows ? (uint32_t)((tokens + kUnit - 1) / kUnit) : 0u;
+  };
+  scan_units(p, prefix, [&](int s) { return units_of(SeqT(p, s)) * (uint32_t)p.cache.heads; });
   const int n_seqs = p.batch.n_seqs, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   if (blockIdx.x == 0)
     for (int s = threadIdx.x; s < n_seqs; s += kThreads)
       if (p.batch.lens[s] > p.w_capacity) p.batch.report(PF_KV8_BAD_LENGTH);
-  for (uint32_t u = blockIdx.x; u < prefix[n_seqs]; u += gridDim.x) {
+  const Split split(prefix[n_seqs], gridDim.x);
+  if ((int)blockIdx.x >= split.n_ctas) return;
+  const int within = p.cache.block_size() - 1;
+  uint32_t u = split.begin(blockIdx.x);
+  const uint32_t u_end = split.begin(blockIdx.x + 1);
+  while (u < u_end) {
     const int s = find_seq(prefix, n_seqs, u);
-    const Seq<kRows> seq(p, s);
-    const int head = (u - prefix[s]) / seq.units, tok = (u - prefix[s]) % seq.units * kUnit + warp * kTile;
-    const int end = min(seq.len, p.w_capacity);
-    if (tok >= end) continue;
-    TileAt at;
-    if (!locate<false>(p, s, head, tok, at)) continue;
-    KTile<kDim> kt;
-    kt.load(at.k, at.row0);
-    float w0 = 0.f, w1 = 0.f;
-    for (int row_first = 0; row_first < seq.rows * p.group; row_first += kRows) {
-      if (seq.visible(p, min(row_first + kRows, seq.rows * p.group) - 1) <= tok) continue;
-      Queries<kDim, 1, kBf16> q;
-      q.load(p, seq, head, row_first);
+    const SeqT seq(p, s);
+    const uint32_t of_head = units_of(seq), unit0 = (u - prefix[s]) % of_head, units = min(of_head - unit0, u_end - u);
+    const int head = (u - prefix[s]) / of_head, end = min(seq.len, p.w_capacity), rows = seq.all_rows(p);
+    float *dst = p.weights + s * p.w_seq + head * p.w_head;
+    // adds row tile row_first's share of the 16 tokens from tok on
+    auto add = [&](const Queries<kDim, 1, kBf16> &q, const float (&base)[2], const int (&see)[2], int tok, float (&w)[2]) {
+      Page page;
+      page.find(p, s, tok);
+      if (!page.there) return;
+      KTile<kDim> kt;
+      kt.load(p.cache.tile(0, page.id, head), tok & within);
+      const float k_scale = __ldg(p.cache.scale(0, page.id, head));
       float c[1][4] = {{0.f, 0.f, 0.f, 0.f}};
       kt.products(q, c);
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
+        const float f = q.factor[0][k] * k_scale;
+        if (tok + g < see[k]) w[0] += exp2_fast(c[0][k] * f - base[k]);
+        if (tok + g + 8 < see[k]) w[1] += exp2_fast(c[0][k + 2] * f - base[k]);
+      }
+    };
+    auto rows_of = [&](Queries<kDim, 1, kBf16> &q, float (&base)[2], int (&see)[2], int row_first) {
+      q.load(p, seq, head, row_first);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
         const int row = row_first + 2 * t + k;
-        if (row < seq.rows * p.group) {
-          const int i = row / p.group, qh = head * p.group + row % p.group, see = seq.visible(p, row);
-          const float f = q.factor[0][k] * at.k_scale;
-          const float base = __ldg(p.lse + (int64_t)(seq.row0 + i) * p.q_heads + qh) * kLog2e;
-          if (tok + g < see) w0 += exp2_fast(c[0][k] * f - base);
-          if (tok + g + 8 < see) w1 += exp2_fast(c[0][k + 2] * f - base);
+        base[k] = 0.f, see[k] = 0;
+        if (row < rows) {
+          see[k] = seq.visible(p, row);
+          base[k] = p.lse[(int64_t)(seq.row0 + row / p.group) * p.q_heads + head * p.group + row % p.group] * kLog2e;
         }
       }
-    }
+    };
+    auto store = [&](int tok, float (&w)[2]) {
 #pragma unroll
-    for (int d = 1; d < 4; d <<= 1) {
-      w0 += __shfl_xor_sync(0xffffffffu, w0, d);
-      w1 += __shfl_xor_sync(0xffffffffu, w1, d);
+      for (int d = 1; d < 4; d <<= 1) {
+        w[0] += __shfl_xor_sync(0xffffffffu, w[0], d);
+        w[1] += __shfl_xor_sync(0xffffffffu, w[1], d);
+      }
+      if (t == 0) {
+        if (tok + g < end) dst[tok + g] += w[0];
+        if (tok + g + 8 < end) dst[tok + g + 8] += w[1];
+      }
+    };
+    Queries<kDim, 1, kBf16> q;
+    float base[2];
+    int see[2];
+    if (rows <= kRows) {
+      rows_of(q, base, see, 0);
+      for (uint32_t i = unit0; i < unit0 + units; ++i) {
+        const int tok = (int)(i * kUnit) + warp * kTile;
+        float w[2] = {0.f, 0.f};
+        if (tok >= end) break;
+        add(q, base, see, tok, w);
+        store(tok, w);
+      }
+    } else {
+      for (uint32_t i = unit0 + warp; i < unit0 + units; i += kWarps) {
+        const int tok = (int)(i * kUnit);
+        float w[kDeep][2] = {};
+        for (int row_first = 0; row_first < rows; row_first += kRows) {
+          if (seq.visible(p, min(row_first + kRows, rows) - 1) <= tok) continue;
+          rows_of(q, base, see, row_first);
+#pragma unroll
+          for (int m = 0; m < kDeep; ++m)
+            if (tok + m * kTile < end) add(q, base, see, tok + m * kTile, w[m]);
+        }
+#pragma unroll
+        for (int m = 0; m < kDeep; ++m)
+          if (tok + m * kTile < end) store(tok + m * kTile, w[m]);
+      }
     }
-    if (t == 0) {
-      float *dst = p.weights + s * p.w_seq + head * p.w_head + tok + g;
-      if (tok + g < end) dst[0] += w0;
-      if (tok + g + 8 < end) dst[8] += w1;
-    }
+    u += units;
   }
 }
 
 // ---------------------------------------------------------------------------------------------- host
 struct Plan {
-  int nt, n_ctas;
+  int nt;               // row tiles of eight, 0: by the hundred
+  int n_ctas, rows;     // rows of a part
   size_t part_o, part_ml, lse, bytes;   // offsets in the workspace
 };
 
@@ -663,10 +605,10 @@ Plan make_plan(int device_id, const Kv8View &c, const pf_kv8_attention_args &a) 
   const size_t group = a.q_heads / c.heads;
   Plan plan{};
   const size_t rows = std::min(a.max_query, a.n_rows) * group;
-  plan.nt = rows <= 8 || c.dim == 256 ? 1 : 2;
-  const int ctas_per_sm = ctas_of(c.dim, plan.nt);
-  plan.n_ctas = kv8_sm_count(device_id) * ctas_per_sm;
-  const size_t slots = 2 * (size_t)plan.n_ctas * 8 * plan.nt;
+  plan.nt = rows <= 8 ? 1 : rows <= 16 && c.dim != 256 ? 2 : 0;
+  plan.n_ctas = kv8_sm_count(device_id) * (plan.nt ? ctas_of(c.dim, plan.nt) : 1);
+  plan.rows = plan.nt ? 8 * plan.nt : kv8_wide_plan(c.dim).rows;
+  const size_t slots = 2 * (size_t)plan.n_ctas * plan.rows;
   plan.part_o = 0;
   plan.part_ml = up256(slots * c.dim * 4);
   plan.lse = plan.part_ml + up256(slots * 8);
@@ -688,14 +630,18 @@ void check_args(const pf_kv8_attention_args *a, const Kv8View &c, const Kv8Batch
   const uint64_t units = ((uint64_t)b.max_blocks << c.block_log2) / kUnit + 1;
   const uint64_t tiles = ((uint64_t)a->n_rows * (a->q_heads / c.heads) + 7) / 8 + b.n_seqs;
   if (units * tiles > 0xffffffffull / c.heads) throw Error::invalid("too many query rows for tables of this width: split the call");
-  if ((rows_of_group + 15) * c.heads * std::max(b.n_seqs, 1) > 0x7fffffffull)
-    throw Error::invalid("too many query rows for so many sequences: split the call");
+}
+
+template <int kDim, int kRows, int kUnits, bool kBf16>
+void launch_join(const AttnParams &p, int ctas_of_a_boundary, cudaStream_t stream) {
+  const dim3 grid((unsigned)p.n_ctas, (unsigned)ctas_of_a_boundary);
+  kv8_attention_join<kDim, kRows, kUnits, kBf16><<<grid, kThreads, ((size_t)p.batch.n_seqs + 1) * 4, stream>>>(p);
+  PF_KV8_LAUNCHED();
 }
 
 template <int kDim, int kNt, bool kBf16>
-void launch(const AttnParams &p, cudaStream_t stream) {
-  const size_t scan = ((size_t)p.batch.n_seqs + 1) * 4;
-  const size_t smem = kWarps * 8 * kNt * (kDim * 4 + 8) + scan;
+void launch_rows(const AttnParams &p, cudaStream_t stream) {
+  const size_t smem = kWarps * 8 * kNt * (kDim * 4 + 8) + ((size_t)p.batch.n_seqs + 1) * 4;
   auto kernel = kv8_attention_rows<kDim, kNt, kBf16>;
   if (smem > 48 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
     throw Error::storage("cudaFuncSetAttribute failed");
@@ -703,20 +649,31 @@ void launch(const AttnParams &p, cudaStream_t stream) {
     kernel<<<p.n_ctas, kThreads, smem, stream>>>(p);
     PF_KV8_LAUNCHED();
   }
-  const size_t join = std::max<size_t>(1, (size_t)p.batch.n_seqs * p.cache.heads * p.row_tiles_most * 8 * kNt);
-  kv8_attention_join<kDim, kNt, kBf16><<<(unsigned)join, kThreads, scan, stream>>>(p);
-  PF_KV8_LAUNCHED();
-  if (p.weights) {
-    kv8_attention_weights<kDim, kBf16><<<p.n_ctas, kThreads, scan, stream>>>(p);
+  launch_join<kDim, 8 * kNt, kUnit, kBf16>(p, 8 * kNt, stream);
+}
+
+template <int kDim, bool kBf16>
+void launch_all(const AttnParams &p, int nt, int n_sms, cudaStream_t stream) {
+  if (nt == 0) {
+    if (p.batch.n_seqs) kv8_wide_launch(p, kBf16, stream);
+    constexpr int kRows = kDim == 256 ? 128 : 256, kTokens = kDim == 256 ? 64 : 128;
+    launch_join<kDim, kRows, kTokens, kBf16>(p, 32, stream);
+  } else if (nt == 1) {
+    launch_rows<kDim, 1, kBf16>(p, stream);
+  } else if constexpr (kDim != 256) {
+    launch_rows<kDim, 2, kBf16>(p, stream);
+  }
+  if (p.weights && p.batch.n_seqs) {
+    kv8_attention_weights<kDim, kBf16><<<n_sms * 4, kThreads, ((size_t)p.batch.n_seqs + 1) * 4, stream>>>(p);
     PF_KV8_LAUNCHED();
   }
 }
 
 template <bool kBf16>
-void launch(const AttnParams &p, int nt, cudaStream_t stream) {
-  if (p.cache.dim == 64) nt == 1 ? launch<64, 1, kBf16>(p, stream) : launch<64, 2, kBf16>(p, stream);
-  else if (p.cache.dim == 128) nt == 1 ? launch<128, 1, kBf16>(p, stream) : launch<128, 2, kBf16>(p, stream);
-  else launch<256, 1, kBf16>(p, stream);
+void launch(const AttnParams &p, int nt, int n_sms, cudaStream_t stream) {
+  if (p.cache.dim == 64) launch_all<64, kBf16>(p, nt, n_sms, stream);
+  else if (p.cache.dim == 128) launch_all<128, kBf16>(p, nt, n_sms, stream);
+  else launch_all<256, kBf16>(p, nt, n_sms, stream);
 }
 
 }  // namespace
@@ -770,7 +727,6 @@ int pf_kv8_attention(int device_id, const pf_kv8_cache *cache, const pf_kv8_batc
     p.q_heads = (int)a.q_heads;
     p.group = (int)a.q_heads / c.heads;
     p.max_query = (int)std::min<size_t>(a.max_query, a.n_rows);
-    p.row_tiles_most = (p.max_query * p.group + 8 * plan.nt - 1) / (8 * plan.nt);
     p.causal = a.causal != 0;
     p.clear_tail = a.clear_tail != 0;
     p.vec_q = (uintptr_t)a.q % 16 == 0 && (a.q_row_stride | a.q_head_stride) % 8 == 0;
@@ -778,8 +734,8 @@ int pf_kv8_attention(int device_id, const pf_kv8_cache *cache, const pf_kv8_batc
     p.scale = a.scale;
     p.n_ctas = plan.n_ctas;
     DeviceGuard on_device(device_id);
-    if (a.dtype == PF_KV8_BF16) launch<true>(p, plan.nt, (cudaStream_t)stream);
-    else launch<false>(p, plan.nt, (cudaStream_t)stream);
+    if (a.dtype == PF_KV8_BF16) launch<true>(p, plan.nt, kv8_sm_count(device_id), (cudaStream_t)stream);
+    else launch<false>(p, plan.nt, kv8_sm_count(device_id), (cudaStream_t)stream);
   });
 }
 

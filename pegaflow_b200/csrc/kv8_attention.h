@@ -1,0 +1,166 @@
+// What the kernels of pf_kv8_attention share: parameters, the split of the work, partial results.
+#pragma once
+
+#include <cuda_fp16.h>
+
+#include "kv8.h"
+
+namespace pf {
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kNone = -1e30f;   // reference of a row that has seen nothing
+
+struct AttnParams {
+  Kv8View cache;
+  Kv8Batch batch;
+  const uint16_t *q;
+  uint16_t *out;
+  float *lse;
+  float *weights;
+  int64_t q_row, q_head, out_row, out_head, w_seq, w_head;
+  int w_capacity;
+  int q_heads, group, max_query;
+  int causal, clear_tail, vec_q, vec_out;
+  float scale;
+  // Partial results: slot 2 c + k of CTA c (k = 0: the segment that its range starts in, 1: the one that it ends in).
+  // part_ml holds (base, sum): the row's sum and its part_o are of terms 2^(score - base), scores in base 2.
+  float *part_o;    // [slots][rows][dim]
+  float2 *part_ml;  // [slots][rows]
+  int n_ctas;
+};
+
+// The work of all sequences, heads and row tiles laid end to end in units of some tokens; CTA c of n takes
+// [total c / n, total (c + 1) / n).  A segment is one (sequence, head, row tile).
+struct Split {
+  uint32_t total;
+  int n_ctas;       // at most total: every CTA that takes part has work
+  __device__ Split(uint32_t total, int n) : total(total), n_ctas((int)min((uint32_t)n, total)) {}
+  __device__ uint32_t begin(int c) const { return (uint32_t)((uint64_t)total * c / n_ctas); }
+  __device__ int owner(uint32_t u) const { return (int)((((uint64_t)u + 1) * n_ctas - 1) / total); }
+};
+
+// One sequence of a call: its rows (row = query * group + head of the group) in tiles of kRows, and its tokens.
+template <int kRows, int kUnit>
+struct Seq {
+  int row0, rows, len, row_tiles;
+  __device__ Seq(const AttnParams &p, int s) {
+    int hi;
+    p.batch.rows(s, row0, hi);
+    rows = min(hi - row0, p.max_query);
+    len = p.batch.length(s, p.cache.block_log2);
+    row_tiles = (rows * p.group + kRows - 1) / kRows;
+  }
+  __device__ int all_rows(const AttnParams &p) const { return rows * p.group; }
+  __device__ int visible(const AttnParams &p, int row) const {   // tokens that query row `row` sees
+    return p.causal ? min(max(len - rows + row / p.group + 1, 0), len) : len;
+  }
+  // Units of one row tile: those that its last row sees, one at least.
+  __device__ uint32_t units(const AttnParams &p, int rt) const {
+    return max(1, (visible(p, min((rt + 1) * kRows, all_rows(p)) - 1) + kUnit - 1) / kUnit);
+  }
+  __device__ uint32_t all_units(const AttnParams &p) const {
+    uint32_t n = 0;
+    for (int rt = 0; rt < row_tiles; ++rt) n += units(p, rt);
+    return n * (uint32_t)p.cache.heads;
+  }
+};
+
+// Where unit u lies: row tile, head, the unit within the segment, and the segment's extent.
+struct Segment {
+  int s, rt, head;
+  uint32_t begin, units;      // first unit of the segment in the whole, its units
+  template <int kRows, int kUnit>
+  __device__ Segment(const AttnParams &p, const Seq<kRows, kUnit> &seq, int s, uint32_t seq_begin, uint32_t u) : s(s) {
+    begin = seq_begin;
+    for (rt = 0;; ++rt) {
+      units = seq.units(p, rt);
+      const uint32_t all = units * (uint32_t)p.cache.heads;
+      if (u - begin < all || rt + 1 >= seq.row_tiles) break;
+      begin += all;
+    }
+    head = (int)((u - begin) / units);
+    begin += head * units;
+  }
+};
+
+// prefix[s] = units before sequence s, prefix[n_seqs] = all of them.  Every CTA of every kernel computes it for
+// itself: lens stay on the device, and no launch and no workspace is spent on it.
+template <class Units>
+__device__ void scan_units(const AttnParams &p, uint32_t *prefix, Units &&units_of) {
+  __shared__ uint32_t warp_sum[32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n_warps = blockDim.x >> 5;
+  uint32_t base = 0;
+  for (int s0 = 0; s0 < p.batch.n_seqs; s0 += blockDim.x) {
+    const int s = s0 + threadIdx.x;
+    const uint32_t mine = s < p.batch.n_seqs ? units_of(s) : 0u;
+    uint32_t x = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const uint32_t y = __shfl_up_sync(0xffffffffu, x, d);
+      if (lane >= d) x += y;
+    }
+    if (lane == 31) warp_sum[warp] = x;
+    __syncthreads();
+    uint32_t before = base, all = 0;
+    for (int w = 0; w < n_warps; ++w) {
+      if (w < warp) before += warp_sum[w];
+      all += warp_sum[w];
+    }
+    if (s < p.batch.n_seqs) prefix[s] = before + x - mine;
+    base += all;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) prefix[p.batch.n_seqs] = base;
+  __syncthreads();
+}
+
+__device__ __forceinline__ int find_seq(const uint32_t *prefix, int n, uint32_t u) {   // last s with prefix[s] <= u
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (prefix[mid] <= u) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+__device__ __forceinline__ uint32_t f16x2(float lo, float hi) {
+  uint32_t d;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+  return d;
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+  float d;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(d) : "f"(x));
+  return d;
+}
+template <bool kBf16>
+__device__ __forceinline__ float widen1(uint16_t x) {
+  return kBf16 ? __uint_as_float((uint32_t)x << 16) : __half2float(__ushort_as_half(x));
+}
+template <bool kBf16>
+__device__ __forceinline__ uint32_t narrow2(float lo, float hi) {
+  if (!kBf16) return f16x2(lo, hi);
+  uint32_t d;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+  return d;
+}
+
+// What cannot be checked before the launch, looked at by one CTA of it.
+__device__ __forceinline__ void check_batch(const AttnParams &p) {
+  if (p.batch.starts) p.batch.check_starts(p.max_query);
+  for (int s = threadIdx.x; s < p.batch.n_seqs; s += blockDim.x)
+    if (p.batch.lens[s] < 0 || p.batch.lens[s] > p.batch.length(s, p.cache.block_log2)) p.batch.report(PF_KV8_BAD_LENGTH);
+}
+
+__device__ __forceinline__ float lse_of(float base, float sum) { return sum == 0.f ? -INFINITY : (base + log2f(sum)) * kLn2; }
+
+// Query rows by the hundred (kv8_attention_wide.cu).
+struct WidePlan {
+  int rows, threads;
+  size_t smem;
+};
+WidePlan kv8_wide_plan(int dim);
+void kv8_wide_launch(const AttnParams &p, bool bf16, cudaStream_t stream);
+
+}  // namespace pf

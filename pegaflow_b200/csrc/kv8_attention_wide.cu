@@ -1,0 +1,583 @@
+// Attention over the 8-bit cache for many query rows (pf_kv8_attention): 256 rows of one KV head at a time on the
+// tcgen05 tensor cores, sums in tensor memory.
+//
+// A CTA takes a row tile (two groups of 128 rows; one at 256 dimensions) along a range of tokens, kTokens per step:
+//   converters  (4 warps)  read K8 and V8, turn them into f16 (exact) and lay them out in shared memory
+//   issuer      (1 thread) S_g = Q_g K^T into tensor memory;  O_g += P_g V, with P_g read from tensor memory
+//   softmax g   (4 warps)  a thread holds a row: scores out of tensor memory, running maximum, exponentials, P_g back into
+//                          the columns that held S_g, as f16; corrects O_g when the maximum has risen by 2^6
+// The two groups take turns: while one is in its exponentials, the other's products run.  Per step both cost about the same
+// at 128 dimensions: 4 * 256 * 128 * 128 flops at 8192 a cycle and 256 * 128 exponentials at 16 a cycle are 2048
+// cycles each.
+//
+// K and V have one layout in shared memory, rows of 128 bytes (64 dimensions) with 16-byte chunks swizzled over
+// eight rows: as the operand of the scores its contracted index runs along the row, as the operand of the output it runs
+// down the rows, which is the other of the two majors that a descriptor can name.
+//
+// Scales: K's goes on the scores, a block of 16 columns at a time.  V's, 2^e, goes on P: P holds
+// 2^(score - ref + shift + e - e_ref), and O is in units of 2^e_ref; e_ref follows the largest e so far.  The row sums
+// leave e out again.  All of these are powers of two.
+#include <cuda_bf16.h>
+
+#include "kv8_attention.h"
+
+namespace pf {
+namespace {
+
+constexpr int kGroupRows = 128;
+constexpr float kShift = 6.f, kSlack = 6.f;   // P <= 2^(6 + 6 + kRoom) = 2^15
+constexpr int kRoom = 3;                      // by how much e may exceed e_ref
+constexpr int kRing = 4;                      // steps of scales kept
+
+constexpr int tokens_of(int dim) { return dim == 256 ? 64 : 128; }
+constexpr int groups_of(int dim) { return dim == 256 ? 1 : 2; }
+constexpr int threads_of(int dim) { return 128 * groups_of(dim) + 128 + 32; }
+
+// Offsets in shared memory, behind the first 1024-byte boundary.
+template <int kDim>
+struct Layout {
+  static constexpr int kTokens = tokens_of(kDim), kGroups = groups_of(kDim);
+  static constexpr int q_bytes = kGroupRows * kDim * 2, kv_bytes = kTokens * kDim * 2, blocks = kTokens / 16;
+  static constexpr int q = 0, k = q + kGroups * q_bytes, v = k + 2 * kv_bytes, end = v + 2 * kv_bytes;
+};
+
+struct Shared {
+  uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2], scales_full[kRing];
+  uint32_t tmem;
+  int stalled, any_nan;
+  float k_scale[kRing][8];
+  int v_exp[kRing][8];       // exponent of V's scale; kHidden: the block is not in the cache
+  int nan_from[256];         // first token whose V is NaN in a dimension
+};
+constexpr int kHidden = 1 << 20;
+
+__device__ __forceinline__ uint32_t shared_of(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void bar_init(uint64_t *bar, int count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(shared_of(bar)), "r"(count) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(uint64_t *bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(shared_of(bar)) : "memory");
+}
+// Waits for the phase of `parity`; false after about two seconds, or as soon as another thread has given up.
+__device__ __forceinline__ bool bar_wait(uint64_t *bar, uint32_t parity, int *stalled) {
+  uint64_t start = 0;
+  for (uint32_t i = 1;; ++i) {
+    uint32_t done;
+    asm volatile("{.reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p;}"
+                 : "=r"(done)
+                 : "r"(shared_of(bar)), "r"(parity)
+                 : "memory");
+    if (done) return true;
+    if ((i & 255) == 0) {
+      uint64_t now;
+      asm volatile("mov.u64 %0, %globaltimer;" : "=l"(now));
+      if (start == 0) start = now;
+      if (*(volatile int *)stalled || now - start > 2000000000ull) {
+        *(volatile int *)stalled = 1;
+        return false;
+      }
+    }
+  }
+}
+// The same for a warp whose next instructions need all of its lanes.
+__device__ __forceinline__ bool bar_wait_warp(uint64_t *bar, uint32_t parity, int *stalled) {
+  return __all_sync(0xffffffffu, bar_wait(bar, parity, stalled));
+}
+
+__device__ __forceinline__ void fence_to_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void wait_stores() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void commit(uint64_t *bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(shared_of(bar)) : "memory");
+}
+// 128-byte swizzled operand: `lead` = bytes between 64-element panels along the rows of a matrix whose contracted index runs
+// down them (unused otherwise), 1024 bytes between groups of eight rows.
+__device__ __forceinline__ uint64_t operand(uint32_t addr, uint32_t lead) {
+  return (uint64_t)((addr >> 4) & 0x3fff) | (uint64_t)((lead >> 4) & 0x3fff) << 16 | (uint64_t)(1024 >> 4) << 32 |
+         (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+// f16 operands, fp32 sums, 128 rows, n columns; B contracted along its rows or down them.
+__host__ __device__ constexpr uint32_t shape(int n, bool b_down) {
+  return 1u << 4 | (b_down ? 1u << 16 : 0u) | (uint32_t)(n / 8) << 17 | (uint32_t)(kGroupRows / 16) << 24;
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t shape_, bool add) {
+  asm volatile(
+      "{.reg .pred p; setp.ne.u32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;}" ::"r"(d), "l"(a),
+      "l"(b), "r"(shape_), "r"((uint32_t)add)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t shape_, bool add) {
+  asm volatile(
+      "{.reg .pred p; setp.ne.u32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;}" ::"r"(d), "r"(a),
+      "l"(b), "r"(shape_), "r"((uint32_t)add)
+      : "memory");
+}
+#define PF_R4(r, i) "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3])
+#define PF_R16(r, i) PF_R4(r, i), PF_R4(r, i + 4), PF_R4(r, i + 8), PF_R4(r, i + 12)
+#define PF_I4(r, i) "r"(r[i]), "r"(r[i + 1]), "r"(r[i + 2]), "r"(r[i + 3])
+#define PF_I16(r, i) PF_I4(r, i), PF_I4(r, i + 4), PF_I4(r, i + 8), PF_I4(r, i + 12)
+__device__ __forceinline__ void load32(uint32_t (&r)[32], uint32_t at) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,"
+      "%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\ttcgen05.wait::ld.sync.aligned;"
+      : PF_R16(r, 0), PF_R16(r, 16)
+      : "r"(at)
+      : "memory");
+}
+__device__ __forceinline__ void store32(uint32_t at, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,"
+      "%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(at),
+      PF_I16(r, 0), PF_I16(r, 16)
+      : "memory");
+}
+__device__ __forceinline__ void store16(uint32_t at, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(at),
+      PF_I16(r, 0)
+      : "memory");
+}
+
+template <int kDim, bool kBf16>
+__global__ void __launch_bounds__(threads_of(kDim), 1) kv8_attention_wide(AttnParams p) {
+  using L = Layout<kDim>;
+  constexpr int kTokens = L::kTokens, kGroups = L::kGroups, kRows = kGroupRows * kGroups, kBlocks = L::blocks;
+  using SeqT = Seq<kRows, kTokens>;
+  // columns of tensor memory: S and P of each group, then O of each group
+  constexpr uint32_t kO = kDim == 256 ? 256 : 2 * kTokens;
+  extern __shared__ char raw[];
+  char *smem = raw + (1024 - (shared_of(raw) & 1023));
+  Shared &sh = *reinterpret_cast<Shared *>(smem + L::end);
+  uint32_t *prefix = reinterpret_cast<uint32_t *>(&sh + 1);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  constexpr int kConvert = 4 * kGroups, kIssue = kConvert + 4;     // first warp of the converters, warp of the issuer
+
+  if (tid == 0) {
+    bar_init(&sh.q_full, kRows);
+    for (int i = 0; i < 2; ++i) {
+      bar_init(&sh.k_full[i], 128);
+      bar_init(&sh.k_empty[i], 1);
+      bar_init(&sh.v_full[i], 128);
+      bar_init(&sh.v_empty[i], 1);
+      bar_init(&sh.s_full[i], 1);
+      bar_init(&sh.p_full[i], kGroupRows);
+      bar_init(&sh.o_full[i], 1);
+    }
+    for (int i = 0; i < kRing; ++i) bar_init(&sh.scales_full[i], kBlocks);
+    sh.stalled = 0;
+    sh.any_nan = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  for (int i = tid; i < kDim; i += blockDim.x) sh.nan_from[i] = INT_MAX;
+  if (warp == kIssue) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(shared_of(&sh.tmem)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  scan_units(p, prefix, [&](int s) { return SeqT(p, s).all_units(p); });
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = sh.tmem;
+  const int n_seqs = p.batch.n_seqs;
+  const Split split(prefix[n_seqs], p.n_ctas);
+  if (blockIdx.x == 0) check_batch(p);
+  uint32_t u = 0, u_end = 0;
+  if ((int)blockIdx.x < split.n_ctas) u = split.begin(blockIdx.x), u_end = split.begin(blockIdx.x + 1);
+  bool first_segment = true;
+  uint32_t step = 0;          // steps done in earlier segments: all roles count alike
+  uint32_t n_segment = 0;
+  bool ok = true;
+  while (u < u_end && ok) {
+    const int s = find_seq(prefix, n_seqs, u);
+    const SeqT seq(p, s);
+    const Segment seg(p, seq, s, prefix[s], u);
+    const uint32_t unit0 = u - seg.begin, units = min(seg.units - unit0, u_end - u);
+    const int row_first = seg.rt * kRows, live_rows = min(seq.all_rows(p) - row_first, kRows);
+    const int head = seg.head;
+    if (warp < kConvert) {
+      // ------------------------------------------------------------------ softmax: a thread holds a row
+      const int g = warp >> 2, r = (warp & 3) * 32 + lane;
+      const int row = row_first + g * kGroupRows + r;
+      const bool live = row < row_first + live_rows;
+      const int i = live ? row / p.group : 0, qh = head * p.group + (live ? row % p.group : 0);
+      const int see = live ? seq.visible(p, row) : 0;
+      const int group_least = g * kGroupRows < live_rows ? seq.visible(p, row_first + g * kGroupRows) : 0;
+      const bool dead = g * kGroupRows + (warp & 3) * 32 >= live_rows;   // no row of this warp counts
+      // the row into shared memory, a power of two (and the scale's sign) taken off it
+      float factor;
+      {
+        const uint16_t *src = p.q + (int64_t)(seq.row0 + i) * p.q_row + qh * p.q_head;
+        char *dst = smem + L::q + g * L::q_bytes + r * 128;
+        auto read8 = [&](int d) {
+          if (!live) return make_uint4(0, 0, 0, 0);
+          const uint16_t *at = src + d;
+          if (p.vec_q) return *reinterpret_cast<const uint4 *>(at);
+          return make_uint4(at[0] | at[1] << 16, at[2] | at[3] << 16, at[4] | at[5] << 16, at[6] | at[7] << 16);
+        };
+        auto wide2 = [](uint32_t two) {
+          if (kBf16) return make_float2(__uint_as_float(two << 16), __uint_as_float(two & 0xffff0000u));
+          return f32x2_from_f16x2(two);
+        };
+        float top = 0.f;
+        for (int d = 0; d < kDim; d += 8) {
+          const uint4 w = read8(d);
+          const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+          for (int m = 0; m < 4; ++m) {
+            const float2 f = wide2(x[m]);
+            top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
+          }
+        }
+        int e = (int)(__float_as_uint(top) >> 23) - 127 - 14;
+        if (top == 0.f || top > 3.4e38f) e = 0;
+        e = max(e, -126);
+        const float down = exp2i(-e) * (p.scale < 0.f ? -1.f : 1.f);
+        factor = fabsf(p.scale) * kLog2e * exp2i(e);
+        for (int d = 0; d < kDim; d += 8) {
+          const uint4 w = read8(d);
+          const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+          uint32_t h[4];
+#pragma unroll
+          for (int m = 0; m < 4; ++m) {
+            const float2 f = wide2(x[m]);
+            h[m] = f16x2(f.x * down, f.y * down);
+          }
+          *reinterpret_cast<uint4 *>(dst + d / 64 * (kGroupRows * 128) + ((d / 8 % 8) ^ (r & 7)) * 16) = make_uint4(h[0], h[1], h[2], h[3]);
+        }
+        fence_to_async();
+        bar_arrive(&sh.q_full);
+      }
+      const uint32_t lanes = tmem + ((uint32_t)(warp & 3) * 32 << 16);
+      const uint32_t s_col = lanes + g * kTokens, o_col = lanes + kO + g * kDim;
+      float ref = kNone, sum = 0.f;
+      int e_ref = 0;
+      for (uint32_t j = 0; j < units; ++j) {
+        const uint32_t at = step + j, ring = at % kRing;
+        const int tok = (int)((unit0 + j) * kTokens);
+        if (!(ok = bar_wait_warp(&sh.scales_full[ring], at / kRing & 1, &sh.stalled))) break;
+        if (!(ok = bar_wait_warp(&sh.s_full[g], at & 1, &sh.stalled))) break;
+        fence_after();
+        if (!dead) {
+          float f[kBlocks];
+          int ve[kBlocks], e_top = kKv8MinExp;
+          bool hidden = tok + kTokens > group_least;
+#pragma unroll
+          for (int b = 0; b < kBlocks; ++b) {
+            f[b] = factor * sh.k_scale[ring][b];
+            ve[b] = sh.v_exp[ring][b];
+            if (ve[b] == kHidden) hidden = true;
+            else e_top = max(e_top, ve[b]);
+          }
+          // largest score that the row sees
+          float top = kNone;
+#pragma unroll
+          for (int c = 0; c < kTokens / 32; ++c) {
+            uint32_t x[32];
+            load32(x, s_col + 32 * c);
+            if (!hidden) {
+#pragma unroll
+              for (int b = 0; b < 2; ++b) {
+                float m = __uint_as_float(x[16 * b]);
+#pragma unroll
+                for (int k = 1; k < 16; ++k) m = fmaxf(m, __uint_as_float(x[16 * b + k]));
+                top = fmaxf(top, m * f[2 * c + b]);
+              }
+            } else {
+#pragma unroll
+              for (int k = 0; k < 32; ++k)
+                if (tok + 32 * c + k < see && ve[2 * c + k / 16] != kHidden) top = fmaxf(top, __uint_as_float(x[k]) * f[2 * c + k / 16]);
+            }
+          }
+          // both references, and O with them
+          const bool start = j == 0;
+          if (start) e_ref = e_top;
+          float down = 1.f;
+          bool change = false;
+          if (top > ref + kSlack) {
+            if (!start) down = exp2_fast(ref - top), change = true;
+            sum *= exp2_fast(ref - top);
+            ref = top;
+          }
+          if (e_top > e_ref + kRoom) {
+            down *= exp2i(e_ref - e_top);
+            change = true;
+            e_ref = e_top;
+          }
+          if (__any_sync(0xffffffffu, change)) {
+            for (int c = 0; c < kDim / 32; ++c) {
+              uint32_t x[32];
+              load32(x, o_col + 32 * c);
+  #pragma unroll
+              for (int k = 0; k < 32; ++k) x[k] = __float_as_uint(__uint_as_float(x[k]) * down);
+              store32(o_col + 32 * c, x);
+            }
+          }
+#pragma unroll
+          for (int c = 0; c < kTokens / 32; ++c) {
+            uint32_t x[32], h[16];
+            load32(x, s_col + 32 * c);
+            uint32_t seen = 0xffffffffu;
+            if (hidden) {
+              const int n = see - (tok + 32 * c);
+              seen = n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1;
+              if (ve[2 * c] == kHidden) seen &= 0xffff0000u;
+              if (ve[2 * c + 1] == kHidden) seen &= 0x0000ffffu;
+            }
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+              const int de = ve[2 * c + b] == kHidden ? 0 : ve[2 * c + b] - e_ref;
+              // so far below e_ref, P would leave fp32's range and the row sum with it: the factor then goes on afterwards
+              const bool far = de < -60;
+              const float fb = f[2 * c + b], minus = kShift + (far ? 0.f : (float)de) - ref;
+              float part = 0.f;
+              auto entry = [&](int k) {
+                const float y = fmaf(__uint_as_float(x[16 * b + k]), fb, minus);
+                return exp2_fast(!hidden || (seen >> (16 * b + k) & 1) ? y : -INFINITY);
+              };
+#pragma unroll
+              for (int k = 0; k < 16; k += 2) {
+                const float a = entry(k), d = entry(k + 1);
+                part += a + d;
+                h[8 * b + k / 2] = far ? f16x2(a * exp2i(de), d * exp2i(de)) : f16x2(a, d);
+              }
+              sum = fmaf(part, far ? 1.f : exp2i(-de), sum);
+            }
+            store16(s_col + 16 * c, h);
+          }
+          wait_stores();
+        }
+        fence_before();
+        bar_arrive(&sh.p_full[g]);
+      }
+      if (ok) ok = bar_wait_warp(&sh.o_full[g], n_segment & 1, &sh.stalled);
+      const uint32_t last = step + units - 1;       // what the converters noted of NaN is seen behind their last arrival
+      if (ok) ok = bar_wait_warp(&sh.v_full[last & 1], last >> 1 & 1, &sh.stalled);
+      if (ok) {
+        fence_after();
+        const bool whole = units == seg.units;
+        const int slot = 2 * blockIdx.x + (first_segment ? 0 : 1), n = g * kGroupRows + r;
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        const bool nan = sh.any_nan;
+        uint16_t *dst = p.out + (int64_t)(seq.row0 + i) * p.out_row + qh * p.out_head;
+        float *part = p.part_o + ((int64_t)slot * kRows + n) * kDim;
+        if (!dead) {
+          for (int c = 0; c < kDim / 32; ++c) {
+            uint32_t x[32];
+            load32(x, o_col + 32 * c);
+            // O is in units of 2^e_ref; the two factors are applied one after the other, their product may leave the range
+            const float unit = exp2i(e_ref);
+#pragma unroll
+            for (int k = 0; k < 32; ++k) {
+              float y = sum == 0.f ? 0.f : __uint_as_float(x[k]) * unit;
+              if (whole) y *= inv;
+              if (nan && sh.nan_from[32 * c + k] < see) y = __int_as_float(0x7fffffff);
+              x[k] = __float_as_uint(y);
+            }
+            if (!live) continue;
+            if (whole) {
+              if (p.vec_out) {
+#pragma unroll
+                for (int k = 0; k < 32; k += 4) {
+                  const float *y = reinterpret_cast<const float *>(x) + k;
+                  uint2 w;
+                  if (kBf16) {
+                    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w.x) : "f"(y[1]), "f"(y[0]));
+                    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w.y) : "f"(y[3]), "f"(y[2]));
+                  } else {
+                    w = make_uint2(f16x2(y[0], y[1]), f16x2(y[2], y[3]));
+                  }
+                  *reinterpret_cast<uint2 *>(dst + 32 * c + k) = w;
+                }
+              } else {
+#pragma unroll
+                for (int k = 0; k < 32; ++k) {
+                  const float y = __uint_as_float(x[k]);
+                  dst[32 * c + k] = kBf16 ? __bfloat16_as_ushort(__float2bfloat16_rn(y)) : __half_as_ushort(__float2half_rn(y));
+                }
+              }
+            } else {
+#pragma unroll
+              for (int k = 0; k < 32; k += 4) *reinterpret_cast<uint4 *>(part + 32 * c + k) = make_uint4(x[k], x[k + 1], x[k + 2], x[k + 3]);
+            }
+          }
+        }
+        if (live) {
+          if (!whole) p.part_ml[slot * kRows + n] = make_float2(ref - kShift, sum);
+          else if (p.lse) p.lse[(int64_t)(seq.row0 + i) * p.q_heads + qh] = lse_of(ref - kShift, sum);
+        }
+        fence_before();
+      }
+    } else if (warp < kIssue) {
+      // ------------------------------------------------------------------ converters
+      constexpr int kLanes = kDim / 16, kVecs = kTokens * kLanes / 128;      // lanes of a row, 16-byte vectors of a thread
+      const int ct = tid - kConvert * 32, sub = ct % kLanes, row_of = ct / kLanes;
+      const int within = p.cache.block_size() - 1, tok_stop = seq.len;
+      auto fetch = [&](int kv, uint32_t j, uint4 (&x)[kVecs]) {
+#pragma unroll
+        for (int v = 0; v < kVecs; ++v) {
+          const int tok = (int)((unit0 + j) * kTokens) + v * (128 / kLanes) + row_of;
+          uint32_t id;
+          x[v] = make_uint4(0, 0, 0, 0);
+          if (tok < tok_stop && p.batch.block(p.cache, s, tok >> p.cache.block_log2, id))
+            x[v] = __ldg(reinterpret_cast<const uint4 *>(p.cache.tile(kv, id, head) + (tok & within) * kDim + 16 * sub));
+        }
+      };
+      auto lay = [&](char *base, const uint4 (&x)[kVecs]) {
+#pragma unroll
+        for (int v = 0; v < kVecs; ++v) {
+          const int t = v * (128 / kLanes) + row_of;
+          char *dst = base + sub / 4 * (kTokens * 128) + t * 128;
+          const uint4 a = make_uint4(f16x2_from_e4m3<0>(x[v].x), f16x2_from_e4m3<1>(x[v].x), f16x2_from_e4m3<0>(x[v].y), f16x2_from_e4m3<1>(x[v].y));
+          const uint4 b = make_uint4(f16x2_from_e4m3<0>(x[v].z), f16x2_from_e4m3<1>(x[v].z), f16x2_from_e4m3<0>(x[v].w), f16x2_from_e4m3<1>(x[v].w));
+          // lanes of odd panels store their second half first: eight lanes then fill eight different chunks
+          const int c = 2 * (sub % 4), odd = sub / 4 & 1;
+          *reinterpret_cast<uint4 *>(dst + ((c + odd) ^ (t & 7)) * 16) = odd ? b : a;
+          *reinterpret_cast<uint4 *>(dst + ((c + 1 - odd) ^ (t & 7)) * 16) = odd ? a : b;
+        }
+        fence_to_async();
+      };
+      uint4 kx[kVecs], vx[kVecs];
+      fetch(0, 0, kx);
+      for (uint32_t j = 0; j < units; ++j) {
+        const uint32_t at = step + j, stage = at & 1;
+        fetch(1, j, vx);
+        if (!(ok = bar_wait(&sh.k_empty[stage], (at >> 1 & 1) ^ 1, &sh.stalled))) break;
+        if (ct < kBlocks) {
+          const int tok = (int)((unit0 + j) * kTokens) + 16 * ct;
+          uint32_t id;
+          float ks = 0.f;
+          int ve = kHidden;
+          if (tok < tok_stop) {
+            if (p.batch.block(p.cache, s, tok >> p.cache.block_log2, id)) {
+              ks = __ldg(p.cache.scale(0, id, head));
+              ve = kv8_scale_exponent(__ldg(p.cache.scale(1, id, head)));
+            } else {
+              p.batch.report(PF_KV8_BAD_BLOCK);
+            }
+          }
+          sh.k_scale[at % kRing][ct] = ks;
+          sh.v_exp[at % kRing][ct] = ve;
+          bar_arrive(&sh.scales_full[at % kRing]);
+        }
+        lay(smem + L::k + stage * L::kv_bytes, kx);
+        bar_arrive(&sh.k_full[stage]);
+        if (j + 1 < units) fetch(0, j + 1, kx);
+        // A NaN in V reaches the rows that see its token and no other: it is taken out here and remembered.
+        bool any = false;
+#pragma unroll
+        for (int v = 0; v < kVecs; ++v) {
+          const uint32_t w[4] = {vx[v].x, vx[v].y, vx[v].z, vx[v].w};
+#pragma unroll
+          for (int m = 0; m < 4; ++m) any |= __vcmpeq4(w[m] & 0x7f7f7f7fu, 0x7f7f7f7fu) != 0;
+        }
+        if (any) {
+          sh.any_nan = 1;
+#pragma unroll
+          for (int v = 0; v < kVecs; ++v) {
+            uint32_t *w = reinterpret_cast<uint32_t *>(&vx[v]);
+            const int tok = (int)((unit0 + j) * kTokens) + v * (128 / kLanes) + row_of;
+            for (int b = 0; b < 16; ++b)
+              if ((w[b / 4] >> (8 * (b % 4)) & 0x7f) == 0x7f) {
+                atomicMin(&sh.nan_from[16 * sub + b], tok);
+                w[b / 4] &= ~(0xffu << (8 * (b % 4)));
+              }
+          }
+        }
+        if (!(ok = bar_wait(&sh.v_empty[stage], (at >> 1 & 1) ^ 1, &sh.stalled))) break;
+        lay(smem + L::v + stage * L::kv_bytes, vx);
+        bar_arrive(&sh.v_full[stage]);
+      }
+    } else if (lane == 0) {
+      // ------------------------------------------------------------------ issuer
+      constexpr uint32_t kScores = shape(kTokens, false), kOutput = shape(kDim, true);
+      auto scores = [&](int g, uint32_t stage) {
+        const uint32_t a = shared_of(smem + L::q + g * L::q_bytes), b = shared_of(smem + L::k + stage * L::kv_bytes);
+#pragma unroll
+        for (int k = 0; k < kDim / 16; ++k)
+          mma_ss(tmem + g * kTokens, operand(a + k / 4 * (kGroupRows * 128) + k % 4 * 32, 16),
+                 operand(b + k / 4 * (kTokens * 128) + k % 4 * 32, 16), kScores, k != 0);
+      };
+      auto output = [&](int g, uint32_t stage, bool add) {
+        const uint32_t b = shared_of(smem + L::v + stage * L::kv_bytes);
+#pragma unroll
+        for (int k = 0; k < kTokens / 16; ++k)
+          mma_ts(tmem + kO + g * kDim, tmem + g * kTokens + 8 * k, operand(b + k * 2048, kTokens * 128), kOutput, add || k != 0);
+      };
+      const int n_groups = live_rows > kGroupRows ? 2 : 1;
+      ok = bar_wait(&sh.q_full, n_segment & 1, &sh.stalled);
+      for (uint32_t j = 0; j <= units && ok; ++j) {
+        const uint32_t at = step + j, before = at - 1;
+        if (j < units && !(ok = bar_wait(&sh.k_full[at & 1], at >> 1 & 1, &sh.stalled))) break;
+        for (int g = 0; g < kGroups; ++g) {
+          if (j > 0) {
+            if (!(ok = bar_wait(&sh.p_full[g], before & 1, &sh.stalled))) break;
+            if (!(ok = bar_wait(&sh.v_full[before & 1], before >> 1 & 1, &sh.stalled))) break;
+            fence_after();
+            if (g < n_groups) output(g, before & 1, j > 1);
+            if (g == kGroups - 1) commit(&sh.v_empty[before & 1]);
+            if (j == units) commit(&sh.o_full[g]);
+          }
+          if (j < units) {
+            fence_after();
+            if (g < n_groups) scores(g, at & 1);
+            commit(&sh.s_full[g]);
+            if (g == kGroups - 1) commit(&sh.k_empty[at & 1]);
+          }
+        }
+      }
+    }
+    step += units;
+    ++n_segment;
+    u += units;
+    first_segment = false;
+    __syncwarp();
+    // every thread is through with this segment's marks before the next one sets them
+    if (u < u_end) {
+      if (__syncthreads_or(sh.stalled)) break;
+      if (sh.any_nan) {
+        __syncthreads();
+        for (int k = tid; k < kDim; k += blockDim.x) sh.nan_from[k] = INT_MAX;
+        if (tid == 0) sh.any_nan = 0;
+      }
+      __syncthreads();
+    }
+  }
+  // Everything that was issued has completed (the last commit was waited for), or a wait ran out.
+  __syncwarp();
+  fence_before();
+  __syncthreads();
+  fence_after();
+  if (sh.stalled && tid == 0) p.batch.report(PF_KV8_STALLED);
+  if (warp == kIssue) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+}
+
+template <int kDim, bool kBf16>
+void launch(const AttnParams &p, cudaStream_t stream) {
+  auto kernel = kv8_attention_wide<kDim, kBf16>;
+  const size_t smem = kv8_wide_plan(kDim).smem + ((size_t)p.batch.n_seqs + 1) * 4;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+    throw Error::storage("cudaFuncSetAttribute failed");
+  kernel<<<p.n_ctas, threads_of(kDim), smem, stream>>>(p);
+  PF_KV8_LAUNCHED();
+}
+
+}  // namespace
+
+static_assert(1024 + Layout<128>::end + sizeof(Shared) + 4 * (PF_KV8_MAX_SEQS + 1) + 128 <= 227 * 1024, "shared memory");
+static_assert(Layout<256>::end <= Layout<128>::end && Layout<64>::end <= Layout<128>::end, "shared memory");
+
+WidePlan kv8_wide_plan(int dim) {
+  const int end = dim == 64 ? Layout<64>::end : dim == 128 ? Layout<128>::end : Layout<256>::end;
+  return WidePlan{kGroupRows * groups_of(dim), threads_of(dim), 1024 + (size_t)end + sizeof(Shared)};
+}
+
+void kv8_wide_launch(const AttnParams &p, bool bf16, cudaStream_t stream) {
+  switch (p.cache.dim) {
+    case 64: return bf16 ? launch<64, true>(p, stream) : launch<64, false>(p, stream);
+    case 128: return bf16 ? launch<128, true>(p, stream) : launch<128, false>(p, stream);
+    default: return bf16 ? launch<256, true>(p, stream) : launch<256, false>(p, stream);
+  }
+}
+
+}  // namespace pf

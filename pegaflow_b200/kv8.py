@@ -95,7 +95,8 @@ class Kv8Cache:
             self._status.zero_()
             what = [text for bit, text in ((N.KV8_BAD_BLOCK, "a block id outside the cache"),
                                            (N.KV8_BAD_LENGTH, "a length below 0 or above what block tables or weights hold"),
-                                           (N.KV8_BAD_ROWS, "row starts that fall, leave the tensors or exceed max_query"))
+                                           (N.KV8_BAD_ROWS, "row starts that fall, leave the tensors or exceed max_query"),
+                                           (N.KV8_STALLED, "a wait inside a kernel ran out: the outputs are not valid"))
                     if bits & bit]
             _refuse("8-bit cache: " + "; ".join(what))
 

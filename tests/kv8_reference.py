@@ -95,7 +95,7 @@ def attention(q, cache, tables, lens, starts, scale, causal):
                     p = torch.exp(sc - lse[i, g])
                     out[i, g] = p @ v[:see]
                     size_of[i, g] = p @ v[:see].abs()
-                    spread[i, g] = (k[:see].abs() @ x.abs()).max() * scale
+                    spread[i, g] = (k[:see].abs() @ x.abs()).max() * abs(scale)
                     weights[s][head][:see] += p
     return out, lse, size_of, spread, weights
 

@@ -5,7 +5,8 @@ Tolerances of attention, from the kernel's arithmetic (u32 = 2^-24, halves of a 
            magnitudes, truncation included), scaled and turned to base 2 (three roundings):
            ds = (dim + 8) * 2^-23 * spread, spread = scale * max_j sum |q k|
   p        exp2 of it: ds + 2^-21 relative; f16 for the product with V: 2^-11 more; each p below 2^-24 of f16's
-           range by 2^-25 - kShift against the largest: less than n * 2^-33 of the largest |v|
+           range by half its smallest step, 2^-25, in units of 2^-9 (few rows) or of 2^-6 and the largest scale so far
+           (more than 16 rows): less than n * 2^-33 or n * 2^-31 of the largest |v|
   sums     fp32 over at most n terms: n * 2^-24
   out      sum p |v| * (2 (ds + 2^-21) + 2^-11 + 2 n 2^-24) + half a step of its type
 """
@@ -184,7 +185,7 @@ def check_attention(pf, cache, q, tables, lens, counts, *, causal=True, scale=No
     ds = (dim + 8) * 2.0 ** -23 * spread
     rel = 2 * (ds + 2.0 ** -21) + 2.0 ** -11 + 2 * longest * 2.0 ** -24
     big = (rc.values.abs().nan_to_num() * rc.scales[..., None, None]).max() if longest else 0.0
-    tol = size * rel[..., None] + HALF[q.dtype] * want.abs() + big * longest * 2.0 ** -33 + 1e-30
+    tol = size * rel[..., None] + HALF[q.dtype] * want.abs() + big * longest * (2.0 ** -33 if max(counts) * q.shape[1] / heads <= 16 else 2.0 ** -31) + 1e-30
     nan = torch.isnan(want)
     assert torch.equal(torch.isnan(got_), nan)
     off = ((got_ - want).abs() - tol)[~nan]
@@ -221,6 +222,13 @@ ATTENTION = [
     (torch.float16, 32, 1, 3, 64, [90, 20], [35, 20]),
     (torch.bfloat16, 16, 1, 2, 128, [3], [10]),          # more rows than tokens: the first ones see nothing
     (torch.float16, 16, 1, 4, 128, [2100], [2]),
+    # many rows: tiles of 256 (128 at 256 dimensions)
+    (torch.bfloat16, 16, 2, 4, 128, [700, 0, 300], [130, 0, 65]),
+    (torch.float16, 64, 1, 2, 64, [1500, 128], [200, 128]),
+    (torch.bfloat16, 32, 1, 1, 256, [400, 90], [150, 90]),
+    (torch.bfloat16, 16, 1, 8, 128, [2000], [33]),
+    (torch.float16, 128, 3, 17, 128, [257, 1], [1, 1]),
+    (torch.float16, 16, 1, 3, 128, [40], [100]),
 ]
 
 
@@ -296,6 +304,14 @@ def test_attention_over_scales_far_apart(pf):
     check_attention(pf, cache, (q * 2.0 ** -20), tables, lens, [1], scale=2.0 ** 18)
     check_attention(pf, cache, (q.float() * 2.0 ** 100).bfloat16(), tables, lens, [1], scale=2.0 ** -104)
     check_attention(pf, cache, q * 0, tables, lens, [1], weights=True)
+    q = torch.randn((20, 4, 128), generator=gen(44), device="cuda").bfloat16() * 8
+    check_attention(pf, cache, q, tables, lens, [20], weights=True)
+    check_attention(pf, cache, (q * 2.0 ** -20), tables, lens, [20], scale=-2.0 ** 18)
+    cache.values[1, tables[0, 4].item()] = 0               # a block of zeros: the smallest scale
+    cache.scales[1, tables[0, 4].item()] = 2.0 ** -110
+    check_attention(pf, cache, (q.float() * 2.0 ** 100).bfloat16(), tables, lens, [20], scale=2.0 ** -104)
+    check_attention(pf, cache, q * 0, tables, lens, [20], weights=True)
+    check_attention(pf, cache, q, tables, lens, [20], scale=0.0)
 
 
 def test_attention_is_the_same_on_every_run(pf):
