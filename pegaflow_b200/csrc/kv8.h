@@ -106,6 +106,12 @@ __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
   return d;
 }
 __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) { return e4m3x2(a, b) | (e4m3x2(c, d) << 16); }
+__device__ __forceinline__ uint32_t e4m3x4_from_f16(uint32_t a, uint32_t b) {
+  uint16_t x, y;
+  asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(x) : "r"(a));
+  asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(y) : "r"(b));
+  return x | (uint32_t)y << 16;
+}
 // Exact: every e4m3 value is an f16 value.  `half` selects the low or the high two bytes of `w`.
 template <int half>
 __device__ __forceinline__ uint32_t f16x2_from_e4m3(uint32_t w) {
@@ -121,15 +127,32 @@ __device__ __forceinline__ float2 f32x2_from_f16x2(uint32_t h) {
   return r;
 }
 
+// Kernels follow each other closely: each is launched with launch_after, may start while the one before it on the stream
+// drains, and every thread of it calls after_previous() before it touches what earlier work wrote.  The wait comes
+// before the permission to start the next kernel, so that a kernel that has started knows that everything before its
+// predecessor is complete: a call's later kernels may read the caller's lens and starts ahead of their own wait.
+__device__ __forceinline__ void after_previous() {
+  asm volatile("griddepcontrol.wait;\n\tgriddepcontrol.launch_dependents;" ::: "memory");
+}
+template <class... Params, class... Args>
+void launch_after(void (*kernel)(Params...), dim3 grid, int threads, size_t smem, cudaStream_t stream, Args... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, Params(args)...);
+  if (e != cudaSuccess) throw Error::storage(strf("kernel launch failed: %s", cudaGetErrorString(e)));
+}
+
 // Host side of every call: checks of the arguments that all of them take.
 Kv8View kv8_check_cache(const pf_kv8_cache *cache);
 Kv8Batch kv8_check_batch(const pf_kv8_batch *batch, size_t n_rows);
 int kv8_sm_count(int device_id);   // throws CudaInit for a device that is not there
-
-#define PF_KV8_LAUNCHED()                                                                                   \
-  do {                                                                                                      \
-    cudaError_t e_ = cudaGetLastError();                                                                    \
-    if (e_ != cudaSuccess) throw Error::storage(strf("kernel launch failed: %s", cudaGetErrorString(e_))); \
-  } while (0)
 
 }  // namespace pf

@@ -3,6 +3,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <algorithm>
 #include <atomic>
 
 #include "kv8.h"
@@ -89,18 +90,39 @@ __device__ __forceinline__ float2 widen(uint32_t two) {
   if (kBf16) return make_float2(__uint_as_float(two << 16), __uint_as_float(two & 0xffff0000u));
   return f32x2_from_f16x2(two);
 }
+// Largest finite magnitude of eight elements, as bits of their type: magnitudes order like integers.
+template <bool kBf16>
+__device__ __forceinline__ uint32_t finite_top(const uint4 &v) {
+  constexpr uint32_t kInf = kBf16 ? 0x7f80u : 0x7c00u;
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  uint32_t top = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t lo = w[j] & 0x7fff, hi = w[j] >> 16 & 0x7fff;
+    top = max(top, max(lo < kInf ? lo : 0u, hi < kInf ? hi : 0u));
+  }
+  return top;
+}
 
-// One CTA writes one (touched block, head, K or V): block_size * head_dim / 32 threads, each with four vectors of
-// eight elements in registers, so that the rows are read once: largest magnitude, then scale, then store.
+// One warp writes 2048 elements of a tile ((touched block, head, K or V), block_size * head_dim elements; kWarps warps
+// hold one tile), eight vectors of eight a lane, in registers: read once, largest magnitude, scale, store.
+// It is bound by HBM: 2 bytes read and 1 written for each element.  What it took to come near it: packed 16-bit maxima
+// (infinities and NaN are looked at only where one was met), and eight warps to a CTA, because finding the block
+// of an item is a chain of four dependent loads that many warps have to share.
 //
 // Work items: sequence s with n > 0 new rows touches at most n / bs + 2 blocks.  Items f(s) = starts[s] / bs + 2 s
 // onwards are its own; f(s + 1) - f(s) >= touched blocks, whatever lens holds, so the grid is sized without reading
 // lens and a CTA finds its sequence by bisection.  Surplus items return.
-template <bool kBf16, bool kVec>
-__global__ void __launch_bounds__(1024) kv8_append_kernel(Kv8View cache, Kv8Batch batch, AppendSource src) {
-  const int bl = cache.block_log2, bs = 1 << bl;
-  const int item = blockIdx.x, head = blockIdx.y, kv = blockIdx.z;
-  if (batch.starts && item == 0 && head == 0 && kv == 0) batch.check_starts(batch.n_rows);
+__host__ __device__ constexpr int append_warps(int warps) { return warps < 8 ? 8 : warps; }   // of a CTA
+
+template <bool kBf16, bool kVec, int kWarps>
+__global__ void __launch_bounds__(32 * append_warps(kWarps)) kv8_append_kernel(Kv8View cache, Kv8Batch batch, AppendSource src) {
+  constexpr int kTiles = append_warps(kWarps) / kWarps;     // tiles of a CTA
+  const int bl = cache.block_log2, bs = 1 << bl, dim_log2 = 31 - __clz(cache.dim);
+  const int item = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int which = blockIdx.y * kTiles + warp / kWarps, head = which >> 1, kv = which & 1, part = warp % kWarps;
+  after_previous();
+  if (batch.starts && item == 0 && blockIdx.y == 0) batch.check_starts(batch.n_rows);
   int lo = 0, hi = batch.n_seqs;   // last s with f(s) <= item
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
@@ -116,14 +138,12 @@ __global__ void __launch_bounds__(1024) kv8_append_kernel(Kv8View cache, Kv8Batc
   const int index = item - ((row0 >> bl) + 2 * seq);
   const int len_raw = batch.lens[seq];
   const int64_t cap = (int64_t)batch.max_blocks << bl;
-  const bool reporter = threadIdx.x == 0 && index == 0 && head == 0 && kv == 0;
   if (len_raw < 0 || len_raw + (int64_t)n > cap) {
-    if (reporter) batch.report(PF_KV8_BAD_LENGTH);
+    if (threadIdx.x == 0 && index == 0 && blockIdx.y == 0) batch.report(PF_KV8_BAD_LENGTH);
     if (len_raw < 0) return;
   }
   const int64_t len = len_raw;
-  const int64_t first_block = len >> bl;
-  const int64_t b = first_block + index;
+  const int64_t b = (len >> bl) + index;
   const int64_t tok0 = b << bl;                           // first token of this block
   if (index < 0 || tok0 >= len + n || tok0 >= cap) return;
   uint32_t id;
@@ -131,45 +151,53 @@ __global__ void __launch_bounds__(1024) kv8_append_kernel(Kv8View cache, Kv8Batc
     if (threadIdx.x == 0) batch.report(PF_KV8_BAD_BLOCK);
     return;
   }
+  const bool mine = head < cache.heads;                                  // the last CTA of an item may have warps to spare
   const int old_rows = (int)max((int64_t)0, len - tok0);                 // rows of the block that were there before
-  const int end_row = (int)min((int64_t)bs, len + n - tok0);
-  const uint16_t *x = src.ptr[kv] + head * src.head_stride[kv] + (row0 + (tok0 - len)) * src.row_stride[kv];
-  uint8_t *tile = cache.tile(kv, id, head);
-  float *scale_ptr = cache.scale(kv, id, head);
-  const int T = blockDim.x, dim = cache.dim;
+  const int end_row = mine ? (int)min((int64_t)bs, len + n - tok0) : 0;
+  const int64_t row_stride = src.row_stride[kv];
+  const uint16_t *x = src.ptr[kv] + head * src.head_stride[kv] + (row0 + (tok0 - len)) * row_stride;
 
-  uint4 v[4];
-  uint32_t top = 0;
+  uint4 v[8];
+  uint32_t tops = 0;                                                     // of both halves of a pair
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int e = (i * T + (int)threadIdx.x) * 8, row = e / dim, col = e % dim;
+  for (int i = 0; i < 8; ++i) {
+    const int e = ((part * 8 + i) * 32 + lane) * 8, row = e >> dim_log2, col = e & (cache.dim - 1);
     v[i] = make_uint4(0, 0, 0, 0);
     if (row >= old_rows && row < end_row) {
-      const uint16_t *p = x + row * src.row_stride[kv] + col;
-      if (kVec) {
-        v[i] = *reinterpret_cast<const uint4 *>(p);
-      } else {
-        v[i] = make_uint4(p[0] | p[1] << 16, p[2] | p[3] << 16, p[4] | p[5] << 16, p[6] | p[7] << 16);
-      }
-    }
-    const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float2 f = widen<kBf16>(w[j]);
-      top = max(top, max(kv8_magnitude(f.x), kv8_magnitude(f.y)));
+      const uint16_t *p = x + row * row_stride + col;
+      if (kVec) v[i] = __ldg(reinterpret_cast<const uint4 *>(p));
+      else v[i] = make_uint4(p[0] | p[1] << 16, p[2] | p[3] << 16, p[4] | p[5] << 16, p[6] | p[7] << 16);
     }
   }
-  __shared__ uint32_t tops[32];
-  top = __reduce_max_sync(0xffffffffu, top);
-  if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
-  const int e_old = old_rows ? kv8_scale_exponent(*scale_ptr) : kKv8MinExp;   // read before the barrier, written behind it
-  __syncthreads();
-  for (int w = 0; w < T / 32; ++w) top = max(top, tops[w]);
-  const int e = max(e_old, kv8_exponent(top));
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t a = __vmaxu2(v[i].x & 0x7fff7fffu, v[i].y & 0x7fff7fffu), c = __vmaxu2(v[i].z & 0x7fff7fffu, v[i].w & 0x7fff7fffu);
+    tops = __vmaxu2(tops, __vmaxu2(a, c));
+  }
+  uint32_t top = __reduce_max_sync(0xffffffffu, max(tops & 0xffff, tops >> 16));
+  if (top >= (kBf16 ? 0x7f80u : 0x7c00u)) {                              // an infinity or a NaN
+    top = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = max(top, finite_top<kBf16>(v[i]));
+    top = __reduce_max_sync(0xffffffffu, top);
+  }
+  uint8_t *tile = cache.tile(kv, id, mine ? head : 0);
+  float *scale_ptr = cache.scale(kv, id, mine ? head : 0);
+  const int e_old = old_rows ? kv8_scale_exponent(*scale_ptr) : kKv8MinExp;
+  if (kWarps > 1) {                          // every warp has read the old scale before one writes the new
+    __shared__ uint32_t sh_top[append_warps(kWarps)];
+    if (lane == 0) sh_top[warp] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) top = max(top, sh_top[warp / kWarps * kWarps + w]);
+  }
+  __syncwarp();
+  if (!mine) return;
+  const int e = max(e_old, kv8_exponent(__float_as_uint(widen<kBf16>(top).x)));
   const float inv = exp2i(-e), old_factor = exp2i(e_old - e);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int el = (i * T + (int)threadIdx.x) * 8, row = el / dim;
+  for (int i = 0; i < 8; ++i) {
+    const int el = ((part * 8 + i) * 32 + lane) * 8, row = el >> dim_log2;
     uint2 *out = reinterpret_cast<uint2 *>(tile + el);
     if (row >= old_rows && row < end_row) {
       const float2 a = widen<kBf16>(v[i].x), c = widen<kBf16>(v[i].y), d = widen<kBf16>(v[i].z), f = widen<kBf16>(v[i].w);
@@ -182,7 +210,23 @@ __global__ void __launch_bounds__(1024) kv8_append_kernel(Kv8View cache, Kv8Batc
       *out = make_uint2(e4m3x4(a.x * r, a.y * r, c.x * r, c.y * r), e4m3x4(d.x * r, d.y * r, f.x * r, f.y * r));
     }
   }
-  if (threadIdx.x == 0) *scale_ptr = exp2i(e);
+  if (lane == 0 && part == 0) *scale_ptr = exp2i(e);
+}
+
+template <bool kBf16, bool kVec>
+void launch_append(const Kv8View &c, const Kv8Batch &b, const AppendSource &src, unsigned items, cudaStream_t s) {
+  const int warps = std::max(1, (int)(c.tile_bytes() / 2048));      // of a tile: 1, 2, 4, 8 or 16
+  auto go = [&](auto kernel, int tile_warps) {
+    const int tiles = append_warps(tile_warps) / tile_warps;
+    launch_after(kernel, dim3(items, (2 * c.heads + tiles - 1) / tiles), 32 * append_warps(tile_warps), 0, s, c, b, src);
+  };
+  switch (warps) {
+    case 1: return go(kv8_append_kernel<kBf16, kVec, 1>, 1);
+    case 2: return go(kv8_append_kernel<kBf16, kVec, 2>, 2);
+    case 4: return go(kv8_append_kernel<kBf16, kVec, 4>, 4);
+    case 8: return go(kv8_append_kernel<kBf16, kVec, 8>, 8);
+    default: return go(kv8_append_kernel<kBf16, kVec, 16>, 16);
+  }
 }
 
 }  // namespace
@@ -216,18 +260,11 @@ int pf_kv8_append(int device_id, const pf_kv8_cache *cache, const pf_kv8_batch *
                      (k_row_stride | k_head_stride | v_row_stride | v_head_stride) % 8 == 0;
     const size_t items = (n_rows >> c.block_log2) + 2 * (size_t)b.n_seqs;
     kv8_sm_count(device_id);
-    const dim3 grid((unsigned)items, c.heads, 2);
-    const int threads = (int)(c.tile_bytes() / 32);
     DeviceGuard on_device(device_id);
     cudaStream_t s = (cudaStream_t)stream;
-    if (dtype == PF_KV8_BF16) {
-      if (vec) kv8_append_kernel<true, true><<<grid, threads, 0, s>>>(c, b, src);
-      else kv8_append_kernel<true, false><<<grid, threads, 0, s>>>(c, b, src);
-    } else {
-      if (vec) kv8_append_kernel<false, true><<<grid, threads, 0, s>>>(c, b, src);
-      else kv8_append_kernel<false, false><<<grid, threads, 0, s>>>(c, b, src);
-    }
-    PF_KV8_LAUNCHED();
+    const bool bf16 = dtype == PF_KV8_BF16;
+    if (bf16) vec ? launch_append<true, true>(c, b, src, (unsigned)items, s) : launch_append<true, false>(c, b, src, (unsigned)items, s);
+    else vec ? launch_append<false, true>(c, b, src, (unsigned)items, s) : launch_append<false, false>(c, b, src, (unsigned)items, s);
   });
 }
 

@@ -152,12 +152,12 @@ struct VTile {
     }
   }
   __device__ bool has_nan() const {   // a byte 0x7f or 0xff
-    bool any = false;
+    uint32_t any = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int x = 0; x < kWords; ++x) any |= __vcmpeq4(w[i][x] & 0x7f7f7f7fu, 0x7f7f7f7fu) != 0;
-    return any;
+      for (int x = 0; x < kWords; ++x) any |= (w[i][x] & 0x7f7f7f7fu) + 0x01010101u;
+    return any & 0x80808080u;
   }
 };
 
@@ -173,35 +173,23 @@ __device__ __forceinline__ void clear_behind(VTile<kDim> &v, int first_hidden) {
       for (int x = 0; x < VTile<kDim>::kWords; ++x) v.w[i][x] = 0;
 }
 
-// A NaN in V reaches the rows that see its token, and no other: 0 * NaN would.  Called for tiles that some row sees in part
-// and that hold a NaN: marks the outputs of the rows that see it and takes it out of the tile.
-template <int kDim, int kNt>
-__device__ __noinline__ void spread_nan(VTile<kDim> &v, float (&o)[kNt][kDim / 16][4], const int (&see)[kNt][2], int tok) {
-  const int lane = threadIdx.x & 31;
+// A NaN in V reaches the rows that see its token and no other: 0 * NaN would.  In tiles that some row sees in part it is
+// taken out, and the first such token is remembered for each dimension.
+__device__ __noinline__ void note_nan(uint32_t word, int *nan_from, int token) {
+  for (int b = 0; b < 4; ++b)
+    if ((word >> (8 * b) & 0x7f) == 0x7f) atomicMin(nan_from + b, token);
+}
+template <int kDim>
+__device__ __forceinline__ void take_nan_out(VTile<kDim> &v, int *nan_from, int tok) {
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
-    for (int from = 0; from < 4; ++from) {
-      const int token = tok + 2 * from + (i & 1) + 8 * (i >> 1);
 #pragma unroll
-      for (int x = 0; x < VTile<kDim>::kWords; ++x) {
-        const uint32_t w = __shfl_sync(0xffffffffu, v.w[i][x], (lane & ~3) | from);
-#pragma unroll
-        for (int b = 0; b < 4; ++b)
-          if (((w >> (8 * b)) & 0x7f) == 0x7f)
-#pragma unroll
-            for (int j = 0; j < kNt; ++j)
-#pragma unroll
-              for (int k = 0; k < 2; ++k)
-                if (token < see[j][k]) o[j][2 * x + b / 2][k + 2 * (b & 1)] = __int_as_float(0x7fffffff);
-      }
+    for (int x = 0; x < VTile<kDim>::kWords; ++x) {
+      const uint32_t w = v.w[i][x], mask = (((w & 0x7f7f7f7fu) + 0x01010101u) >> 7 & 0x01010101u) * 255u;
+      if (mask) note_nan(w, nan_from + g * (kDim / 8) + 4 * x, tok + 2 * t + (i & 1) + 8 * (i >> 1));
+      v.w[i][x] = w & ~mask;
     }
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int x = 0; x < VTile<kDim>::kWords; ++x)
-#pragma unroll
-      for (int b = 0; b < 4; ++b)
-        if (((v.w[i][x] >> (8 * b)) & 0x7f) == 0x7f) v.w[i][x] &= ~(0xffu << (8 * b));
 }
 
 // A block of the sequence's table, looked up ahead of its use.
@@ -222,6 +210,10 @@ __global__ void __launch_bounds__(kThreads, ctas_of(kDim, kNt)) kv8_attention_ro
   float *sh_o = reinterpret_cast<float *>(smem);                       // [kWarps][kRows][kDim]
   float2 *sh_ml = reinterpret_cast<float2 *>(sh_o + kWarps * kRows * kDim);   // [kWarps][kRows]
   uint32_t *prefix = reinterpret_cast<uint32_t *>(sh_ml + kWarps * kRows);    // [n_seqs + 1]
+  __shared__ int sh_nan_from[kDim], sh_any_nan;
+  after_previous();
+  for (int i = threadIdx.x; i < kDim; i += kThreads) sh_nan_from[i] = INT_MAX;
+  if (threadIdx.x == 0) sh_any_nan = 0;
   scan_units(p, prefix, [&](int s) { return SeqT(p, s).all_units(p); });
   const int n_seqs = p.batch.n_seqs, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const Split split(prefix[n_seqs], p.n_ctas);
@@ -304,7 +296,10 @@ __global__ void __launch_bounds__(kThreads, ctas_of(kDim, kNt)) kv8_attention_ro
               if (tok + g + 8 >= see[j][k]) c[j][k + 2] = -INFINITY;
             }
           if (tok + kTile > seq.len) clear_behind(vt, seq.len - tok);
-          if (__any_sync(0xffffffffu, vt.has_nan())) spread_nan<kDim, kNt>(vt, o, see, tok);
+          if (vt.has_nan()) {
+            sh_any_nan = 1;
+            take_nan_out(vt, sh_nan_from, tok);
+          }
         }
         bool over = false;
 #pragma unroll
@@ -403,6 +398,13 @@ __global__ void __launch_bounds__(kThreads, ctas_of(kDim, kNt)) kv8_attention_ro
         const float4 x = *reinterpret_cast<const float4 *>(sh_o + (w * kRows + n) * kDim + d);
         a.x += x.x, a.y += x.y, a.z += x.z, a.w += x.w;
       }
+      if (sh_any_nan) {
+        const int see_row = seq.visible(p, row_first + n);
+        float *y = &a.x;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (sh_nan_from[d + k] < see_row) y[k] = __int_as_float(0x7fffffff);
+      }
       if (whole) {
         const int row = row_first + n, i = row / p.group, qh = head * p.group + row % p.group;
         const float inv = l == 0.f ? 0.f : 1.f / l;
@@ -416,37 +418,45 @@ __global__ void __launch_bounds__(kThreads, ctas_of(kDim, kNt)) kv8_attention_ro
         if (d == 0) p.part_ml[slot * kRows + n] = make_float2(top - kShift, l);
       }
     }
+    const bool any_nan = sh_any_nan;
     __syncthreads();
     u += units;
     first_segment = false;
+    if (any_nan) {
+      for (int i = threadIdx.x; i < kDim; i += kThreads) sh_nan_from[i] = INT_MAX;
+      if (threadIdx.x == 0) sh_any_nan = 0;
+      __syncthreads();
+    }
   }
 }
 
 // Joins the parts of segments that several CTAs shared, in the order of the tokens.  CTA (b, y) looks at the boundary
-// between the ranges of CTAs b and b + 1: if it is the first one within a segment, it joins rows y, y + gridDim.y, ...
-// of it.  A row of a part is kDim / 4 threads' float4; kThreads / (kDim / 4) parts are read at a time.
+// between the ranges of CTAs b and b + 1: if it is the first one within a segment, it joins rows of it, a team of threads
+// for each.  kDim / 4 threads hold a row of a part as float4; a team of more reads several parts at once.
+constexpr int kJoinThreads = 256;
 template <int kDim, int kRows, int kUnits, bool kBf16>
-__global__ void __launch_bounds__(kThreads) kv8_attention_join(AttnParams p) {
-  constexpr int kSpan = kDim / 4, kAtOnce = kThreads / kSpan;
+__global__ void __launch_bounds__(kJoinThreads) kv8_attention_join(AttnParams p, int team) {
+  constexpr int kSpan = kDim / 4, kDeep = 4;
   using SeqT = Seq<kRows, kUnits>;
   extern __shared__ __align__(16) char smem[];
   uint32_t *prefix = reinterpret_cast<uint32_t *>(smem);
-  __shared__ float4 sh_a[kThreads];
-  __shared__ float sh_l[kAtOnce];
+  __shared__ float4 sh_a[kJoinThreads];
+  __shared__ float sh_l[kJoinThreads], sh_top[kJoinThreads / 32];
   const int n_seqs = p.batch.n_seqs;
+  scan_units(p, prefix, [&](int s) { return SeqT(p, s).all_units(p); });
+  after_previous();
   if (p.clear_tail) {
     int lo, hi = 0;
     if (n_seqs) p.batch.rows(n_seqs - 1, lo, hi);
-    const int64_t id = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * kThreads + threadIdx.x;
+    const int64_t id = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * kJoinThreads + threadIdx.x;
     for (int64_t e = (int64_t)hi * p.q_heads * kDim + id; e < (int64_t)p.batch.n_rows * p.q_heads * kDim;
-         e += (int64_t)gridDim.x * gridDim.y * kThreads) {
+         e += (int64_t)gridDim.x * gridDim.y * kJoinThreads) {
       const int64_t row = e / (p.q_heads * kDim);
       const int qh = (int)(e / kDim % p.q_heads), d = (int)(e % kDim);
       p.out[row * p.out_row + qh * p.out_head + d] = 0;
       if (d == 0 && p.lse) p.lse[row * p.q_heads + qh] = -INFINITY;
     }
   }
-  scan_units(p, prefix, [&](int s) { return SeqT(p, s).all_units(p); });
   const Split split(prefix[n_seqs], p.n_ctas);
   const int c0 = blockIdx.x;
   if (c0 + 1 >= split.n_ctas) return;
@@ -455,31 +465,60 @@ __global__ void __launch_bounds__(kThreads) kv8_attention_join(AttnParams p) {
   const SeqT seq(p, s);
   const Segment seg(p, seq, s, prefix[s], u);
   if (seg.begin == u || split.owner(seg.begin) != c0) return;
-  const int c1 = split.owner(seg.begin + seg.units - 1), slot0 = 2 * c0 + (split.begin(c0) < seg.begin ? 1 : 0);
-  const int part = threadIdx.x / kSpan, d = threadIdx.x % kSpan * 4;
+  const int parts = split.owner(seg.begin + seg.units - 1) - c0 + 1, slot0 = 2 * c0 + (split.begin(c0) < seg.begin ? 1 : 0);
+  const int teams = kJoinThreads / team, lane = threadIdx.x % team, part0 = lane / kSpan, at_once = team / kSpan, d = lane % kSpan * 4;
   const int live_rows = min(seq.all_rows(p) - seg.rt * kRows, kRows);
-  for (int n = blockIdx.y; n < live_rows; n += gridDim.y) {
+  auto slot_of = [&](int k) { return k == 0 ? slot0 : 2 * (c0 + k); };
+  for (int n0 = blockIdx.y * teams; n0 < live_rows; n0 += gridDim.y * teams) {
+    const int n = min(n0 + (int)threadIdx.x / team, live_rows - 1);      // surplus teams repeat the last row
     float top = kNone;
-    for (int c = c0; c <= c1; ++c) top = fmaxf(top, p.part_ml[(c == c0 ? slot0 : 2 * c) * kRows + n].x);
+    if (at_once == 1) {
+      for (int k = 0; k < parts; ++k) top = fmaxf(top, p.part_ml[slot_of(k) * kRows + n].x);
+    } else {                // a team of several warps: the only one, or one of few
+      for (int k = lane; k < parts; k += team) top = fmaxf(top, p.part_ml[slot_of(k) * kRows + n].x);
+#pragma unroll
+      for (int k = 1; k < 32; k <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k, min(team, 32)));
+      if (team > 32) {
+        if ((threadIdx.x & 31) == 0) sh_top[threadIdx.x >> 5] = top;
+        __syncthreads();
+        const int warp0 = (int)threadIdx.x / team * (team / 32);
+        for (int k = 0; k < team / 32; ++k) top = fmaxf(top, sh_top[warp0 + k]);
+      }
+    }
     float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
     float l = 0.f;
-    for (int c = c0 + part; c <= c1; c += kAtOnce) {
-      const int slot = c == c0 ? slot0 : 2 * c;
-      const float2 ml = p.part_ml[slot * kRows + n];
-      const float r = exp2_fast(ml.x - top);
-      const float4 x = *reinterpret_cast<const float4 *>(p.part_o + ((int64_t)slot * kRows + n) * kDim + d);
-      l += ml.y * r;
-      a.x += x.x * r, a.y += x.y * r, a.z += x.z * r, a.w += x.w * r;
-    }
-    sh_a[threadIdx.x] = a;
-    if (d == 0) sh_l[part] = l;
-    __syncthreads();
-    if (part == 0) {
-      for (int k = 1; k < kAtOnce; ++k) {
-        const float4 x = sh_a[k * kSpan + threadIdx.x];
-        a.x += x.x, a.y += x.y, a.z += x.z, a.w += x.w;
-        l += sh_l[k];
+    for (int k0 = part0; k0 < parts; k0 += kDeep * at_once) {
+      float2 ml[kDeep];
+      float4 x[kDeep];
+#pragma unroll
+      for (int i = 0; i < kDeep; ++i) {
+        const int k = k0 + i * at_once;
+        ml[i] = make_float2(kNone, 0.f);
+        x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (k < parts) {
+          ml[i] = p.part_ml[slot_of(k) * kRows + n];
+          x[i] = *reinterpret_cast<const float4 *>(p.part_o + ((int64_t)slot_of(k) * kRows + n) * kDim + d);
+        }
       }
+#pragma unroll
+      for (int i = 0; i < kDeep; ++i) {
+        const float r = exp2_fast(ml[i].x - top);
+        l += ml[i].y * r;
+        a.x += x[i].x * r, a.y += x[i].y * r, a.z += x[i].z * r, a.w += x[i].w * r;
+      }
+    }
+    if (at_once > 1) {
+      sh_a[threadIdx.x] = a;
+      sh_l[threadIdx.x] = l;
+      __syncthreads();
+      if (part0 == 0)
+        for (int k = 1; k < at_once; ++k) {
+          const float4 x = sh_a[threadIdx.x + k * kSpan];
+          a.x += x.x, a.y += x.y, a.z += x.z, a.w += x.w;
+          l += sh_l[threadIdx.x + k * kSpan];
+        }
+    }
+    if (part0 == 0 && n0 + (int)threadIdx.x / team < live_rows) {
       const int row = seg.rt * kRows + n, i = row / p.group, qh = seg.head * p.group + row % p.group;
       const float inv = l == 0.f ? 0.f : 1.f / l;
       uint16_t *dst = p.out + (int64_t)(seq.row0 + i) * p.out_row + qh * p.out_head + d;
@@ -488,7 +527,7 @@ __global__ void __launch_bounds__(kThreads) kv8_attention_join(AttnParams p) {
       else dst[0] = (uint16_t)x, dst[1] = x >> 16, dst[2] = (uint16_t)y, dst[3] = y >> 16;
       if (d == 0 && p.lse) p.lse[(int64_t)(seq.row0 + i) * p.q_heads + qh] = lse_of(top, l);
     }
-    __syncthreads();
+    if (at_once > 1) __syncthreads();
   }
 }
 
@@ -505,6 +544,7 @@ __global__ void __launch_bounds__(kThreads) kv8_attention_weights(AttnParams p) 
     return seq.rows ? (uint32_t)((tokens + kUnit - 1) / kUnit) : 0u;
   };
   scan_units(p, prefix, [&](int s) { return units_of(SeqT(p, s)) * (uint32_t)p.cache.heads; });
+  after_previous();
   const int n_seqs = p.batch.n_seqs, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   if (blockIdx.x == 0)
     for (int s = threadIdx.x; s < n_seqs; s += kThreads)
@@ -633,23 +673,26 @@ void check_args(const pf_kv8_attention_args *a, const Kv8View &c, const Kv8Batch
 }
 
 template <int kDim, int kRows, int kUnits, bool kBf16>
-void launch_join(const AttnParams &p, int ctas_of_a_boundary, cudaStream_t stream) {
-  const dim3 grid((unsigned)p.n_ctas, (unsigned)ctas_of_a_boundary);
-  kv8_attention_join<kDim, kRows, kUnits, kBf16><<<grid, kThreads, ((size_t)p.batch.n_seqs + 1) * 4, stream>>>(p);
-  PF_KV8_LAUNCHED();
+void launch_join(const AttnParams &p, cudaStream_t stream) {
+  // About n_ctas / segments parts meet in a segment: few are read one after the other by the fewest threads that hold a row,
+  // many (a long sequence alone) by a whole CTA.  One rule for all: a quarter of them at a time.
+  constexpr int kSpan = kDim / 4;
+  const int segments = std::max(1, p.batch.n_seqs * p.cache.heads);
+  int team = kSpan;
+  while (team < kJoinThreads && team / kSpan * 4 * segments < p.n_ctas) team *= 2;
+  const int passes = std::max(1, kRows * team / kJoinThreads);
+  const dim3 grid((unsigned)p.n_ctas, (unsigned)std::min(passes, 16));
+  launch_after(kv8_attention_join<kDim, kRows, kUnits, kBf16>, grid, kJoinThreads, ((size_t)p.batch.n_seqs + 1) * 4, stream, p, team);
 }
 
 template <int kDim, int kNt, bool kBf16>
 void launch_rows(const AttnParams &p, cudaStream_t stream) {
   const size_t smem = kWarps * 8 * kNt * (kDim * 4 + 8) + ((size_t)p.batch.n_seqs + 1) * 4;
   auto kernel = kv8_attention_rows<kDim, kNt, kBf16>;
-  if (smem > 48 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+  if (smem > 47 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
     throw Error::storage("cudaFuncSetAttribute failed");
-  if (p.batch.n_seqs) {
-    kernel<<<p.n_ctas, kThreads, smem, stream>>>(p);
-    PF_KV8_LAUNCHED();
-  }
-  launch_join<kDim, 8 * kNt, kUnit, kBf16>(p, 8 * kNt, stream);
+  if (p.batch.n_seqs) launch_after(kernel, p.n_ctas, kThreads, smem, stream, p);
+  launch_join<kDim, 8 * kNt, kUnit, kBf16>(p, stream);
 }
 
 template <int kDim, bool kBf16>
@@ -657,15 +700,14 @@ void launch_all(const AttnParams &p, int nt, int n_sms, cudaStream_t stream) {
   if (nt == 0) {
     if (p.batch.n_seqs) kv8_wide_launch(p, kBf16, stream);
     constexpr int kRows = kDim == 256 ? 128 : 256, kTokens = kDim == 256 ? 64 : 128;
-    launch_join<kDim, kRows, kTokens, kBf16>(p, 32, stream);
+    launch_join<kDim, kRows, kTokens, kBf16>(p, stream);
   } else if (nt == 1) {
     launch_rows<kDim, 1, kBf16>(p, stream);
   } else if constexpr (kDim != 256) {
     launch_rows<kDim, 2, kBf16>(p, stream);
   }
   if (p.weights && p.batch.n_seqs) {
-    kv8_attention_weights<kDim, kBf16><<<n_sms * 4, kThreads, ((size_t)p.batch.n_seqs + 1) * 4, stream>>>(p);
-    PF_KV8_LAUNCHED();
+    launch_after(kv8_attention_weights<kDim, kBf16>, n_sms * 4, kThreads, ((size_t)p.batch.n_seqs + 1) * 4, stream, p);
   }
 }
 

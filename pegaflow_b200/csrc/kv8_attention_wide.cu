@@ -174,6 +174,7 @@ __global__ void __launch_bounds__(threads_of(kDim), 1) kv8_attention_wide(AttnPa
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(shared_of(&sh.tmem)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
+  after_previous();
   scan_units(p, prefix, [&](int s) { return SeqT(p, s).all_units(p); });
   fence_before();
   __syncthreads();
@@ -558,8 +559,7 @@ void launch(const AttnParams &p, cudaStream_t stream) {
   const size_t smem = kv8_wide_plan(kDim).smem + ((size_t)p.batch.n_seqs + 1) * 4;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
     throw Error::storage("cudaFuncSetAttribute failed");
-  kernel<<<p.n_ctas, threads_of(kDim), smem, stream>>>(p);
-  PF_KV8_LAUNCHED();
+  launch_after(kernel, p.n_ctas, threads_of(kDim), smem, stream, p);
 }
 
 }  // namespace

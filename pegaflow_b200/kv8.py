@@ -21,7 +21,10 @@ import torch
 from . import _native as N
 
 _DTYPES = {torch.bfloat16: N.KV8_BF16, torch.float16: N.KV8_F16}
+_INT32, _FLOAT32 = torch.int32, torch.float32
 _byref = C.byref
+_append, _attention, _attention_workspace, _evict = (N.lib.pf_kv8_append, N.lib.pf_kv8_attention,
+                                                     N.lib.pf_kv8_attention_workspace, N.lib.pf_kv8_evict)
 
 
 def _refuse(text: str):
@@ -72,20 +75,12 @@ class Kv8Cache:
         self._desc_ref = _byref(self._desc)
         self._status = torch.zeros(1, dtype=torch.int32, device=t.device)
         self._status_ptr = self._status.data_ptr()
-
-    # ------------------------------------------------------------------ what the tensor holds
-    @property
-    def values(self):
-        """View of the e4m3 values: [2, num_blocks, kv_heads, block_size, head_dim]."""
-        n = self.kv_heads * self.block_size * self.head_dim
-        return self.tensor[:, :, :n].view(torch.float8_e4m3fn).view(2, self.num_blocks, self.kv_heads, self.block_size,
-                                                                    self.head_dim)
-
-    @property
-    def scales(self):
-        """View of the scales: [2, num_blocks, kv_heads], float32."""
-        n = self.kv_heads * self.block_size * self.head_dim
-        return self.tensor[:, :, n:n + 4 * self.kv_heads].view(torch.float32)
+        self._workspaces = {}      # sizes of a call -> workspace bytes
+        n = kv_heads * block_size * head_dim
+        #: View of the e4m3 values: [2, num_blocks, kv_heads, block_size, head_dim].
+        self.values = t[:, :, :n].view(torch.float8_e4m3fn).view(2, t.shape[1], kv_heads, block_size, head_dim)
+        #: View of the scales: [2, num_blocks, kv_heads], float32.
+        self.scales = t[:, :, n:n + 4 * kv_heads].view(torch.float32)
 
     def check(self):
         """Raise if a call since the last check met a block id, a length or row starts that it had to leave out.  Waits
@@ -102,43 +97,46 @@ class Kv8Cache:
 
     # ------------------------------------------------------------------ arguments
     def _ints(self, name, t, dim):
-        if t.dtype != torch.int32 or t.dim() != dim or t.device != self.device:
+        if t.dtype is not _INT32 or t.dim() != dim or t.device != self.device:
             _refuse(f"{name}: an int32 tensor of {dim} dimension(s) on {self.device} is needed, not {t.dtype} "
                     f"{tuple(t.shape)} on {t.device}")
-        if t.shape[-1] > 1 and t.stride(-1) != 1:
+        if t.stride(-1) != 1 and t.shape[-1] > 1:
             _refuse(f"{name}: the last dimension must be dense")
+        return t.data_ptr()
 
     def _batch(self, block_tables, lens, starts):
-        self._ints("block_tables", block_tables, 2)
-        self._ints("lens", lens, 1)
-        n = lens.shape[0]
-        if block_tables.shape[0] != n:
-            _refuse(f"block_tables has {block_tables.shape[0]} rows for {n} lengths")
+        tables_ptr = self._ints("block_tables", block_tables, 2)
+        lens_ptr = self._ints("lens", lens, 1)
+        n, width = block_tables.shape
+        if lens.shape[0] != n:
+            _refuse(f"block_tables has {n} rows for {lens.shape[0]} lengths")
         ptr = None
         if starts is not None:
-            self._ints("starts", starts, 1)
+            ptr = self._ints("starts", starts, 1)
             if starts.shape[0] != n + 1:
                 _refuse(f"starts has {starts.shape[0]} entries for {n} sequences: {n + 1} are needed")
-            ptr = starts.data_ptr()
-        return N.Kv8Batch(block_tables.data_ptr(), block_tables.stride(0), block_tables.shape[1], n, lens.data_ptr(), ptr,
-                          self._status_ptr)
+        return N.Kv8Batch(tables_ptr, block_tables.stride(0), width, n, lens_ptr, ptr, self._status_ptr)
 
     def _rows(self, name, t, heads=None):
-        if t.dtype not in _DTYPES or t.dim() != 3 or t.device != self.device:
+        """Checks a tensor of rows; returns its dtype's code and its strides."""
+        code = _DTYPES.get(t.dtype)
+        if code is None or t.dim() != 3 or t.device != self.device:
             _refuse(f"{name}: a bfloat16 or float16 tensor [rows, heads, {self.head_dim}] on {self.device} is needed, not "
                     f"{t.dtype} {tuple(t.shape)} on {t.device}")
-        if t.shape[2] != self.head_dim or (heads is not None and t.shape[1] != heads):
-            _refuse(f"{name}: shape {tuple(t.shape)} does not fit kv_heads={self.kv_heads}, head_dim={self.head_dim}")
-        if t.stride(2) != 1:
+        shape, strides = t.shape, t.stride()
+        if shape[2] != self.head_dim or (heads is not None and shape[1] != heads):
+            _refuse(f"{name}: shape {tuple(shape)} does not fit kv_heads={self.kv_heads}, head_dim={self.head_dim}")
+        if strides[2] != 1:
             _refuse(f"{name}: the last dimension must be dense")
         if t.requires_grad and torch.is_grad_enabled():
             _refuse(f"{name} requires a gradient: the 8-bit cache has no backward pass")
+        return code, strides
 
-    def _stream(self, stream):
-        """(handle, the context in which memory for that stream is allocated)."""
-        if stream is None:
-            return torch.cuda.current_stream(self.device).cuda_stream
-        return stream
+    def _per_token(self, name, t, n):
+        if t.dtype is not _FLOAT32 or t.dim() != 3 or t.device != self.device or t.shape[0] != n or \
+                t.shape[1] != self.kv_heads or (t.stride(2) != 1 and t.shape[2] > 1):
+            _refuse(f"{name}: a float32 tensor [{n}, {self.kv_heads}, tokens] on {self.device} with a dense last dimension is "
+                    f"needed, not {t.dtype} {tuple(t.shape)} on {t.device}")
 
     def _on(self, stream):
         return torch.cuda.stream(torch.cuda.ExternalStream(stream, device=self.device))
@@ -149,14 +147,15 @@ class Kv8Cache:
         share of the rows) become tokens lens[s], lens[s] + 1, ... of sequence s.  lens holds the lengths before the call
         and is not changed.  A block takes the scale that its largest magnitude needs; where a new row raises it,
         the block's old rows are rounded anew."""
-        self._rows("k", k, self.kv_heads)
-        self._rows("v", v, self.kv_heads)
-        if k.dtype != v.dtype or k.shape != v.shape:
+        code, ks = self._rows("k", k, self.kv_heads)
+        v_code, vs = self._rows("v", v, self.kv_heads)
+        if code != v_code or k.shape != v.shape:
             _refuse(f"k ({k.dtype} {tuple(k.shape)}) and v ({v.dtype} {tuple(v.shape)}) differ")
         batch = self._batch(block_tables, lens, starts)
-        ks, vs = k.stride(), v.stride()
-        N.check(N.lib.pf_kv8_append(self._index, self._desc_ref, _byref(batch), k.data_ptr(), v.data_ptr(), _DTYPES[k.dtype],
-                                    k.shape[0], ks[0], ks[1], vs[0], vs[1], self._stream(stream)))
+        if stream is None:
+            stream = torch.cuda.current_stream(self.device).cuda_stream
+        N.check(_append(self._index, self._desc_ref, _byref(batch), k.data_ptr(), v.data_ptr(), code, k.shape[0], ks[0], ks[1],
+                        vs[0], vs[1], stream))
 
     def attention(self, q, block_tables, lens, *, starts=None, max_query: Optional[int] = None,
                   scale: Optional[float] = None, causal: bool = True, weights=None, lse: bool = False, out=None,
@@ -169,7 +168,7 @@ class Kv8Cache:
         unless given.  weights, float32 [sequences, kv_heads, >= longest]: each token's probability, summed over the
         sequence's rows and the query heads of the KV head, is added in place.  Rows behind the last sequence are
         left as they were in a given ``out``, and 0 in one that the call allocates."""
-        self._rows("q", q)
+        code, qs = self._rows("q", q)
         n_rows, q_heads, dim = q.shape
         if q_heads == 0 or q_heads % self.kv_heads:
             _refuse(f"{q_heads} query heads are not a multiple of {self.kv_heads} KV heads")
@@ -180,46 +179,40 @@ class Kv8Cache:
             max_query = n_rows // max(1, batch.n_seqs)
         elif max_query < 0:
             _refuse(f"max_query={max_query}")
-        qs = q.stride()
-        a = N.Kv8AttentionArgs()
+        w_ptr, w_seq, w_head, capacity = None, 0, 0, 0
         if weights is not None:
-            if weights.dtype != torch.float32 or weights.dim() != 3 or weights.device != self.device or \
-                    weights.shape[0] != batch.n_seqs or weights.shape[1] != self.kv_heads or \
-                    (weights.shape[2] > 1 and weights.stride(2) != 1):
-                _refuse(f"weights: a float32 tensor [{batch.n_seqs}, {self.kv_heads}, tokens] on {self.device} with a dense "
-                        f"last dimension is needed, not {weights.dtype} {tuple(weights.shape)} on {weights.device}")
-            a.weights, a.weights_capacity = weights.data_ptr(), weights.shape[2]
-            a.weights_seq_stride, a.weights_head_stride = weights.stride(0), weights.stride(1)
-        given = out is not None
-        if given:
+            self._per_token("weights", weights, batch.n_seqs)
+            w_ptr, (w_seq, w_head, _), capacity = weights.data_ptr(), weights.stride(), weights.shape[2]
+        clear = 0
+        if out is not None:
             self._rows("out", out)
             if out.shape != q.shape or out.dtype != q.dtype:
                 _refuse(f"out ({out.dtype} {tuple(out.shape)}) and q ({q.dtype} {tuple(q.shape)}) differ")
-        a.q, a.n_rows, a.max_query, a.q_row_stride, a.q_head_stride = q.data_ptr(), n_rows, max_query, qs[0], qs[1]
-        a.q_heads, a.dtype, a.causal = q_heads, _DTYPES[q.dtype], int(causal)
-        a.scale = dim ** -0.5 if scale is None else scale
-        a.clear_tail = int(not given and starts is not None)
-        handle = self._stream(stream)
-        if stream is None:
-            return self._attend(a, batch, q, out, lse, handle)
-        with self._on(stream):     # what the call allocates belongs to the stream that uses it
-            return self._attend(a, batch, q, out, lse, handle)
-
-    def _attend(self, a, batch, q, out, want_lse, handle):
-        need = N.sz()
+        elif starts is not None:
+            clear = 1
+        if stream is not None:
+            with self._on(stream):     # what the call allocates belongs to the stream that uses it
+                return self.attention(q, block_tables, lens, starts=starts, max_query=max_query, scale=scale, causal=causal,
+                                      weights=weights, lse=lse, out=out)
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        lse = None
-        if want_lse:
-            lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
-            a.lse = lse.data_ptr()
-        a.out = out.data_ptr()
-        a.out_row_stride, a.out_head_stride = out.stride(0), out.stride(1)
-        N.check(N.lib.pf_kv8_attention_workspace(self._index, self._desc_ref, _byref(batch), _byref(a), _byref(need)))
-        space = torch.empty(need.value, dtype=torch.uint8, device=q.device)
-        N.check(N.lib.pf_kv8_attention(self._index, self._desc_ref, _byref(batch), _byref(a), space.data_ptr(), need.value,
-                                       handle))
-        return (out, lse) if want_lse else out
+            out = torch.empty(q.shape, dtype=q.dtype, device=self.device)
+        os = out.stride()
+        lse_out = torch.empty((n_rows, q_heads), dtype=_FLOAT32, device=self.device) if lse else None
+        args = N.Kv8AttentionArgs(q.data_ptr(), out.data_ptr(), lse_out.data_ptr() if lse else None, w_ptr, n_rows, max_query,
+                                  qs[0], qs[1], os[0], os[1], w_seq, w_head, capacity, q_heads, code, 1 if causal else 0, clear,
+                                  dim ** -0.5 if scale is None else scale)
+        sizes = (n_rows, q_heads, max_query, batch.n_seqs, batch.max_blocks, starts is None, lse, w_ptr is None)
+        need = self._workspaces.get(sizes)
+        if need is None:
+            size = N.sz()
+            N.check(_attention_workspace(self._index, self._desc_ref, _byref(batch), _byref(args), _byref(size)))
+            if len(self._workspaces) >= 1024:
+                self._workspaces.clear()
+            need = self._workspaces[sizes] = size.value
+        space = torch.empty(need, dtype=torch.uint8, device=self.device)
+        N.check(_attention(self._index, self._desc_ref, _byref(batch), _byref(args), space.data_ptr(), need,
+                           torch.cuda.current_stream(self.device).cuda_stream))
+        return (out, lse_out) if lse else out
 
     def evict(self, block_tables, lens, weights, dst_tables, keep: int, *, recent: int = 0,
               stream: Optional[int] = None) -> Tuple["torch.Tensor", "torch.Tensor", "torch.Tensor"]:
@@ -233,30 +226,23 @@ class Kv8Cache:
         Returns (lens, weights, kept): int32 [sequences]; float32 like weights, 0 behind the kept tokens, so that
         attention can go on adding; int32 [sequences, kv_heads, keep], the source token of each, -1 behind the last."""
         batch = self._batch(block_tables, lens, None)
-        self._ints("dst_tables", dst_tables, 2)
-        n = batch.n_seqs
+        dst_ptr = self._ints("dst_tables", dst_tables, 2)
+        n, heads = batch.n_seqs, self.kv_heads
         if not 0 < keep < 1 << 31 or not 0 <= recent <= keep:
             _refuse(f"keep={keep}, recent={recent}: keep must be positive and recent at most keep")
         if dst_tables.shape[0] != n or dst_tables.shape[1] * self.block_size < keep:
             _refuse(f"dst_tables {tuple(dst_tables.shape)} does not hold {keep} tokens of {n} sequences")
-        if weights.dtype != torch.float32 or weights.dim() != 3 or weights.device != self.device or \
-                weights.shape[0] != n or weights.shape[1] != self.kv_heads or (weights.shape[2] > 1 and weights.stride(2) != 1):
-            _refuse(f"weights: a float32 tensor [{n}, {self.kv_heads}, tokens] on {self.device} with a dense last dimension "
-                    f"is needed, not {weights.dtype} {tuple(weights.shape)} on {weights.device}")
-        handle = self._stream(stream)
-        if stream is None:
-            return self._evict(batch, weights, dst_tables, keep, recent, handle)
-        with self._on(stream):
-            return self._evict(batch, weights, dst_tables, keep, recent, handle)
-
-    def _evict(self, batch, weights, dst_tables, keep, recent, handle):
-        n, heads, capacity = weights.shape
-        capacity = max(capacity, keep)
-        new_lens = torch.empty(n, dtype=torch.int32, device=self.device)
-        new_weights = torch.empty((n, heads, capacity), dtype=torch.float32, device=self.device)
-        kept = torch.empty((n, heads, keep), dtype=torch.int32, device=self.device)
-        a = N.Kv8EvictArgs(weights.data_ptr(), weights.stride(0), weights.stride(1), weights.shape[2], dst_tables.data_ptr(),
-                           dst_tables.stride(0), keep, recent, new_lens.data_ptr(), new_weights.data_ptr(), capacity,
-                           kept.data_ptr())
-        N.check(N.lib.pf_kv8_evict(self._index, self._desc_ref, _byref(batch), _byref(a), handle))
+        self._per_token("weights", weights, n)
+        if stream is not None:
+            with self._on(stream):
+                return self.evict(block_tables, lens, weights, dst_tables, keep, recent=recent)
+        ws, tokens = weights.stride(), weights.shape[2]
+        capacity = max(tokens, keep)
+        new_lens = torch.empty(n, dtype=_INT32, device=self.device)
+        new_weights = torch.empty((n, heads, capacity), dtype=_FLOAT32, device=self.device)
+        kept = torch.empty((n, heads, keep), dtype=_INT32, device=self.device)
+        args = N.Kv8EvictArgs(weights.data_ptr(), ws[0], ws[1], tokens, dst_ptr, dst_tables.stride(0), keep, recent,
+                              new_lens.data_ptr(), new_weights.data_ptr(), capacity, kept.data_ptr())
+        N.check(_evict(self._index, self._desc_ref, _byref(batch), _byref(args),
+                       torch.cuda.current_stream(self.device).cuda_stream))
         return new_lens, new_weights, kept
