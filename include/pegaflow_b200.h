@@ -553,7 +553,7 @@ void pf_load_state_free(pf_load_state *state);                   /* unlinks when
  * ---------------------------------------------------------------------------------------- */
 typedef struct pf_kv8_cache {
   uint64_t data_ptr;         /* 16-byte aligned, like both strides */
-  size_t block_stride_bytes; /* at least pf_kv8_record_bytes */
+  size_t block_stride_bytes; /* at least pf_kv8_record_bytes, below 4 GiB */
   size_t kv_stride_bytes;    /* K record -> V record of the same block */
   size_t num_blocks;
   uint32_t block_size;       /* tokens: 16, 32, 64 or 128 */

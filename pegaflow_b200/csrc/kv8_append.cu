@@ -23,6 +23,8 @@ Kv8View kv8_check_cache(const pf_kv8_cache *c) {
     throw Error::invalid(strf("8-bit cache: num_blocks=%zu out of range", c->num_blocks));
   if (c->num_blocks > 1 && c->block_stride_bytes < record)
     throw Error::invalid(strf("8-bit cache: block stride of %zu bytes is below the record's %zu", c->block_stride_bytes, record));
+  if (c->num_blocks > 1 && c->block_stride_bytes > 0xffffffffu)
+    throw Error::invalid(strf("8-bit cache: block stride of %zu bytes exceeds 4 GiB", c->block_stride_bytes));
   if (c->kv_stride_bytes < record)
     throw Error::invalid(strf("8-bit cache: K/V stride of %zu bytes is below the record's %zu", c->kv_stride_bytes, record));
   Kv8View v{};
@@ -116,7 +118,7 @@ __device__ __forceinline__ uint32_t finite_top(const uint4 &v) {
 __host__ __device__ constexpr int append_warps(int warps) { return warps < 8 ? 8 : warps; }   // of a CTA
 
 template <bool kBf16, bool kVec, int kWarps>
-__global__ void __launch_bounds__(32 * append_warps(kWarps)) kv8_append_kernel(Kv8View cache, Kv8Batch batch, AppendSource src) {
+__global__ void __launch_bounds__(32 * append_warps(kWarps), kWarps > 8 ? 2 : 4) kv8_append_kernel(Kv8View cache, Kv8Batch batch, AppendSource src) {
   constexpr int kTiles = append_warps(kWarps) / kWarps;     // tiles of a CTA
   const int bl = cache.block_log2, bs = 1 << bl, dim_log2 = 31 - __clz(cache.dim);
   const int item = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -154,17 +156,21 @@ __global__ void __launch_bounds__(32 * append_warps(kWarps)) kv8_append_kernel(K
   const bool mine = head < cache.heads;                                  // the last CTA of an item may have warps to spare
   const int old_rows = (int)max((int64_t)0, len - tok0);                 // rows of the block that were there before
   const int end_row = mine ? (int)min((int64_t)bs, len + n - tok0) : 0;
-  const int64_t row_stride = src.row_stride[kv];
-  const uint16_t *x = src.ptr[kv] + head * src.head_stride[kv] + (row0 + (tok0 - len)) * row_stride;
+  const int64_t row_stride = kv ? src.row_stride[1] : src.row_stride[0];
+  // a warp's vector i lies 256 elements behind its vector i - 1: some whole rows
+  const int row_step = 256 >> dim_log2, first = (part * 8 * 32 + lane) * 8, row_0 = first >> dim_log2;
+  const uint16_t *x = (kv ? src.ptr[1] : src.ptr[0]) + head * (kv ? src.head_stride[1] : src.head_stride[0]) +
+                      (row0 + (tok0 - len) + row_0) * row_stride + (first & (cache.dim - 1));
+  const int64_t step = row_step * row_stride;
 
   uint4 v[8];
   uint32_t tops = 0;                                                     // of both halves of a pair
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const int e = ((part * 8 + i) * 32 + lane) * 8, row = e >> dim_log2, col = e & (cache.dim - 1);
+    const int row = row_0 + i * row_step;
     v[i] = make_uint4(0, 0, 0, 0);
     if (row >= old_rows && row < end_row) {
-      const uint16_t *p = x + row * row_stride + col;
+      const uint16_t *p = x + i * step;
       if (kVec) v[i] = __ldg(reinterpret_cast<const uint4 *>(p));
       else v[i] = make_uint4(p[0] | p[1] << 16, p[2] | p[3] << 16, p[4] | p[5] << 16, p[6] | p[7] << 16);
     }
@@ -197,8 +203,8 @@ __global__ void __launch_bounds__(32 * append_warps(kWarps)) kv8_append_kernel(K
   const float inv = exp2i(-e), old_factor = exp2i(e_old - e);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const int el = ((part * 8 + i) * 32 + lane) * 8, row = el >> dim_log2;
-    uint2 *out = reinterpret_cast<uint2 *>(tile + el);
+    const int row = row_0 + i * row_step;
+    uint2 *out = reinterpret_cast<uint2 *>(tile + first + 256 * i);
     if (row >= old_rows && row < end_row) {
       const float2 a = widen<kBf16>(v[i].x), c = widen<kBf16>(v[i].y), d = widen<kBf16>(v[i].z), f = widen<kBf16>(v[i].w);
       *out = make_uint2(e4m3x4(a.x * inv, a.y * inv, c.x * inv, c.y * inv), e4m3x4(d.x * inv, d.y * inv, f.x * inv, f.y * inv));

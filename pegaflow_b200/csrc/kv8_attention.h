@@ -20,6 +20,7 @@ struct AttnParams {
   int64_t q_row, q_head, out_row, out_head, w_seq, w_head;
   int w_capacity;
   int q_heads, group, max_query;
+  int row_tiles_most;   // of a sequence
   int causal, clear_tail, vec_q, vec_out;
   float scale;
   // Partial results: slot 2 c + k of CTA c (k = 0: the segment that its range starts in, 1: the one that it ends in).
@@ -39,8 +40,9 @@ struct Split {
   __device__ int owner(uint32_t u) const { return (int)((((uint64_t)u + 1) * n_ctas - 1) / total); }
 };
 
-// One sequence of a call: its rows (row = query * group + head of the group) in tiles of kRows, and its tokens.
-template <int kRows, int kUnit>
+// One sequence of a call: its rows (row = query * group + head of the group) in tiles of kRows, and its tokens.  kWhole:
+// one tile of all rows, that reaches over all tokens.
+template <int kRows, int kUnit, bool kWhole = false>
 struct Seq {
   int row0, rows, len, row_tiles;
   __device__ Seq(const AttnParams &p, int s) {
@@ -48,7 +50,7 @@ struct Seq {
     p.batch.rows(s, row0, hi);
     rows = min(hi - row0, p.max_query);
     len = p.batch.length(s, p.cache.block_log2);
-    row_tiles = (rows * p.group + kRows - 1) / kRows;
+    row_tiles = kWhole ? min(rows, 1) : (rows * p.group + kRows - 1) / kRows;
   }
   __device__ int all_rows(const AttnParams &p) const { return rows * p.group; }
   __device__ int visible(const AttnParams &p, int row) const {   // tokens that query row `row` sees
@@ -56,73 +58,89 @@ struct Seq {
   }
   // Units of one row tile: those that its last row sees, one at least.
   __device__ uint32_t units(const AttnParams &p, int rt) const {
-    return max(1, (visible(p, min((rt + 1) * kRows, all_rows(p)) - 1) + kUnit - 1) / kUnit);
-  }
-  __device__ uint32_t all_units(const AttnParams &p) const {
-    uint32_t n = 0;
-    for (int rt = 0; rt < row_tiles; ++rt) n += units(p, rt);
-    return n * (uint32_t)p.cache.heads;
+    return max(1, ((kWhole ? len : visible(p, min((rt + 1) * kRows, all_rows(p)) - 1)) + kUnit - 1) / kUnit);
   }
 };
 
-// Where unit u lies: row tile, head, the unit within the segment, and the segment's extent.
+// The units of all (sequence, row tile) entries in order, as sums before every chunk of entries (one, unless there are more
+// than kMost).  Every CTA of every kernel computes them for itself: lens stay on the device, and no launch and no
+// workspace is spent on it.
+template <int kRows, int kUnit, bool kWhole = false>
+struct Work {
+  using SeqT = Seq<kRows, kUnit, kWhole>;
+  static constexpr int kMost = 1024;
+  uint32_t *prefix;         // [chunks + 1] in shared memory
+  int entries, chunk, chunks;
+  static __host__ __device__ int chunk_of(int entries) { return max((entries + kMost - 1) / kMost, 1); }
+  static __host__ size_t bytes(int n_seqs, int row_tiles_most) {
+    const int entries = n_seqs * row_tiles_most, chunk = chunk_of(entries);
+    return ((size_t)(entries + chunk - 1) / chunk + 1) * 4;
+  }
+  __device__ uint32_t units_of(const AttnParams &p, int e) const {
+    const SeqT seq(p, e / p.row_tiles_most);
+    const int rt = e % p.row_tiles_most;
+    return rt < seq.row_tiles ? seq.units(p, rt) * (uint32_t)p.cache.heads : 0u;
+  }
+  __device__ Work(const AttnParams &p, uint32_t *prefix) : prefix(prefix) {
+    __shared__ uint32_t warp_sum[32];
+    entries = p.batch.n_seqs * p.row_tiles_most;
+    chunk = chunk_of(entries);
+    chunks = (entries + chunk - 1) / chunk;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n_warps = (blockDim.x + 31) >> 5;
+    uint32_t base = 0;
+    for (int c0 = 0; c0 < chunks; c0 += blockDim.x) {
+      const int c = c0 + threadIdx.x;
+      uint32_t mine = 0;
+      for (int e = c * chunk; c < chunks && e < min((c + 1) * chunk, entries); ++e) mine += units_of(p, e);
+      uint32_t x = mine;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const uint32_t y = __shfl_up_sync(0xffffffffu, x, d);
+        if (lane >= d) x += y;
+      }
+      if (lane == 31) warp_sum[warp] = x;
+      __syncthreads();
+      uint32_t before = base, all = 0;
+      for (int w = 0; w < n_warps; ++w) {
+        if (w < warp) before += warp_sum[w];
+        all += warp_sum[w];
+      }
+      if (c < chunks) prefix[c] = before + x - mine;
+      base += all;
+      __syncthreads();
+    }
+    if (threadIdx.x == 0) prefix[chunks] = base;
+    __syncthreads();
+  }
+  __device__ uint32_t total() const { return prefix[chunks]; }
+};
+
+// The segment in which unit u < total lies.
 struct Segment {
   int s, rt, head;
-  uint32_t begin, units;      // first unit of the segment in the whole, its units
-  template <int kRows, int kUnit>
-  __device__ Segment(const AttnParams &p, const Seq<kRows, kUnit> &seq, int s, uint32_t seq_begin, uint32_t u) : s(s) {
-    begin = seq_begin;
-    for (rt = 0;; ++rt) {
-      units = seq.units(p, rt);
-      const uint32_t all = units * (uint32_t)p.cache.heads;
-      if (u - begin < all || rt + 1 >= seq.row_tiles) break;
-      begin += all;
+  uint32_t begin, units;      // its first unit, how many it has
+  template <int kRows, int kUnit, bool kWhole>
+  __device__ Segment(const AttnParams &p, const Work<kRows, kUnit, kWhole> &work, uint32_t u) {
+    int lo = 0, hi = work.chunks;      // last chunk that begins at or before u
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (work.prefix[mid] <= u) lo = mid;
+      else hi = mid;
     }
+    int e = lo * work.chunk;
+    begin = work.prefix[lo];
+    uint32_t all = work.units_of(p, e);
+    while (u - begin >= all) {
+      begin += all;
+      all = work.units_of(p, ++e);
+    }
+    s = e / p.row_tiles_most;
+    rt = e % p.row_tiles_most;
+    units = all / (uint32_t)p.cache.heads;
     head = (int)((u - begin) / units);
     begin += head * units;
   }
 };
-
-// prefix[s] = units before sequence s, prefix[n_seqs] = all of them.  Every CTA of every kernel computes it for
-// itself: lens stay on the device, and no launch and no workspace is spent on it.
-template <class Units>
-__device__ void scan_units(const AttnParams &p, uint32_t *prefix, Units &&units_of) {
-  __shared__ uint32_t warp_sum[32];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n_warps = blockDim.x >> 5;
-  uint32_t base = 0;
-  for (int s0 = 0; s0 < p.batch.n_seqs; s0 += blockDim.x) {
-    const int s = s0 + threadIdx.x;
-    const uint32_t mine = s < p.batch.n_seqs ? units_of(s) : 0u;
-    uint32_t x = mine;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const uint32_t y = __shfl_up_sync(0xffffffffu, x, d);
-      if (lane >= d) x += y;
-    }
-    if (lane == 31) warp_sum[warp] = x;
-    __syncthreads();
-    uint32_t before = base, all = 0;
-    for (int w = 0; w < n_warps; ++w) {
-      if (w < warp) before += warp_sum[w];
-      all += warp_sum[w];
-    }
-    if (s < p.batch.n_seqs) prefix[s] = before + x - mine;
-    base += all;
-    __syncthreads();
-  }
-  if (threadIdx.x == 0) prefix[p.batch.n_seqs] = base;
-  __syncthreads();
-}
-
-__device__ __forceinline__ int find_seq(const uint32_t *prefix, int n, uint32_t u) {   // last s with prefix[s] <= u
-  int lo = 0, hi = n;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (prefix[mid] <= u) lo = mid;
-    else hi = mid;
-  }
-  return lo;
-}
 
 __device__ __forceinline__ uint32_t f16x2(float lo, float hi) {
   uint32_t d;
@@ -155,6 +173,11 @@ __device__ __forceinline__ void check_batch(const AttnParams &p) {
 
 __device__ __forceinline__ float lse_of(float base, float sum) { return sum == 0.f ? -INFINITY : (base + log2f(sum)) * kLn2; }
 
+// Few query rows (kv8_attention_few.cu): tiles of 4, 8, 16 or 32 rows, 0 when there are more.  And the accumulated weights.
+int kv8_few_rows(int64_t rows);
+int kv8_few_ctas(int dim, int rows);      // CTAs of an SM
+void kv8_few_launch(const AttnParams &p, int rows, bool bf16, cudaStream_t stream);
+void kv8_weights_launch(const AttnParams &p, bool bf16, int n_sms, cudaStream_t stream);
 // Query rows by the hundred (kv8_attention_wide.cu).
 struct WidePlan {
   int rows, threads;

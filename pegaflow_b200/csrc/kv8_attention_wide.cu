@@ -20,6 +20,7 @@
 #include <cuda_bf16.h>
 
 #include "kv8_attention.h"
+#include "kv8_tensor.h"
 
 namespace pf {
 namespace {
@@ -50,94 +51,6 @@ struct Shared {
   int nan_from[256];         // first token whose V is NaN in a dimension
 };
 constexpr int kHidden = 1 << 20;
-
-__device__ __forceinline__ uint32_t shared_of(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ void bar_init(uint64_t *bar, int count) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(shared_of(bar)), "r"(count) : "memory");
-}
-__device__ __forceinline__ void bar_arrive(uint64_t *bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(shared_of(bar)) : "memory");
-}
-// Waits for the phase of `parity`; false after about two seconds, or as soon as another thread has given up.
-__device__ __forceinline__ bool bar_wait(uint64_t *bar, uint32_t parity, int *stalled) {
-  uint64_t start = 0;
-  for (uint32_t i = 1;; ++i) {
-    uint32_t done;
-    asm volatile("{.reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p;}"
-                 : "=r"(done)
-                 : "r"(shared_of(bar)), "r"(parity)
-                 : "memory");
-    if (done) return true;
-    if ((i & 255) == 0) {
-      uint64_t now;
-      asm volatile("mov.u64 %0, %globaltimer;" : "=l"(now));
-      if (start == 0) start = now;
-      if (*(volatile int *)stalled || now - start > 2000000000ull) {
-        *(volatile int *)stalled = 1;
-        return false;
-      }
-    }
-  }
-}
-// The same for a warp whose next instructions need all of its lanes.
-__device__ __forceinline__ bool bar_wait_warp(uint64_t *bar, uint32_t parity, int *stalled) {
-  return __all_sync(0xffffffffu, bar_wait(bar, parity, stalled));
-}
-
-__device__ __forceinline__ void fence_to_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void wait_stores() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void commit(uint64_t *bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(shared_of(bar)) : "memory");
-}
-// 128-byte swizzled operand: `lead` = bytes between 64-element panels along the rows of a matrix whose contracted index runs
-// down them (unused otherwise), 1024 bytes between groups of eight rows.
-__device__ __forceinline__ uint64_t operand(uint32_t addr, uint32_t lead) {
-  return (uint64_t)((addr >> 4) & 0x3fff) | (uint64_t)((lead >> 4) & 0x3fff) << 16 | (uint64_t)(1024 >> 4) << 32 |
-         (uint64_t)1 << 46 | (uint64_t)2 << 61;
-}
-// f16 operands, fp32 sums, 128 rows, n columns; B contracted along its rows or down them.
-__host__ __device__ constexpr uint32_t shape(int n, bool b_down) {
-  return 1u << 4 | (b_down ? 1u << 16 : 0u) | (uint32_t)(n / 8) << 17 | (uint32_t)(kGroupRows / 16) << 24;
-}
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t shape_, bool add) {
-  asm volatile(
-      "{.reg .pred p; setp.ne.u32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;}" ::"r"(d), "l"(a),
-      "l"(b), "r"(shape_), "r"((uint32_t)add)
-      : "memory");
-}
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t shape_, bool add) {
-  asm volatile(
-      "{.reg .pred p; setp.ne.u32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;}" ::"r"(d), "r"(a),
-      "l"(b), "r"(shape_), "r"((uint32_t)add)
-      : "memory");
-}
-#define PF_R4(r, i) "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3])
-#define PF_R16(r, i) PF_R4(r, i), PF_R4(r, i + 4), PF_R4(r, i + 8), PF_R4(r, i + 12)
-#define PF_I4(r, i) "r"(r[i]), "r"(r[i + 1]), "r"(r[i + 2]), "r"(r[i + 3])
-#define PF_I16(r, i) PF_I4(r, i), PF_I4(r, i + 4), PF_I4(r, i + 8), PF_I4(r, i + 12)
-__device__ __forceinline__ void load32(uint32_t (&r)[32], uint32_t at) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,"
-      "%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\ttcgen05.wait::ld.sync.aligned;"
-      : PF_R16(r, 0), PF_R16(r, 16)
-      : "r"(at)
-      : "memory");
-}
-__device__ __forceinline__ void store32(uint32_t at, const uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,"
-      "%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(at),
-      PF_I16(r, 0), PF_I16(r, 16)
-      : "memory");
-}
-__device__ __forceinline__ void store16(uint32_t at, const uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(at),
-      PF_I16(r, 0)
-      : "memory");
-}
 
 template <int kDim, bool kBf16>
 __global__ void __launch_bounds__(threads_of(kDim), 1) kv8_attention_wide(AttnParams p) {
@@ -175,13 +88,12 @@ __global__ void __launch_bounds__(threads_of(kDim), 1) kv8_attention_wide(AttnPa
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
   after_previous();
-  scan_units(p, prefix, [&](int s) { return SeqT(p, s).all_units(p); });
+  const Work<kRows, kTokens> work(p, prefix);
   fence_before();
   __syncthreads();
   fence_after();
   const uint32_t tmem = sh.tmem;
-  const int n_seqs = p.batch.n_seqs;
-  const Split split(prefix[n_seqs], p.n_ctas);
+  const Split split(work.total(), p.n_ctas);
   if (blockIdx.x == 0) check_batch(p);
   uint32_t u = 0, u_end = 0;
   if ((int)blockIdx.x < split.n_ctas) u = split.begin(blockIdx.x), u_end = split.begin(blockIdx.x + 1);
@@ -190,9 +102,9 @@ __global__ void __launch_bounds__(threads_of(kDim), 1) kv8_attention_wide(AttnPa
   uint32_t n_segment = 0;
   bool ok = true;
   while (u < u_end && ok) {
-    const int s = find_seq(prefix, n_seqs, u);
+    const Segment seg(p, work, u);
+    const int s = seg.s;
     const SeqT seq(p, s);
-    const Segment seg(p, seq, s, prefix[s], u);
     const uint32_t unit0 = u - seg.begin, units = min(seg.units - unit0, u_end - u);
     const int row_first = seg.rt * kRows, live_rows = min(seq.all_rows(p) - row_first, kRows);
     const int head = seg.head;
@@ -491,19 +403,19 @@ __global__ void __launch_bounds__(threads_of(kDim), 1) kv8_attention_wide(AttnPa
       }
     } else if (lane == 0) {
       // ------------------------------------------------------------------ issuer
-      constexpr uint32_t kScores = shape(kTokens, false), kOutput = shape(kDim, true);
+      constexpr uint32_t kScores = shape_f16(kTokens, false), kOutput = shape_f16(kDim, true);
       auto scores = [&](int g, uint32_t stage) {
         const uint32_t a = shared_of(smem + L::q + g * L::q_bytes), b = shared_of(smem + L::k + stage * L::kv_bytes);
 #pragma unroll
         for (int k = 0; k < kDim / 16; ++k)
-          mma_ss(tmem + g * kTokens, operand(a + k / 4 * (kGroupRows * 128) + k % 4 * 32, 16),
-                 operand(b + k / 4 * (kTokens * 128) + k % 4 * 32, 16), kScores, k != 0);
+          mma_f16_ss(tmem + g * kTokens, operand(a + k / 4 * (kGroupRows * 128) + k % 4 * 32, 16, 1024, kSwizzle128),
+                 operand(b + k / 4 * (kTokens * 128) + k % 4 * 32, 16, 1024, kSwizzle128), kScores, k != 0);
       };
       auto output = [&](int g, uint32_t stage, bool add) {
         const uint32_t b = shared_of(smem + L::v + stage * L::kv_bytes);
 #pragma unroll
         for (int k = 0; k < kTokens / 16; ++k)
-          mma_ts(tmem + kO + g * kDim, tmem + g * kTokens + 8 * k, operand(b + k * 2048, kTokens * 128), kOutput, add || k != 0);
+          mma_f16_ts(tmem + kO + g * kDim, tmem + g * kTokens + 8 * k, operand(b + k * 2048, kTokens * 128, 1024, kSwizzle128), kOutput, add || k != 0);
       };
       const int n_groups = live_rows > kGroupRows ? 2 : 1;
       ok = bar_wait(&sh.q_full, n_segment & 1, &sh.stalled);
@@ -556,7 +468,7 @@ __global__ void __launch_bounds__(threads_of(kDim), 1) kv8_attention_wide(AttnPa
 template <int kDim, bool kBf16>
 void launch(const AttnParams &p, cudaStream_t stream) {
   auto kernel = kv8_attention_wide<kDim, kBf16>;
-  const size_t smem = kv8_wide_plan(kDim).smem + ((size_t)p.batch.n_seqs + 1) * 4;
+  const size_t smem = kv8_wide_plan(kDim).smem + Work<kGroupRows * groups_of(kDim), tokens_of(kDim)>::bytes(p.batch.n_seqs, p.row_tiles_most);
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
     throw Error::storage("cudaFuncSetAttribute failed");
   launch_after(kernel, p.n_ctas, threads_of(kDim), smem, stream, p);
@@ -564,7 +476,7 @@ void launch(const AttnParams &p, cudaStream_t stream) {
 
 }  // namespace
 
-static_assert(1024 + Layout<128>::end + sizeof(Shared) + 4 * (PF_KV8_MAX_SEQS + 1) + 128 <= 227 * 1024, "shared memory");
+static_assert(1024 + Layout<128>::end + sizeof(Shared) + 4 * (1024 + 1) + 128 <= 227 * 1024, "shared memory");
 static_assert(Layout<256>::end <= Layout<128>::end && Layout<64>::end <= Layout<128>::end, "shared memory");
 
 WidePlan kv8_wide_plan(int dim) {

@@ -4,11 +4,12 @@ Tolerances of attention, from the kernel's arithmetic (u32 = 2^-24, halves of a 
   scores   products of exact f16 operands, dim of them added in fp32 (each addition at most 2^-23 of the sum of
            magnitudes, truncation included), scaled and turned to base 2 (three roundings):
            ds = (dim + 8) * 2^-23 * spread, spread = scale * max_j sum |q k|
-  p        exp2 of it: ds + 2^-21 relative; f16 for the product with V: 2^-11 more; each p below 2^-24 of f16's
-           range by half its smallest step, 2^-25, in units of 2^-9 (few rows) or of 2^-6 and the largest scale so far
-           (more than 16 rows): less than n * 2^-33 or n * 2^-31 of the largest |v|
+  p        exp2 of it: ds + 2^-21 relative; f16 for the product with V: 2^-11 more; and what is too small for that
+           form by half its smallest step, 2^-22 in units of 2^-6 (up to 32 rows: four e4m3 pieces) or 2^-25 in units
+           of 2^-6 (more), times V in units of the largest scale so far, at most 448 where the largest |v| is 224 or more:
+           n * 2^-27 or n * 2^-30 of the largest |v|
   sums     fp32 over at most n terms: n * 2^-24
-  out      sum p |v| * (2 (ds + 2^-21) + 2^-11 + 2 n 2^-24) + half a step of its type
+  out      sum p |v| * (2 (ds + 2^-21) + 2^-11 + 2 n 2^-24) + that + half a step of its type
 """
 import math
 
@@ -185,7 +186,7 @@ def check_attention(pf, cache, q, tables, lens, counts, *, causal=True, scale=No
     ds = (dim + 8) * 2.0 ** -23 * spread
     rel = 2 * (ds + 2.0 ** -21) + 2.0 ** -11 + 2 * longest * 2.0 ** -24
     big = (rc.values.abs().nan_to_num() * rc.scales[..., None, None]).max() if longest else 0.0
-    tol = size * rel[..., None] + HALF[q.dtype] * want.abs() + big * longest * (2.0 ** -33 if max(counts) * q.shape[1] / heads <= 16 else 2.0 ** -31) + 1e-30
+    tol = size * rel[..., None] + HALF[q.dtype] * want.abs() + big * longest * (2.0 ** -27 if max(counts) * q.shape[1] / heads <= 32 else 2.0 ** -30) + 1e-30
     nan = torch.isnan(want)
     assert torch.equal(torch.isnan(got_), nan)
     off = ((got_ - want).abs() - tol)[~nan]
