@@ -29,7 +29,7 @@ Kv8View kv8_check_cache(const pf_kv8_cache *c) {
     throw Error::invalid(strf("8-bit cache: K/V stride of %zu bytes is below the record's %zu", c->kv_stride_bytes, record));
   Kv8View v{};
   v.base = reinterpret_cast<char *>(c->data_ptr);
-  v.block_stride = c->block_stride_bytes;
+  v.block_stride = std::max(c->block_stride_bytes, record);    // of one block it may be anything
   v.kv_stride = c->kv_stride_bytes;
   v.num_blocks = (uint32_t)c->num_blocks;
   v.block_log2 = __builtin_ctz(c->block_size);

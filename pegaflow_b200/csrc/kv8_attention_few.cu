@@ -5,9 +5,10 @@
 //
 // The cache is read once and each byte is used for as many products as there are rows, so HBM bounds it, if the arithmetic
 // keeps out of the way.  It does when no thread touches K and V at all: 128 tokens at a time go from global into shared memory
-// by asynchronous copies, and the tcgen05 tensor cores take the products on the e4m3 bytes as they are, transposed:
+// by TMA, and the tcgen05 tensor cores take the products on the e4m3 bytes as they are, transposed:
 //   S^T [128 tokens, columns] = K Q^T           O^T [head dimensions, columns] += V^T P^T
-// A thread holds a token's scores (a lane of tensor memory), and at the end a dimension's outputs.  What is not e4m3, q and
+// One warp feeds tiles, across the segments' ends, a thread of another issues the products, four warps turn scores into P and
+// write outputs.  A thread of these holds a token's scores (a lane of tensor memory), and at the end a dimension's outputs.  What is not e4m3, q and
 // p, is written as four e4m3 pieces in columns of their own, x = x0 + x1 / 16 + x2 / 256 + x3 / 4096, each piece the
 // rounding of 16 times what the one before it left: a column tile of 16 holds four rows, which is the narrowest that the
 // instruction takes.
@@ -20,6 +21,7 @@
 // Other forms were measured at 48 requests of 700 to 16001 tokens, 8 heads of 128 (75 us at the copy rate): K and V converted
 // to f16 in registers for m16n8k16 104 us, the same from rings in shared memory 108 us, m16n8k32 on e4m3 (which sm_100
 // does not have: it is converted and issued as f16) 109 us: bound by the issue of conversions with few warps to hide them.
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -31,39 +33,41 @@
 namespace pf {
 namespace {
 
-constexpr int kThreads = 128, kTokens = 128, kGroups = kTokens / 16;   // tokens of a step, and of those that share a scale
+constexpr int kWorkers = 128, kThreads = kWorkers + 64;                // workers, then the feeding and the issuing warp
+constexpr int kTokens = 128, kGroups = kTokens / 16;                   // of a step; a group lies within a block
 constexpr float kShift = 6.f, kSlack = 2.f;
 
-__host__ __device__ constexpr int few_ctas(int dim, int rows) {        // of an SM: by shared and by tensor memory
-  return dim == 256 || rows == 64 ? 1 : rows == 32 ? 2 : dim == 128 ? 2 : 4;
-}
+__host__ __device__ constexpr int few_ctas(int dim, int rows) { return dim == 256 || rows >= 32 ? 1 : 2; }   // of an SM
 
 // Offsets in shared memory behind the first 1024-byte boundary.  kWithV: attention; otherwise the weights, which read K only.
 template <int kDim, int kRows, bool kWithV>
 struct Few {
   static constexpr int kN = 4 * kRows;                                 // columns
   static constexpr int kKv = kWithV ? 2 : 1, kTile = kTokens * kDim, kStage = kKv * kTile;
-  static constexpr int kP = 0, kQ = kP + (kWithV ? kTokens * kN : 0), kFirst = kQ + (kN * kDim < 1024 ? 1024 : kN * kDim);
+  static constexpr int kPBytes = kWithV ? kTokens * kN : 0;            // twice
+  static constexpr int kP = 0, kQ = 2 * kPBytes, kFirst = kQ + (kN * kDim < 1024 ? 1024 : kN * kDim);
   static constexpr int kRoom = 227 * 1024 / few_ctas(kDim, kRows) - 2 * 1024 - (kWithV ? 8 : 16) * 1024 - kFirst;   // Shared and Work
-  static constexpr int kFit = kRoom / kStage, kStages = kFit > 4 ? 4 : kFit;
+  static constexpr int kFit = kRoom / kStage, kStages = kFit > 6 ? 6 : kFit;
   static constexpr int kEnd = kFirst + kStages * kStage;
-  static constexpr int kColumns = kN * (1 + (kWithV ? (kDim == 256 ? 2 : 1) : 0));
+  static constexpr int kO = 2 * kN;                                    // first column of O behind two S
+  static constexpr int kColumns = kO + (kWithV ? kN * (kDim == 256 ? 2 : 1) : 0);
   static constexpr int kAlloc = kColumns <= 32 ? 32 : kColumns <= 64 ? 64 : kColumns <= 128 ? 128 : kColumns <= 256 ? 256 : 512;
   static_assert(kStages >= 2, "two tiles in flight");
-  static_assert(kAlloc * few_ctas(kDim, kRows) <= 512, "tensor memory");
+  static_assert(kColumns <= 512 && kAlloc * few_ctas(kDim, kRows) <= 512, "tensor memory");
 };
 
 constexpr int kPass = 16;      // steps whose weights are summed over the row tiles before they are added
 template <int kDim, int kRows, int kStages, bool kWithV>
 struct FewShared {
-  uint64_t s_full, pv_done;
+  float4 scale[kStages][2][kGroups];          // of K, of V: the four heads that share 16 bytes
+  uint64_t full[kStages], empty[kStages], q_ready, s_full[2], p_ready[2], pv_done[2];
+  uint32_t there[kStages];                    // bits of the groups whose block is in the cache
   uint32_t tmem;
   int stalled, any_nan;
-  float k_scale[kStages][kGroups], v_scale[kStages][kGroups];          // V's is -1 where there is no block
   float factor[kRows], ref[kRows], down[kRows], base[kRows], top[4][kRows], sum[4][kRows], v_top[4];
   int see[kRows];
   int nan_from[kDim];
-  float weight[kWithV ? 1 : kPass][kThreads];
+  float weight[kWithV ? 1 : kPass][kWorkers];
 };
 
 // Where 16-byte chunk c of row r lies: rows of 128 bytes (64 at 64 dimensions; two panels at 256) swizzled over eight rows.
@@ -76,10 +80,20 @@ __device__ __forceinline__ int place(int r, int c, int panel_rows) {
 template <int kDim>
 constexpr __host__ __device__ uint32_t swizzle_of() { return kDim == 64 ? kSwizzle64 : kSwizzle128; }
 
+// Barriers of the workers alone; whole warps come to them.
+__device__ __forceinline__ void workers_sync() { __syncwarp(); asm volatile("barrier.cta.sync.aligned 1, 128;" ::: "memory"); }
+__device__ __forceinline__ bool workers_or(bool x) {
+  uint32_t y;
+  __syncwarp();
+  asm volatile("{.reg .pred p, q; setp.ne.u32 p, %1, 0; barrier.cta.red.or.pred.aligned q, 1, 128, p; selp.u32 %0, 1, 0, q;}" : "=r"(y) : "r"((uint32_t)x) : "memory");
+  return y;
+}
+__device__ __forceinline__ bool workers_and(bool x) { return !workers_or(!x); }
+
 template <int kDim, int kRows, bool kWithV, bool kBf16>
-__global__ void __launch_bounds__(kThreads, few_ctas(kDim, kRows)) kv8_attention_few(AttnParams p) {
+__global__ void __launch_bounds__(kThreads, few_ctas(kDim, kRows)) kv8_attention_few(AttnParams p, const __grid_constant__ CUtensorMap map) {
   using L = Few<kDim, kRows, kWithV>;
-  constexpr int kN = L::kN, kStages = L::kStages, kChunks = kRows / 4, kRowBytes = kDim == 64 ? 64 : 128;
+  constexpr int kN = L::kN, kStages = L::kStages, kChunks = kRows / 4, kRowBytes = kDim == 64 ? 64 : 128, kHalves = kDim == 256 ? 2 : 1;
   using SeqT = Seq<kRows, kTokens, !kWithV>;
   using SharedT = FewShared<kDim, kRows, kStages, kWithV>;
   extern __shared__ char raw[];
@@ -87,13 +101,21 @@ __global__ void __launch_bounds__(kThreads, few_ctas(kDim, kRows)) kv8_attention
   SharedT &sh = *reinterpret_cast<SharedT *>(smem + L::kEnd);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
-    bar_init(&sh.s_full, 1);
-    bar_init(&sh.pv_done, 1);
+    for (int i = 0; i < kStages; ++i) {
+      bar_init(&sh.full[i], 1);
+      bar_init(&sh.empty[i], 1);
+    }
+    bar_init(&sh.q_ready, kWorkers);
+    for (int i = 0; i < 2; ++i) {
+      bar_init(&sh.s_full[i], 1);
+      bar_init(&sh.p_ready[i], kWorkers);
+      bar_init(&sh.pv_done[i], 1);
+    }
     sh.stalled = 0;
     sh.any_nan = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 0) {
+  if (warp == 5) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(shared_of(&sh.tmem)), "n"(L::kAlloc) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
@@ -104,7 +126,7 @@ __global__ void __launch_bounds__(kThreads, few_ctas(kDim, kRows)) kv8_attention
   fence_before();
   __syncthreads();
   fence_after();
-  const uint32_t tmem = sh.tmem, lanes = tmem + ((uint32_t)warp * 32 << 16);
+  const uint32_t tmem = sh.tmem;
   const uint32_t at_p = shared_of(smem + L::kP), at_q = shared_of(smem + L::kQ), at_stage = shared_of(smem + L::kFirst);
   const Split split(work.total(), kWithV ? p.n_ctas : (int)gridDim.x);
   if (blockIdx.x == 0) {
@@ -116,11 +138,7 @@ __global__ void __launch_bounds__(kThreads, few_ctas(kDim, kRows)) kv8_attention
   uint32_t u = 0, u_end = 0;
   if ((int)blockIdx.x < split.n_ctas) u = split.begin(blockIdx.x), u_end = split.begin(blockIdx.x + 1);
   bool first_segment = true, ok = true;
-  uint32_t n_scores = 0, n_outputs = 0;     // products waited for so far: phases of the two barriers
-  const int within = p.cache.block_size() - 1;
-  // a thread's copies: chunk `sub` of rows row_of, row_of + kAtOnce, ...
-  constexpr int kLanes = kDim / 16, kAtOnce = kThreads / kLanes, kCopies = kTokens / kAtOnce;
-  const int sub = tid % kLanes, row_of = tid / kLanes;
+  uint32_t n_tiles = 0, n_rows = 0;         // tiles and row tiles so far: what all roles count phases by
 
   while (u < u_end && ok) {
     const Segment seg(p, work, u);
@@ -131,10 +149,7 @@ __global__ void __launch_bounds__(kThreads, few_ctas(kDim, kRows)) kv8_attention
     // Attention: one row tile.  Weights: all of them, one after the other, each over all units.
     const int tiles = kWithV ? 1 : (all_rows + kRows - 1) / kRows;
     const int units = (int)min(min(seg.units - unit0, u_end - u), tiles > 1 ? (uint32_t)kPass : 0xffffffffu);
-    const int32_t *table = p.batch.tables + s * p.batch.table_stride;
-    const char *tile_of[2] = {p.cache.base + head * p.cache.tile_bytes(), p.cache.base + p.cache.kv_stride + head * p.cache.tile_bytes()};
-    const char *scale_of = p.cache.base + p.cache.heads * p.cache.tile_bytes() + 4 * head;
-    if (tiles > 1)
+    if (!kWithV && tiles > 1 && warp < 4)
       for (int j = 0; j < units; ++j) sh.weight[j][tid] = 0.f;         // a thread's own
     for (int tile = 0; tile < tiles && ok; ++tile) {
       const int row_first = (kWithV ? seg.rt : tile) * kRows, live_rows = min(all_rows - row_first, kRows);
@@ -142,360 +157,399 @@ __global__ void __launch_bounds__(kThreads, few_ctas(kDim, kRows)) kv8_attention
       const int least = seq.visible(p, row_first);                       // tokens that all rows see
       const int tok0 = (int)(unit0 * kTokens), tok_end = min(seq.len, kWithV ? most : min(most, p.w_capacity));
       const int steps = max(0, min(units, (tok_end - tok0 + kTokens - 1) / kTokens));
-
-      // pages of a step, looked up one step before they are asked for
-      uint32_t page[kCopies];
-      auto look_up = [&](int j) {
-#pragma unroll
-        for (int i = 0; i < kCopies; ++i) {
-          const int tok = tok0 + j * kTokens + i * kAtOnce + row_of;
-          page[i] = tok < tok_end ? (uint32_t)table[tok >> p.cache.block_log2] : 0xffffffffu;
-        }
-      };
-      auto ask = [&](int j) {             // always one group of copies
-        if (j < steps) {
-          const int stage = j % kStages, tok1 = tok0 + j * kTokens;
-          const uint32_t dst = at_stage + stage * L::kStage;
-#pragma unroll
-          for (int i = 0; i < kCopies; ++i) {
-            const int row = i * kAtOnce + row_of;
-            // rows behind the last token, and of blocks that are not in the cache, become zeros
-            const bool there = page[i] < p.cache.num_blocks && tok1 + row < seq.len;
-            const uint64_t from = there ? (uint64_t)page[i] * (uint32_t)p.cache.block_stride + (uint32_t)(((tok1 + row) & within) * kDim + 16 * sub) : 0;
-            const int bytes = there ? 16 : 0;
-#pragma unroll
-            for (int kv = 0; kv < L::kKv; ++kv)
-              asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + kv * L::kTile + place<kDim>(row, sub, kTokens)),
-                           "l"(tile_of[kv] + from), "r"(bytes)
-                           : "memory");
+      if (warp == 4) {
+        // ---------------------------------------------------------------- feeding: lane = (values or scales, K or V, group)
+        const int32_t *table = p.batch.tables + s * p.batch.table_stride;
+        const int group = lane & 7, kv = lane >> 3 & 1;
+        const bool values = lane < 16, part = kv < L::kKv;
+        const char *scale_of = p.cache.base + kv * p.cache.kv_stride + p.cache.heads * p.cache.tile_bytes() + 16 * (head >> 2);
+        auto look_up = [&](int j) {
+          const int tok = tok0 + j * kTokens + 16 * group;
+          return tok < tok_end ? (uint32_t)table[tok >> p.cache.block_log2] : 0xffffffffu;
+        };
+        uint32_t next = look_up(0);
+        for (int j = 0; j < steps; ++j) {
+          const uint32_t at = n_tiles + j, stage = at % kStages, id = next;
+          if (j + 1 < steps) next = look_up(j + 1);
+          const int tok = tok0 + j * kTokens + 16 * group;
+          const bool there = id < p.cache.num_blocks;
+          if (!there && tok < tok_end && lane < 8) p.batch.report(PF_KV8_BAD_BLOCK);
+          const uint32_t all = __ballot_sync(0xffffffffu, there);
+          if (!(ok = bar_wait_warp(&sh.empty[stage], (at / kStages & 1) ^ 1, &sh.stalled))) break;
+          if (lane == 0) {
+            sh.there[stage] = all & 0xff;
+            asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(shared_of(&sh.full[stage])),
+                         "r"((uint32_t)(L::kStage + 16 * L::kKv * __popc(all & 0xff)))
+                         : "memory");
           }
-          if (tid < kGroups) {
-            const int tok = tok1 + 16 * tid;
-            const uint32_t id = tok < tok_end ? (uint32_t)table[tok >> p.cache.block_log2] : 0xffffffffu;
-            if (id < p.cache.num_blocks) {
-              const char *at = scale_of + (uint64_t)id * (uint32_t)p.cache.block_stride;
-              asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(shared_of(&sh.k_scale[stage][tid])), "l"(at) : "memory");
-              if (kWithV)
-                asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(shared_of(&sh.v_scale[stage][tid])), "l"(at + p.cache.kv_stride) : "memory");
-              else
-                sh.v_scale[stage][tid] = 1.f;
-            } else {
-              if (tok < tok_end) p.batch.report(PF_KV8_BAD_BLOCK);
-              sh.k_scale[stage][tid] = 0.f;
-              sh.v_scale[stage][tid] = -1.f;
-            }
+          __syncwarp();
+          if (values && part) {
+            // a group that is not there lies behind the last block: the copy fills it with zeros
+            const int row = tok & (p.cache.block_size() - 1), block = there ? (int)id : (int)p.cache.num_blocks;
+#pragma unroll
+            for (int half = 0; half < kHalves; ++half)
+              asm volatile(
+                  "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(
+                      at_stage + stage * L::kStage + kv * L::kTile + half * (kTokens * 128) + group * 16 * kRowBytes),
+                  "l"(&map), "r"(half * 128), "r"(row), "r"(head), "r"(block), "r"(kv), "r"(shared_of(&sh.full[stage]))
+                  : "memory");
+          } else if (!values && part && there) {
+            asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], 16, [%2];" ::"r"(shared_of(&sh.scale[stage][kv][group])),
+                         "l"(scale_of + (uint64_t)id * (uint32_t)p.cache.block_stride), "r"(shared_of(&sh.full[stage]))
+                         : "memory");
           }
         }
-        asm volatile("cp.async.commit_group;" ::: "memory");
-      };
+      } else if (warp == 5) {
+        // ---------------------------------------------------------------- issuing
+        if (lane == 0 && steps > 0) {
+          constexpr uint32_t kScores = shape_of(kN, false, false), kOutputs = shape_of(kN, true, true);
+          ok = bar_wait(&sh.q_ready, n_rows & 1, &sh.stalled);
+          for (int j = 0; j <= steps && ok; ++j) {
+            const uint32_t at = n_tiles + j;
+            if (j < steps) {
+              const uint32_t stage = at % kStages, at_k = at_stage + stage * L::kStage;
+              if (!(ok = bar_wait(&sh.full[stage], at / kStages & 1, &sh.stalled))) break;
+              fence_after();
 #pragma unroll
-      for (int i = 0; i < kStages - 1; ++i) {
-        look_up(i);
-        ask(i);
-      }
-      look_up(kStages - 1);
-
-      // the rows' pieces, factors and lengths
-      for (int e = tid; e < kRows * kLanes; e += kThreads) {
-        const int r = e / kLanes, c = e % kLanes, row = row_first + r;
-        const bool live = r < live_rows;
-        const int i = live ? row / p.group : 0, qh = head * p.group + (live ? row % p.group : 0);
-        const uint16_t *src = p.q + (int64_t)(seq.row0 + i) * p.q_row + qh * p.q_head + 16 * c;
-        float x[16], top = 0.f;
-#pragma unroll
-        for (int k = 0; k < 16; k += 8) {
-          uint4 w = make_uint4(0, 0, 0, 0);
-          if (live) {
-            if (p.vec_q) w = *reinterpret_cast<const uint4 *>(src + k);
-            else {
-              const uint16_t *at = src + k;
-              w = make_uint4(at[0] | at[1] << 16, at[2] | at[3] << 16, at[4] | at[5] << 16, at[6] | at[7] << 16);
-            }
-          }
-          const uint32_t y[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-          for (int m = 0; m < 4; ++m) {
-            const float2 f = kBf16 ? make_float2(__uint_as_float(y[m] << 16), __uint_as_float(y[m] & 0xffff0000u)) : f32x2_from_f16x2(y[m]);
-            x[k + 2 * m] = f.x, x[k + 2 * m + 1] = f.y;
-            top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
-          }
-        }
-#pragma unroll
-        for (int d = 1; d < kLanes; d <<= 1) top = fmaxf(top, __shfl_xor_sync(__activemask(), top, d));
-        int ex = (int)(__float_as_uint(top) >> 23) - 127 - 7;
-        if (top == 0.f || top > 3.4e38f) ex = 0;
-        ex = max(ex, -126);
-        const float down = exp2i(-ex);
-        // an infinity would become 448
-#pragma unroll
-        for (int k = 0; k < 16; ++k) x[k] = fabsf(x[k]) > 3.4e38f ? __int_as_float(0x7fffffff) : x[k] * down;
-#pragma unroll
-        for (int piece = 0; piece < 4; ++piece) {
-          uint32_t w[4];
-#pragma unroll
-          for (int k = 0; k < 16; k += 4) {
-            const uint32_t lo = e4m3x2(x[k], x[k + 1]), hi = e4m3x2(x[k + 2], x[k + 3]);
-            w[k / 4] = lo | hi << 16;
-            const float2 a = f32x2_from_f16x2(f16x2_from_e4m3<0>(lo)), b = f32x2_from_f16x2(f16x2_from_e4m3<0>(hi));
-            x[k] = (x[k] - a.x) * 16.f, x[k + 1] = (x[k + 1] - a.y) * 16.f;
-            x[k + 2] = (x[k + 2] - b.x) * 16.f, x[k + 3] = (x[k + 3] - b.y) * 16.f;
-          }
-          const int n = 16 * (r / 4) + 4 * piece + r % 4;
-          *reinterpret_cast<uint4 *>(smem + L::kQ + place<kDim>(n, c, kN)) = make_uint4(w[0], w[1], w[2], w[3]);
-        }
-        if (c == 0) {
-          sh.factor[r] = p.scale * kLog2e * exp2i(ex);
-          sh.see[r] = live ? seq.visible(p, row) : 0;
-          sh.ref[r] = kNone;
-          // rows that are not there, or see nothing, weigh nothing
-          if (!kWithV) sh.base[r] = sh.see[r] > 0 ? p.lse[(int64_t)(seq.row0 + i) * p.q_heads + qh] * kLog2e : INFINITY;
-        }
-      }
-      float sum[kRows];
-#pragma unroll
-      for (int r = 0; r < kRows; ++r) sum[r] = 0.f;
-      float v_ref = 0.f;                     // 2^e_ref
-
-      for (int j = 0; j < steps; ++j) {
-        const int stage = j % kStages, tok1 = tok0 + j * kTokens, tok = tok1 + tid;
-        const uint32_t at_k = at_stage + stage * L::kStage, at_v = at_k + L::kTile;
-        asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
-        const bool partly = tok1 + kTokens > least;      // some row does not see all of it
-        if (kWithV && partly) {
-          // A NaN in V reaches the rows that see its token and no other: 0 * NaN would.  It is taken out, and the first such
-          // token remembered for each dimension.  (A thread's own copies: no other has to be waited for.)
-#pragma unroll 1
-          for (int i = 0; i < kCopies; ++i) {
-            const int row = i * kAtOnce + row_of;
-            uint32_t *w = reinterpret_cast<uint32_t *>(smem + L::kFirst + stage * L::kStage + L::kTile + place<kDim>(row, sub, kTokens));
-            uint32_t any = 0;
-            for (int k = 0; k < 4; ++k) any |= (w[k] & 0x7f7f7f7fu) + 0x01010101u;
-            if (!(any & 0x80808080u)) continue;
-            sh.any_nan = 1;
-            for (int k = 0; k < 16; ++k)
-              if ((w[k / 4] >> (8 * (k % 4)) & 0x7f) == 0x7f) {
-                atomicMin(&sh.nan_from[16 * sub + k], tok1 + row);
-                w[k / 4] &= ~(0xffu << (8 * (k % 4)));
+              for (int k = 0; k < kDim / 32; ++k) {
+                const uint32_t in = kDim == 64 ? k * 32 : k % 4 * 32;
+                mma_e4m3_ss(tmem + (at & 1) * kN, operand(at_k + k / 4 * (kTokens * 128) + in, 16, 8 * kRowBytes, swizzle_of<kDim>()),
+                            operand(at_q + k / 4 * (kN * 128) + in, 16, 8 * kRowBytes, swizzle_of<kDim>()), kScores, k != 0);
               }
+              commit(&sh.s_full[at & 1]);
+            }
+            if (j > 0) {          // the tile before: its scores have been read, and its P written
+              const uint32_t was = at - 1, stage = was % kStages, at_v = at_stage + stage * L::kStage + L::kTile;
+              if (!(ok = bar_wait(&sh.p_ready[was & 1], was >> 1 & 1, &sh.stalled))) break;
+              if (!kWithV) {      // K and its scales have been read
+                bar_arrive(&sh.empty[stage]);
+                continue;
+              }
+              fence_after();
+#pragma unroll
+              for (int half = 0; half < kHalves; ++half)
+#pragma unroll
+                for (int k = 0; k < kTokens / 32; ++k)
+                  // at 64 dimensions the second half of the rows repeats the first: nobody reads it
+                  mma_e4m3_ss(tmem + L::kO + half * kN, operand(at_v + half * (kTokens * 128) + k * 32 * kRowBytes, 0, 8 * kRowBytes, swizzle_of<kDim>()),
+                              operand(at_p + (was & 1) * L::kPBytes + k * 512, 128, kTokens * 16, kNoSwizzle), kOutputs, j > 1 || k != 0);
+              commit(&sh.pv_done[was & 1]);
+              commit(&sh.empty[stage]);
+            }
+          }
+        }
+      } else {
+        // ---------------------------------------------------------------- workers
+        const uint32_t lanes = tmem + ((uint32_t)warp * 32 << 16);
+        // the rows' pieces, factors and lengths
+        constexpr int kLanes = kDim / 16;
+        for (int e = tid; e < kRows * kLanes; e += kWorkers) {
+          const int r = e / kLanes, c = e % kLanes, row = row_first + r;
+          const bool live = r < live_rows;
+          const int i = live ? row / p.group : 0, qh = head * p.group + (live ? row % p.group : 0);
+          const uint16_t *src = p.q + (int64_t)(seq.row0 + i) * p.q_row + qh * p.q_head + 16 * c;
+          float x[16], top = 0.f;
+#pragma unroll
+          for (int k = 0; k < 16; k += 8) {
+            uint4 w = make_uint4(0, 0, 0, 0);
+            if (live) {
+              if (p.vec_q) w = *reinterpret_cast<const uint4 *>(src + k);
+              else {
+                const uint16_t *at = src + k;
+                w = make_uint4(at[0] | at[1] << 16, at[2] | at[3] << 16, at[4] | at[5] << 16, at[6] | at[7] << 16);
+              }
+            }
+            const uint32_t y[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int m = 0; m < 4; ++m) {
+              const float2 f = kBf16 ? make_float2(__uint_as_float(y[m] << 16), __uint_as_float(y[m] & 0xffff0000u)) : f32x2_from_f16x2(y[m]);
+              x[k + 2 * m] = f.x, x[k + 2 * m + 1] = f.y;
+              top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
+            }
+          }
+#pragma unroll
+          for (int d = 1; d < kLanes; d <<= 1) top = fmaxf(top, __shfl_xor_sync(__activemask(), top, d));
+          int ex = (int)(__float_as_uint(top) >> 23) - 127 - 7;
+          if (top == 0.f || top > 3.4e38f) ex = 0;
+          ex = max(ex, -126);
+          const float down = exp2i(-ex);
+          // an infinity would become 448
+#pragma unroll
+          for (int k = 0; k < 16; ++k) x[k] = fabsf(x[k]) > 3.4e38f ? __int_as_float(0x7fffffff) : x[k] * down;
+#pragma unroll
+          for (int piece = 0; piece < 4; ++piece) {
+            uint32_t w[4];
+#pragma unroll
+            for (int k = 0; k < 16; k += 4) {
+              const uint32_t lo = e4m3x2(x[k], x[k + 1]), hi = e4m3x2(x[k + 2], x[k + 3]);
+              w[k / 4] = lo | hi << 16;
+              const float2 a = f32x2_from_f16x2(f16x2_from_e4m3<0>(lo)), b = f32x2_from_f16x2(f16x2_from_e4m3<0>(hi));
+              x[k] = (x[k] - a.x) * 16.f, x[k + 1] = (x[k + 1] - a.y) * 16.f;
+              x[k + 2] = (x[k + 2] - b.x) * 16.f, x[k + 3] = (x[k + 3] - b.y) * 16.f;
+            }
+            const int n = 16 * (r / 4) + 4 * piece + r % 4;
+            *reinterpret_cast<uint4 *>(smem + L::kQ + place<kDim>(n, c, kN)) = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+          if (c == 0) {
+            sh.factor[r] = p.scale * kLog2e * exp2i(ex);
+            sh.see[r] = live ? seq.visible(p, row) : 0;
+            sh.ref[r] = kNone;
+            // rows that are not there, or see nothing, weigh nothing
+            if (!kWithV) sh.base[r] = sh.see[r] > 0 ? p.lse[(int64_t)(seq.row0 + i) * p.q_heads + qh] * kLog2e : INFINITY;
           }
         }
         fence_to_async();
-        fence_before();
-        __syncthreads();
-        if (tid == 0) {
+        if (steps > 0) bar_arrive(&sh.q_ready);
+        workers_sync();
+        float sum[kRows];
+#pragma unroll
+        for (int r = 0; r < kRows; ++r) sum[r] = 0.f;
+        float v_ref = 0.f;                     // 2^e_ref
+
+        for (int j = 0; j < steps; ++j) {
+          const uint32_t at = n_tiles + j, stage = at % kStages;
+          const int tok1 = tok0 + j * kTokens, tok = tok1 + tid;
+          ok = bar_wait(&sh.full[stage], at / kStages & 1, &sh.stalled);
+          if (kWithV && j > 1) ok = ok && bar_wait(&sh.pv_done[at & 1], (at - 2) >> 1 & 1, &sh.stalled);    // P's place is free
+          ok = ok && bar_wait(&sh.s_full[at & 1], at >> 1 & 1, &sh.stalled);
+          if (!(ok = workers_and(ok))) break;
           fence_after();
-          constexpr uint32_t kShape = shape_of(kN, false, false);
-#pragma unroll
-          for (int k = 0; k < kDim / 32; ++k) {
-            const uint32_t in = kDim == 64 ? k * 32 : k % 4 * 32;
-            mma_e4m3_ss(tmem, operand(at_k + k / 4 * (kTokens * 128) + in, 16, 8 * kRowBytes, swizzle_of<kDim>()),
-                        operand(at_q + k / 4 * (kN * 128) + in, 16, 8 * kRowBytes, swizzle_of<kDim>()), kShape, k != 0);
-          }
-          commit(&sh.s_full);
-        }
-        // the tile before is done with: its place is for the tile kStages - 1 ahead, and P for this one
-        if (kWithV && j > 0) {
-          ok = __syncthreads_and(bar_wait(&sh.pv_done, n_outputs++ & 1, &sh.stalled));
-          if (!ok) break;
-        }
-        const float k_scale = sh.k_scale[stage][tid / 16], v_scale = sh.v_scale[stage][tid / 16];
-        ok = __syncthreads_and(bar_wait(&sh.s_full, n_scores++ & 1, &sh.stalled));
-        if (!ok) break;
-        fence_after();
-        ask(j + kStages - 1);
-        look_up(j + kStages);
-        const bool gone = v_scale < 0.f;
-        auto scores = [&](int c, float (&x)[4]) {       // of rows 4 c .. 4 c + 3, for this thread's token
-          uint32_t y[16];
-          load16(y, lanes + 16 * c);
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const float lo = fmaf(__uint_as_float(y[12 + r]), 1.f / 16, __uint_as_float(y[8 + r]));
-            x[r] = fmaf(fmaf(lo, 1.f / 16, __uint_as_float(y[4 + r])), 1.f / 16, __uint_as_float(y[r])) * (sh.factor[4 * c + r] * k_scale);
-            if (partly || gone)
-              if (gone || tok >= sh.see[4 * c + r]) x[r] = -INFINITY;
-          }
-        };
-        if constexpr (!kWithV) {
-          float w = 0.f;
-#pragma unroll 2
-          for (int c = 0; c < kChunks; ++c) {
-            float x[4];
-            scores(c, x);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) w += exp2_fast(x[r] - sh.base[4 * c + r]);
-          }
-          if (tiles > 1) sh.weight[j][tid] += w;
-          else if (tok < tok_end && !gone) p.weights[s * p.w_seq + head * p.w_head + tok] += w;
-        } else {
-          float first[4];
-          bool over = v_scale > v_ref;
-#pragma unroll
-          for (int c = 0; c < kChunks; ++c) {
-            float x[4];
-            scores(c, x);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              over |= x[r] > sh.ref[4 * c + r] + kSlack;
-              if (c == 0) first[r] = x[r];
+          const bool partly = tok1 + kTokens > least;      // some row does not see all of it
+          const int of_group = tid >> 4;
+          const bool gone = !(sh.there[stage] >> of_group & 1);
+          const float k_scale = gone ? 0.f : reinterpret_cast<const float *>(&sh.scale[stage][0][of_group])[head & 3];
+          const float v_scale = gone || !kWithV ? -1.f : reinterpret_cast<const float *>(&sh.scale[stage][1][of_group])[head & 3];
+          if (kWithV && partly) {
+            // Rows behind the last token hold what the block held before.  A NaN reaches the rows that see its token and no
+            // other: 0 * NaN would.  It is taken out, and the first such token remembered for each dimension.
+#pragma unroll 1
+            for (int e = tid; e < kTokens * kLanes; e += kWorkers) {
+              const int row = e / kLanes, c = e % kLanes;
+              uint4 *chunk = reinterpret_cast<uint4 *>(smem + L::kFirst + stage * L::kStage + L::kTile + place<kDim>(row, c, kTokens));
+              if (tok1 + row >= seq.len) {
+                *chunk = make_uint4(0, 0, 0, 0);
+                continue;
+              }
+              uint32_t *w = reinterpret_cast<uint32_t *>(chunk), any = 0;
+              for (int k = 0; k < 4; ++k) any |= (w[k] & 0x7f7f7f7fu) + 0x01010101u;
+              if (!(any & 0x80808080u)) continue;
+              sh.any_nan = 1;
+              for (int k = 0; k < 16; ++k)
+                if ((w[k / 4] >> (8 * (k % 4)) & 0x7f) == 0x7f) {
+                  atomicMin(&sh.nan_from[16 * c + k], tok1 + row);
+                  w[k / 4] &= ~(0xffu << (8 * (k % 4)));
+                }
             }
           }
-          if (__syncthreads_or(over)) {
-            // new references: the largest scores of the tile, the largest of V's scales
-            float v_top = v_scale;
+          __syncwarp();
+          const uint32_t at_s = lanes + (at & 1) * kN;
+          auto scores = [&](int c, float (&x)[4]) {       // of rows 4 c .. 4 c + 3, for this thread's token
+            uint32_t y[16];
+            load16(y, at_s + 16 * c);
 #pragma unroll
-            for (int d = 1; d < 32; d <<= 1) v_top = fmaxf(v_top, __shfl_xor_sync(0xffffffffu, v_top, d));
-            if (lane == 0) sh.v_top[warp] = v_top;
-#pragma unroll 1
+            for (int r = 0; r < 4; ++r) {
+              const float lo = fmaf(__uint_as_float(y[12 + r]), 1.f / 16, __uint_as_float(y[8 + r]));
+              x[r] = fmaf(fmaf(lo, 1.f / 16, __uint_as_float(y[4 + r])), 1.f / 16, __uint_as_float(y[r])) * (sh.factor[4 * c + r] * k_scale);
+              if (partly || gone)
+                if (gone || tok >= sh.see[4 * c + r]) x[r] = -INFINITY;
+            }
+          };
+          if constexpr (!kWithV) {
+            float w = 0.f;
+#pragma unroll 2
+            for (int c = 0; c < kChunks; ++c) {
+              float x[4];
+              scores(c, x);
+#pragma unroll
+              for (int r = 0; r < 4; ++r) w += exp2_fast(x[r] - sh.base[4 * c + r]);
+            }
+            fence_before();
+            bar_arrive(&sh.p_ready[at & 1]);
+            if (tiles > 1) sh.weight[j][tid] += w;
+            else if (tok < tok_end && !gone) p.weights[s * p.w_seq + head * p.w_head + tok] += w;
+          } else {
+            float first[4];
+            bool over = v_scale > v_ref;
+#pragma unroll
             for (int c = 0; c < kChunks; ++c) {
               float x[4];
               scores(c, x);
 #pragma unroll
               for (int r = 0; r < 4; ++r) {
-#pragma unroll
-                for (int d = 1; d < 32; d <<= 1) x[r] = fmaxf(x[r], __shfl_xor_sync(0xffffffffu, x[r], d));
-                if (lane == 0) sh.top[warp][4 * c + r] = x[r];
+                over |= x[r] > sh.ref[4 * c + r] + kSlack;
+                if (c == 0) first[r] = x[r];
               }
             }
-            __syncthreads();
-            v_top = fmaxf(fmaxf(fmaxf(sh.v_top[0], sh.v_top[1]), fmaxf(sh.v_top[2], sh.v_top[3])), fmaxf(v_ref, 0x1p-110f));
-            const float v_down = v_ref / v_top;          // powers of two; 0 at the start
-            v_ref = v_top;
-            if (tid < kRows) {
-              const float was = sh.ref[tid];
-              const float top = fmaxf(fmaxf(sh.top[0][tid], sh.top[1][tid]), fmaxf(sh.top[2][tid], sh.top[3][tid]));
-              const float now = top > was + kSlack ? top : was;
-              sh.ref[tid] = now;
-              sh.down[tid] = exp2_fast(was - now);
-            }
-            __syncthreads();
+            if (workers_or(over)) {
+              // new references: the largest scores of the tile, the largest of V's scales
+              float v_top = v_scale;
 #pragma unroll
-            for (int r = 0; r < kRows; ++r) sum[r] *= sh.down[r];
-            if (j > 0) {
+              for (int d = 1; d < 32; d <<= 1) v_top = fmaxf(v_top, __shfl_xor_sync(0xffffffffu, v_top, d));
+              if (lane == 0) sh.v_top[warp] = v_top;
 #pragma unroll 1
-              for (int half = 0; half < (kDim == 256 ? 2 : 1); ++half)
-#pragma unroll 1
-                for (int c = 0; c < kChunks; ++c) {
-                  uint32_t y[16];
-                  load16(y, lanes + kN * (1 + half) + 16 * c);
+              for (int c = 0; c < kChunks; ++c) {
+                float x[4];
+                scores(c, x);
 #pragma unroll
-                  for (int k = 0; k < 16; ++k) y[k] = __float_as_uint(__uint_as_float(y[k]) * (sh.down[4 * c + k % 4] * v_down));
-                  store16(lanes + kN * (1 + half) + 16 * c, y);
+                for (int r = 0; r < 4; ++r) {
+#pragma unroll
+                  for (int d = 1; d < 32; d <<= 1) x[r] = fmaxf(x[r], __shfl_xor_sync(0xffffffffu, x[r], d));
+                  if (lane == 0) sh.top[warp][4 * c + r] = x[r];
                 }
-              wait_stores();
-            }
-          }
-          // quotient of two powers of two, by their exponents; 0 where it is too small for any piece
-          const float on_p = v_scale > v_ref * 0x1p-60f ? __int_as_float(0x3f800000 + __float_as_int(v_scale) - __float_as_int(v_ref)) : 0.f;
+              }
+              if (j > 0) ok = bar_wait(&sh.pv_done[(at - 1) & 1], (at - 1) >> 1 & 1, &sh.stalled);
+              if (!(ok = workers_and(ok))) break;
+              fence_after();
+              v_top = fmaxf(fmaxf(fmaxf(sh.v_top[0], sh.v_top[1]), fmaxf(sh.v_top[2], sh.v_top[3])), fmaxf(v_ref, 0x1p-110f));
+              const float v_down = v_ref / v_top;          // powers of two; 0 at the start
+              v_ref = v_top;
+              if (tid < kRows) {
+                const float was = sh.ref[tid];
+                const float top = fmaxf(fmaxf(sh.top[0][tid], sh.top[1][tid]), fmaxf(sh.top[2][tid], sh.top[3][tid]));
+                const float now = top > was + kSlack ? top : was;
+                sh.ref[tid] = now;
+                sh.down[tid] = exp2_fast(was - now);
+              }
+              workers_sync();
 #pragma unroll
-          for (int c = 0; c < kChunks; ++c) {
-            float x[4];
-            if (c == 0) x[0] = first[0], x[1] = first[1], x[2] = first[2], x[3] = first[3];
-            else scores(c, x);
+              for (int r = 0; r < kRows; ++r) sum[r] *= sh.down[r];
+              if (j > 0) {
+#pragma unroll 1
+                for (int c = 0; c < kHalves * kChunks; ++c) {
+                  uint32_t y[16];
+                  load16(y, lanes + L::kO + 16 * c);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              x[r] = exp2_fast(x[r] - (sh.ref[4 * c + r] - kShift));
-              sum[4 * c + r] += x[r];
-            }
-            uint32_t h[2] = {f16x2(x[0] * on_p, x[1] * on_p), f16x2(x[2] * on_p, x[3] * on_p)}, w[4];
-#pragma unroll
-            for (int piece = 0; piece < 4; ++piece) {
-              w[piece] = e4m3x4_from_f16(h[0], h[1]);
-              if (piece == 3) break;
-              const uint32_t back[2] = {f16x2_from_e4m3<0>(w[piece]), f16x2_from_e4m3<1>(w[piece])};
-#pragma unroll
-              for (int k = 0; k < 2; ++k) {
-                const __half2 left = __hmul2(__hsub2(*reinterpret_cast<const __half2 *>(&h[k]), *reinterpret_cast<const __half2 *>(&back[k])),
-                                             __float2half2_rn(16.f));
-                h[k] = *reinterpret_cast<const uint32_t *>(&left);
+                  for (int k = 0; k < 16; ++k) y[k] = __float_as_uint(__uint_as_float(y[k]) * (sh.down[4 * (c % kChunks) + k % 4] * v_down));
+                  store16(lanes + L::kO + 16 * c, y);
+                }
+                wait_stores();
               }
             }
-            *reinterpret_cast<uint4 *>(smem + L::kP + c * (kTokens * 16) + tid * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+            // quotient of two powers of two, by their exponents; 0 where it is too small for any piece
+            const float on_p = v_scale > v_ref * 0x1p-60f ? __int_as_float(0x3f800000 + __float_as_int(v_scale) - __float_as_int(v_ref)) : 0.f;
+#pragma unroll
+            for (int c = 0; c < kChunks; ++c) {
+              float x[4];
+              if (c == 0) x[0] = first[0], x[1] = first[1], x[2] = first[2], x[3] = first[3];
+              else scores(c, x);
+#pragma unroll
+              for (int r = 0; r < 4; ++r) {
+                x[r] = exp2_fast(x[r] - (sh.ref[4 * c + r] - kShift));
+                sum[4 * c + r] += x[r];
+              }
+              uint32_t h[2] = {f16x2(x[0] * on_p, x[1] * on_p), f16x2(x[2] * on_p, x[3] * on_p)}, w[4];
+#pragma unroll
+              for (int piece = 0; piece < 4; ++piece) {
+                w[piece] = e4m3x4_from_f16(h[0], h[1]);
+                if (piece == 3) break;
+                const uint32_t back[2] = {f16x2_from_e4m3<0>(w[piece]), f16x2_from_e4m3<1>(w[piece])};
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                  const __half2 left = __hmul2(__hsub2(*reinterpret_cast<const __half2 *>(&h[k]), *reinterpret_cast<const __half2 *>(&back[k])),
+                                               __float2half2_rn(16.f));
+                  h[k] = *reinterpret_cast<const uint32_t *>(&left);
+                }
+              }
+              *reinterpret_cast<uint4 *>(smem + L::kP + (at & 1) * L::kPBytes + c * (kTokens * 16) + tid * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+            fence_to_async();
+            fence_before();
+            bar_arrive(&sh.p_ready[at & 1]);
           }
-          fence_to_async();
-          fence_before();
-          __syncthreads();
-          if (tid == 0) {
+        }
+        if constexpr (kWithV) {
+          const uint32_t last = n_tiles + steps - 1;
+          if (steps > 0) ok = ok && bar_wait(&sh.pv_done[last & 1], last >> 1 & 1, &sh.stalled);
+          if ((ok = workers_and(ok))) {
             fence_after();
-            constexpr uint32_t kShape = shape_of(kN, true, true);
+            // row sums over the threads
 #pragma unroll
-            for (int half = 0; half < (kDim == 256 ? 2 : 1); ++half)
+            for (int r = 0; r < kRows; ++r) {
 #pragma unroll
-              for (int k = 0; k < kTokens / 32; ++k)
-                // at 64 dimensions the second half of the rows repeats the first: nobody reads it
-                mma_e4m3_ss(tmem + kN * (1 + half), operand(at_v + half * (kTokens * 128) + k * 32 * kRowBytes, 0, 8 * kRowBytes, swizzle_of<kDim>()),
-                            operand(at_p + k * 512, 128, kTokens * 16, kNoSwizzle), kShape, j > 0 || k != 0);
-            commit(&sh.pv_done);
-          }
-        }
-      }
-      asm volatile("cp.async.wait_all;" ::: "memory");
-      if constexpr (kWithV) {
-        if (ok && steps > 0) ok = __syncthreads_and(bar_wait(&sh.pv_done, n_outputs++ & 1, &sh.stalled));
-        if (!ok) break;
-        fence_after();
-        // row sums over the threads
-#pragma unroll
-        for (int r = 0; r < kRows; ++r) {
-#pragma unroll
-          for (int d = 1; d < 32; d <<= 1) sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], d);
-          if (lane == 0) sh.sum[warp][r] = sum[r];
-        }
-        __syncthreads();
-        const bool whole = units == (int)seg.units, any_nan = sh.any_nan;
-        const int slot = 2 * blockIdx.x + (first_segment ? 0 : 1);
+              for (int d = 1; d < 32; d <<= 1) sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], d);
+              if (lane == 0) sh.sum[warp][r] = sum[r];
+            }
+            workers_sync();
+            const bool whole = units == (int)seg.units, any_nan = sh.any_nan;
+            const int slot = 2 * blockIdx.x + (first_segment ? 0 : 1);
 #pragma unroll 1
-        for (int half = 0; half < (kDim == 256 ? 2 : 1); ++half) {
-          const int d = half * 128 + tid;
+            for (int half = 0; half < kHalves; ++half) {
+              const int d = half * 128 + tid;
 #pragma unroll 1
-          for (int c = 0; c < (live_rows + 3) / 4; ++c) {
-            uint32_t y[16];
-            load16(y, lanes + kN * (1 + half) + 16 * c);
+              for (int c = 0; c < (live_rows + 3) / 4; ++c) {
+                uint32_t y[16];
+                load16(y, lanes + L::kO + half * kN + 16 * c);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const int r = 4 * c + k;
-              if (r >= live_rows || d >= kDim) continue;
-              const float l = sh.sum[0][r] + sh.sum[1][r] + sh.sum[2][r] + sh.sum[3][r];
-              const float lo = fmaf(__uint_as_float(y[12 + k]), 1.f / 16, __uint_as_float(y[8 + k]));
-              float a = fmaf(fmaf(lo, 1.f / 16, __uint_as_float(y[4 + k])), 1.f / 16, __uint_as_float(y[k])) * v_ref;
-              if (steps == 0 || l == 0.f) a = 0.f;
-              if (any_nan && sh.nan_from[d] < sh.see[r]) a = __int_as_float(0x7fffffff);
-              const int row = row_first + r, i = row / p.group, qh = head * p.group + row % p.group;
-              const float base = sh.ref[r] - kShift;
-              if (whole) {
-                a = l == 0.f ? a : a / l;
-                uint16_t *dst = p.out + (int64_t)(seq.row0 + i) * p.out_row + qh * p.out_head + d;
-                *dst = kBf16 ? __bfloat16_as_ushort(__float2bfloat16_rn(a)) : __half_as_ushort(__float2half_rn(a));
-                if (d == 0 && p.lse) p.lse[(int64_t)(seq.row0 + i) * p.q_heads + qh] = lse_of(base, l);
-              } else {
-                p.part_o[((int64_t)slot * kRows + r) * kDim + d] = a;
-                if (d == 0) p.part_ml[slot * kRows + r] = make_float2(base, l);
+                for (int k = 0; k < 4; ++k) {
+                  const int r = 4 * c + k;
+                  if (r >= live_rows || d >= kDim) continue;
+                  const float l = sh.sum[0][r] + sh.sum[1][r] + sh.sum[2][r] + sh.sum[3][r];
+                  const float lo = fmaf(__uint_as_float(y[12 + k]), 1.f / 16, __uint_as_float(y[8 + k]));
+                  float a = fmaf(fmaf(lo, 1.f / 16, __uint_as_float(y[4 + k])), 1.f / 16, __uint_as_float(y[k])) * v_ref;
+                  if (steps == 0 || l == 0.f) a = 0.f;
+                  if (any_nan && sh.nan_from[d] < sh.see[r]) a = __int_as_float(0x7fffffff);
+                  const int row = row_first + r, i = row / p.group, qh = head * p.group + row % p.group;
+                  const float base = sh.ref[r] - kShift;
+                  if (whole) {
+                    a = l == 0.f ? a : a / l;
+                    uint16_t *dst = p.out + (int64_t)(seq.row0 + i) * p.out_row + qh * p.out_head + d;
+                    *dst = kBf16 ? __bfloat16_as_ushort(__float2bfloat16_rn(a)) : __half_as_ushort(__float2half_rn(a));
+                    if (d == 0 && p.lse) p.lse[(int64_t)(seq.row0 + i) * p.q_heads + qh] = lse_of(base, l);
+                  } else {
+                    p.part_o[((int64_t)slot * kRows + r) * kDim + d] = a;
+                    if (d == 0) p.part_ml[slot * kRows + r] = make_float2(base, l);
+                  }
+                }
               }
+            }
+            fence_before();
+            workers_sync();
+            if (any_nan) {
+              for (int i = tid; i < kDim; i += kWorkers) sh.nan_from[i] = INT_MAX;
+              if (tid == 0) sh.any_nan = 0;
             }
           }
         }
-        fence_before();
-        __syncthreads();
-        if (any_nan) {
-          for (int i = tid; i < kDim; i += kThreads) sh.nan_from[i] = INT_MAX;
-          if (tid == 0) sh.any_nan = 0;
-        }
+        if ((ok = workers_and(ok)) && !kWithV && tiles > 1 && tile + 1 == tiles)
+          for (int j = 0; j < units; ++j) {
+            const int tok = (int)(unit0 + j) * kTokens + tid;
+            if (tok < min(seq.len, p.w_capacity)) p.weights[s * p.w_seq + head * p.w_head + tok] += sh.weight[j][tid];
+          }
       }
-      __syncthreads();         // the rows' pieces, factors and scales have been read
+      n_tiles += steps;
+      n_rows += steps > 0;
     }
-    if (!kWithV && tiles > 1)
-      for (int j = 0; j < units; ++j) {
-        const int tok = (int)(unit0 + j) * kTokens + tid;
-        if (tok < min(seq.len, p.w_capacity)) p.weights[s * p.w_seq + head * p.w_head + tok] += sh.weight[j][tid];
-      }
     u += units;
     first_segment = false;
   }
+  __syncwarp();
   fence_before();
   __syncthreads();
   fence_after();
   if (sh.stalled && tid == 0) p.batch.report(PF_KV8_STALLED);
-  if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(L::kAlloc));
+  if (warp == 5) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(L::kAlloc));
+}
+
+// The cache as [K or V][block][head][row][byte], tiles of 16 rows of (half) a head.
+CUtensorMap map_of(const Kv8View &c) {
+  using Encode = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
+                              const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  static const Encode encode = [] {
+    void *f = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &found) != cudaSuccess || found != cudaDriverEntryPointSuccess) f = nullptr;
+    return reinterpret_cast<Encode>(f);
+  }();
+  if (!encode) throw Error::cuda_init("cuTensorMapEncodeTiled is not available");
+  const cuuint64_t dims[5] = {(cuuint64_t)c.dim, (cuuint64_t)c.block_size(), (cuuint64_t)c.heads, c.num_blocks, 2};
+  const cuuint64_t strides[4] = {(cuuint64_t)c.dim, c.tile_bytes(), c.block_stride, c.kv_stride};
+  const cuuint32_t box[5] = {(cuuint32_t)std::min(c.dim, 128), 16, 1, 1, 1}, ones[5] = {1, 1, 1, 1, 1};
+  CUtensorMap map;
+  if (encode(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 5, c.base, dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             c.dim == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+    throw Error::invalid("8-bit cache: no tensor map describes it");
+  return map;
 }
 
 template <int kDim, int kRows, bool kWithV, bool kBf16>
@@ -506,7 +560,7 @@ void launch(const AttnParams &p, int n_ctas, cudaStream_t stream) {
                       Work<kRows, kTokens, !kWithV>::bytes(p.batch.n_seqs, p.row_tiles_most);
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
     throw Error::storage("cudaFuncSetAttribute failed");
-  launch_after(kernel, n_ctas, kThreads, smem, stream, p);
+  launch_after(kernel, n_ctas, kThreads, smem, stream, p, map_of(p.cache));
 }
 
 template <int kDim, bool kBf16>
