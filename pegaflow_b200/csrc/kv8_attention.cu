@@ -128,7 +128,7 @@ Plan make_plan(int device_id, const Kv8View &c, const pf_kv8_attention_args &a) 
   const size_t group = a.q_heads / c.heads;
   Plan plan{};
   const size_t rows = std::min(a.max_query, a.n_rows) * group;
-  plan.rows = kv8_few_rows((int64_t)rows);
+  plan.rows = kv8_few_rows(c.dim, (int64_t)rows);
   plan.wide = plan.rows == 0;
   if (plan.wide) plan.rows = kv8_wide_plan(c.dim).rows;
   plan.n_ctas = kv8_sm_count(device_id) * (plan.wide ? 1 : kv8_few_ctas(c.dim, plan.rows));

@@ -173,8 +173,9 @@ __device__ __forceinline__ void check_batch(const AttnParams &p) {
 
 __device__ __forceinline__ float lse_of(float base, float sum) { return sum == 0.f ? -INFINITY : (base + log2f(sum)) * kLn2; }
 
-// Few query rows (kv8_attention_few.cu): tiles of 4, 8, 16 or 32 rows, 0 when there are more.  And the accumulated weights.
-int kv8_few_rows(int64_t rows);
+// Few query rows (kv8_attention_few.cu): tiles of 4, 8, 16 or (not at 256 dimensions) 32
+// rows, 0 when there are more.  And the accumulated weights.
+int kv8_few_rows(int dim, int64_t rows);
 int kv8_few_ctas(int dim, int rows);      // CTAs of an SM
 void kv8_few_launch(const AttnParams &p, int rows, bool bf16, cudaStream_t stream);
 void kv8_weights_launch(const AttnParams &p, bool bf16, int n_sms, cudaStream_t stream);

@@ -7,8 +7,11 @@
 // keeps out of the way.  It does when no thread touches K and V at all: 128 tokens at a time go from global into shared memory
 // by TMA, and the tcgen05 tensor cores take the products on the e4m3 bytes as they are, transposed:
 //   S^T [128 tokens, columns] = K Q^T           O^T [head dimensions, columns] += V^T P^T
-// One warp feeds tiles, across the segments' ends, a thread of another issues the products, four warps turn scores into P and
-// write outputs.  A thread of these holds a token's scores (a lane of tensor memory), and at the end a dimension's outputs.  What is not e4m3, q and
+// One warp feeds tiles, across the segments' ends, a thread of another issues the products, and two teams of four warps take
+// tiles in turn, turn scores into P and write outputs.  Each team has references and sums of its own, joined at a segment's
+// end: a tile is a chain of some hundred dependent instructions for a team (2700 cycles with one team, whatever the
+// dimension, and half of HBM's rate for 64 dimensions or 8 rows), so that several have to run at a time.
+// A thread of a team holds a token's scores (a lane of tensor memory), and at the end a dimension's outputs.  What is not e4m3, q and
 // p, is written as four e4m3 pieces in columns of their own, x = x0 + x1 / 16 + x2 / 256 + x3 / 4096, each piece the
 // rounding of 16 times what the one before it left: a column tile of 16 holds four rows, which is the narrowest that the
 // instruction takes.
@@ -33,7 +36,7 @@
 namespace pf {
 namespace {
 
-constexpr int kWorkers = 128, kThreads = kWorkers + 64;                // workers, then the feeding and the issuing warp
+constexpr int kTeam = 128, kWorkers = 2 * kTeam, kThreads = kWorkers + 64;   // two teams, then the feeding and the issuing warp
 constexpr int kTokens = 128, kGroups = kTokens / 16;                   // of a step; a group lies within a block
 constexpr float kShift = 6.f, kSlack = 2.f;
 
@@ -43,31 +46,34 @@ __host__ __device__ constexpr int few_ctas(int dim, int rows) { return dim == 25
 template <int kDim, int kRows, bool kWithV>
 struct Few {
   static constexpr int kN = 4 * kRows;                                 // columns
-  static constexpr int kKv = kWithV ? 2 : 1, kTile = kTokens * kDim, kStage = kKv * kTile;
-  static constexpr int kPBytes = kWithV ? kTokens * kN : 0;            // twice
+  static constexpr int kKv = kWithV ? 2 : 1, kTile = kTokens * kDim;    // K and V take slots of a ring in turn: K's is free sooner
+  static constexpr int kPBytes = kWithV ? kTokens * kN : 0;            // of a team
   static constexpr int kP = 0, kQ = 2 * kPBytes, kFirst = kQ + (kN * kDim < 1024 ? 1024 : kN * kDim);
   static constexpr int kRoom = 227 * 1024 / few_ctas(kDim, kRows) - 2 * 1024 - (kWithV ? 8 : 16) * 1024 - kFirst;   // Shared and Work
-  static constexpr int kFit = kRoom / kStage, kStages = kFit > 6 ? 6 : kFit;
-  static constexpr int kEnd = kFirst + kStages * kStage;
-  static constexpr int kO = 2 * kN;                                    // first column of O behind two S
-  static constexpr int kColumns = kO + (kWithV ? kN * (kDim == 256 ? 2 : 1) : 0);
+  static constexpr int kFit = kRoom / kTile, kSlots = kFit > 12 ? 12 : kFit;
+  static constexpr int kEnd = kFirst + kSlots * kTile;
+  static constexpr int kO = 2 * kN;                                    // first column of the teams' O behind their S
+  static constexpr int kOEach = kN * (kDim == 256 ? 2 : 1), kColumns = kO + (kWithV ? 2 * kOEach : 0);
   static constexpr int kAlloc = kColumns <= 32 ? 32 : kColumns <= 64 ? 64 : kColumns <= 128 ? 128 : kColumns <= 256 ? 256 : 512;
-  static_assert(kStages >= 2, "two tiles in flight");
+  static_assert(kSlots >= 2 * kKv, "two tiles in flight");
   static_assert(kColumns <= 512 && kAlloc * few_ctas(kDim, kRows) <= 512, "tensor memory");
 };
 
 constexpr int kPass = 16;      // steps whose weights are summed over the row tiles before they are added
-template <int kDim, int kRows, int kStages, bool kWithV>
+// Tiles whose scales are kept: a tile is asked for at the earliest when the one six (of the weights: twelve) before it has left
+// its slot, for which the scores of that one's second successor had to be issued, which waits for the tile itself.
+constexpr int kRing = 16;
+template <int kDim, int kRows, int kSlots, bool kWithV>
 struct FewShared {
-  float4 scale[kStages][2][kGroups];          // of K, of V: the four heads that share 16 bytes
-  uint64_t full[kStages], empty[kStages], q_ready, s_full[2], p_ready[2], pv_done[2];
-  uint32_t there[kStages];                    // bits of the groups whose block is in the cache
+  float scale[kRing][2][kGroups];             // of K, of V; -1: the group's block is not in the cache
+  uint64_t full[kSlots], empty[kSlots], q_ready, s_full[2], p_ready[2], pv_done[2];
   uint32_t tmem;
   int stalled, any_nan;
-  float factor[kRows], ref[kRows], down[kRows], base[kRows], top[4][kRows], sum[4][kRows], v_top[4];
+  float factor[kRows], base[kRows];
+  float ref[2][kRows], down[2][kRows], top[2][4][kRows], sum[2][4][kRows], v_top[2][4], v_ref[2];
   int see[kRows];
   int nan_from[kDim];
-  float weight[kWithV ? 1 : kPass][kWorkers];
+  float weight[kWithV ? 1 : kPass][kTeam];
 };
 
 // Where 16-byte chunk c of row r lies: rows of 128 bytes (64 at 64 dimensions; two panels at 256) swizzled over eight rows.
@@ -80,42 +86,50 @@ __device__ __forceinline__ int place(int r, int c, int panel_rows) {
 template <int kDim>
 constexpr __host__ __device__ uint32_t swizzle_of() { return kDim == 64 ? kSwizzle64 : kSwizzle128; }
 
-// Barriers of the workers alone; whole warps come to them.
-__device__ __forceinline__ void workers_sync() { __syncwarp(); asm volatile("barrier.cta.sync.aligned 1, 128;" ::: "memory"); }
-__device__ __forceinline__ bool workers_or(bool x) {
+// Barriers of a team (ids 1 and 2) and of both (3); whole warps come to them.
+__device__ __forceinline__ void team_sync(int team) {
+  __syncwarp();
+  asm volatile("barrier.cta.sync.aligned %0, 128;" ::"r"(1 + team) : "memory");
+}
+template <int kCount>
+__device__ __forceinline__ bool any_of(int id, bool x) {
   uint32_t y;
   __syncwarp();
-  asm volatile("{.reg .pred p, q; setp.ne.u32 p, %1, 0; barrier.cta.red.or.pred.aligned q, 1, 128, p; selp.u32 %0, 1, 0, q;}" : "=r"(y) : "r"((uint32_t)x) : "memory");
+  asm volatile("{.reg .pred p, q; setp.ne.u32 p, %1, 0; barrier.cta.red.or.pred.aligned q, %2, %3, p; selp.u32 %0, 1, 0, q;}"
+               : "=r"(y)
+               : "r"((uint32_t)x), "r"(id), "n"(kCount)
+               : "memory");
   return y;
 }
-__device__ __forceinline__ bool workers_and(bool x) { return !workers_or(!x); }
+__device__ __forceinline__ bool team_any(int team, bool x) { return any_of<kTeam>(1 + team, x); }
+__device__ __forceinline__ bool workers_all(bool x) { return !any_of<kWorkers>(3, !x); }
 
 template <int kDim, int kRows, bool kWithV, bool kBf16>
 __global__ void __launch_bounds__(kThreads, few_ctas(kDim, kRows)) kv8_attention_few(AttnParams p, const __grid_constant__ CUtensorMap map) {
   using L = Few<kDim, kRows, kWithV>;
-  constexpr int kN = L::kN, kStages = L::kStages, kChunks = kRows / 4, kRowBytes = kDim == 64 ? 64 : 128, kHalves = kDim == 256 ? 2 : 1;
+  constexpr int kN = L::kN, kSlots = L::kSlots, kChunks = kRows / 4, kRowBytes = kDim == 64 ? 64 : 128, kHalves = kDim == 256 ? 2 : 1;
   using SeqT = Seq<kRows, kTokens, !kWithV>;
-  using SharedT = FewShared<kDim, kRows, kStages, kWithV>;
+  using SharedT = FewShared<kDim, kRows, kSlots, kWithV>;
   extern __shared__ char raw[];
   char *smem = raw + (1024 - (shared_of(raw) & 1023));
   SharedT &sh = *reinterpret_cast<SharedT *>(smem + L::kEnd);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
-    for (int i = 0; i < kStages; ++i) {
+    for (int i = 0; i < kSlots; ++i) {
       bar_init(&sh.full[i], 1);
       bar_init(&sh.empty[i], 1);
     }
     bar_init(&sh.q_ready, kWorkers);
     for (int i = 0; i < 2; ++i) {
       bar_init(&sh.s_full[i], 1);
-      bar_init(&sh.p_ready[i], kWorkers);
+      bar_init(&sh.p_ready[i], kTeam);
       bar_init(&sh.pv_done[i], 1);
     }
     sh.stalled = 0;
     sh.any_nan = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 5) {
+  if (warp == 9) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(shared_of(&sh.tmem)), "n"(L::kAlloc) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
@@ -127,7 +141,7 @@ __global__ void __launch_bounds__(kThreads, few_ctas(kDim, kRows)) kv8_attention
   __syncthreads();
   fence_after();
   const uint32_t tmem = sh.tmem;
-  const uint32_t at_p = shared_of(smem + L::kP), at_q = shared_of(smem + L::kQ), at_stage = shared_of(smem + L::kFirst);
+  const uint32_t at_p = shared_of(smem + L::kP), at_q = shared_of(smem + L::kQ), at_slot = shared_of(smem + L::kFirst);
   const Split split(work.total(), kWithV ? p.n_ctas : (int)gridDim.x);
   if (blockIdx.x == 0) {
     if (kWithV) check_batch(p);
@@ -138,7 +152,8 @@ __global__ void __launch_bounds__(kThreads, few_ctas(kDim, kRows)) kv8_attention
   uint32_t u = 0, u_end = 0;
   if ((int)blockIdx.x < split.n_ctas) u = split.begin(blockIdx.x), u_end = split.begin(blockIdx.x + 1);
   bool first_segment = true, ok = true;
-  uint32_t n_tiles = 0, n_rows = 0;         // tiles and row tiles so far: what all roles count phases by
+  // tiles so far, those of each team, and row tiles: what all roles count phases by
+  uint32_t n_tiles = 0, n_of[2] = {0, 0}, n_rows = 0;
 
   while (u < u_end && ok) {
     const Segment seg(p, work, u);
@@ -149,57 +164,62 @@ __global__ void __launch_bounds__(kThreads, few_ctas(kDim, kRows)) kv8_attention
     // Attention: one row tile.  Weights: all of them, one after the other, each over all units.
     const int tiles = kWithV ? 1 : (all_rows + kRows - 1) / kRows;
     const int units = (int)min(min(seg.units - unit0, u_end - u), tiles > 1 ? (uint32_t)kPass : 0xffffffffu);
-    if (!kWithV && tiles > 1 && warp < 4)
-      for (int j = 0; j < units; ++j) sh.weight[j][tid] = 0.f;         // a thread's own
+    if (!kWithV && tiles > 1 && warp < 8)
+      for (int j = warp >> 2; j < units; j += 2) sh.weight[j][tid % kTeam] = 0.f;         // a thread's own
     for (int tile = 0; tile < tiles && ok; ++tile) {
       const int row_first = (kWithV ? seg.rt : tile) * kRows, live_rows = min(all_rows - row_first, kRows);
       const int most = seq.visible(p, row_first + live_rows - 1);        // tokens that any row of the tile sees
       const int least = seq.visible(p, row_first);                       // tokens that all rows see
       const int tok0 = (int)(unit0 * kTokens), tok_end = min(seq.len, kWithV ? most : min(most, p.w_capacity));
       const int steps = max(0, min(units, (tok_end - tok0 + kTokens - 1) / kTokens));
-      if (warp == 4) {
-        // ---------------------------------------------------------------- feeding: lane = (values or scales, K or V, group)
+      if (warp == 8) {
+        // ---------------------------------------------------------------- feeding: lane = (values or scale, K or V, group)
         const int32_t *table = p.batch.tables + s * p.batch.table_stride;
         const int group = lane & 7, kv = lane >> 3 & 1;
-        const bool values = lane < 16, part = kv < L::kKv;
-        const char *scale_of = p.cache.base + kv * p.cache.kv_stride + p.cache.heads * p.cache.tile_bytes() + 16 * (head >> 2);
+        const char *scale_of = p.cache.base + kv * p.cache.kv_stride + p.cache.heads * p.cache.tile_bytes() + 4 * head;
         auto look_up = [&](int j) {
           const int tok = tok0 + j * kTokens + 16 * group;
           return tok < tok_end ? (uint32_t)table[tok >> p.cache.block_log2] : 0xffffffffu;
         };
-        uint32_t next = look_up(0);
+        // pages two tiles ahead, scales one: both are loads that wait for memory
+        auto scale_at = [&](uint32_t id) {
+          return lane >= 16 && kv < L::kKv && id < p.cache.num_blocks ? __ldg(reinterpret_cast<const float *>(scale_of + (uint64_t)id * (uint32_t)p.cache.block_stride)) : -1.f;
+        };
+        uint32_t id = look_up(0), next = look_up(1);
+        float scale = scale_at(id);
         for (int j = 0; j < steps; ++j) {
-          const uint32_t at = n_tiles + j, stage = at % kStages, id = next;
-          if (j + 1 < steps) next = look_up(j + 1);
+          const uint32_t at = n_tiles + j;
           const int tok = tok0 + j * kTokens + 16 * group;
           const bool there = id < p.cache.num_blocks;
           if (!there && tok < tok_end && lane < 8) p.batch.report(PF_KV8_BAD_BLOCK);
-          const uint32_t all = __ballot_sync(0xffffffffu, there);
-          if (!(ok = bar_wait_warp(&sh.empty[stage], (at / kStages & 1) ^ 1, &sh.stalled))) break;
-          if (lane == 0) {
-            sh.there[stage] = all & 0xff;
-            asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(shared_of(&sh.full[stage])),
-                         "r"((uint32_t)(L::kStage + 16 * L::kKv * __popc(all & 0xff)))
-                         : "memory");
-          }
-          __syncwarp();
-          if (values && part) {
-            // a group that is not there lies behind the last block: the copy fills it with zeros
-            const int row = tok & (p.cache.block_size() - 1), block = there ? (int)id : (int)p.cache.num_blocks;
+          // a group that is not there lies behind the last block: the copy fills it with zeros
+          const int row = tok & (p.cache.block_size() - 1), block = there ? (int)id : (int)p.cache.num_blocks;
+          id = next;
+          next = look_up(j + 2);
+          const float now = scale;
+          scale = scale_at(id);
 #pragma unroll
-            for (int half = 0; half < kHalves; ++half)
-              asm volatile(
-                  "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(
-                      at_stage + stage * L::kStage + kv * L::kTile + half * (kTokens * 128) + group * 16 * kRowBytes),
-                  "l"(&map), "r"(half * 128), "r"(row), "r"(head), "r"(block), "r"(kv), "r"(shared_of(&sh.full[stage]))
-                  : "memory");
-          } else if (!values && part && there) {
-            asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], 16, [%2];" ::"r"(shared_of(&sh.scale[stage][kv][group])),
-                         "l"(scale_of + (uint64_t)id * (uint32_t)p.cache.block_stride), "r"(shared_of(&sh.full[stage]))
-                         : "memory");
+          for (int of = 0; of < L::kKv; ++of) {
+            const uint32_t i = L::kKv * at + of, slot = i % kSlots;
+            if (!(ok = bar_wait_warp(&sh.empty[slot], (i / kSlots & 1) ^ 1, &sh.stalled))) break;
+            if (of == 0 && lane >= 16) sh.scale[at % kRing][kv][group] = now;
+            __syncwarp();
+            if (lane == 0)
+              asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(shared_of(&sh.full[slot])), "r"(L::kTile) : "memory");
+            __syncwarp();
+            if (lane < 16 && kv == of) {
+#pragma unroll
+              for (int half = 0; half < kHalves; ++half)
+                asm volatile(
+                    "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(
+                        at_slot + slot * L::kTile + half * (kTokens * 128) + group * 16 * kRowBytes),
+                    "l"(&map), "r"(half * 128), "r"(row), "r"(head), "r"(block), "r"(kv), "r"(shared_of(&sh.full[slot]))
+                    : "memory");
+            }
           }
+          if (!ok) break;
         }
-      } else if (warp == 5) {
+      } else if (warp == 9) {
         // ---------------------------------------------------------------- issuing
         if (lane == 0 && steps > 0) {
           constexpr uint32_t kScores = shape_of(kN, false, false), kOutputs = shape_of(kN, true, true);
@@ -207,40 +227,46 @@ __global__ void __launch_bounds__(kThreads, few_ctas(kDim, kRows)) kv8_attention
           for (int j = 0; j <= steps && ok; ++j) {
             const uint32_t at = n_tiles + j;
             if (j < steps) {
-              const uint32_t stage = at % kStages, at_k = at_stage + stage * L::kStage;
-              if (!(ok = bar_wait(&sh.full[stage], at / kStages & 1, &sh.stalled))) break;
+              const uint32_t i = L::kKv * at, slot = i % kSlots, at_k = at_slot + slot * L::kTile;
+              if (!(ok = bar_wait(&sh.full[slot], i / kSlots & 1, &sh.stalled))) break;
               fence_after();
 #pragma unroll
               for (int k = 0; k < kDim / 32; ++k) {
                 const uint32_t in = kDim == 64 ? k * 32 : k % 4 * 32;
-                mma_e4m3_ss(tmem + (at & 1) * kN, operand(at_k + k / 4 * (kTokens * 128) + in, 16, 8 * kRowBytes, swizzle_of<kDim>()),
+                mma_e4m3_ss(tmem + (j & 1) * kN, operand(at_k + k / 4 * (kTokens * 128) + in, 16, 8 * kRowBytes, swizzle_of<kDim>()),
                             operand(at_q + k / 4 * (kN * 128) + in, 16, 8 * kRowBytes, swizzle_of<kDim>()), kScores, k != 0);
               }
-              commit(&sh.s_full[at & 1]);
+              commit(&sh.s_full[j & 1]);
+              if (kWithV) commit(&sh.empty[slot]);
             }
             if (j > 0) {          // the tile before: its scores have been read, and its P written
-              const uint32_t was = at - 1, stage = was % kStages, at_v = at_stage + stage * L::kStage + L::kTile;
-              if (!(ok = bar_wait(&sh.p_ready[was & 1], was >> 1 & 1, &sh.stalled))) break;
-              if (!kWithV) {      // K and its scales have been read
-                bar_arrive(&sh.empty[stage]);
+              const int team = (j - 1) & 1;
+              const uint32_t i = L::kKv * (at - 1) + L::kKv - 1, slot = i % kSlots, at_v = at_slot + slot * L::kTile;
+              if (!(ok = bar_wait(&sh.p_ready[team], (n_of[team] + ((j - 1) >> 1)) & 1, &sh.stalled))) break;
+              if (!kWithV) {      // K has been read
+                bar_arrive(&sh.empty[slot]);
                 continue;
               }
+              // The workers have waited for V too, but V of two tiles need not land in order, and a team that runs ahead could take
+              // the barrier's phase for its own: in this thread every phase is waited for.
+              if (!(ok = bar_wait(&sh.full[slot], i / kSlots & 1, &sh.stalled))) break;
               fence_after();
 #pragma unroll
               for (int half = 0; half < kHalves; ++half)
 #pragma unroll
                 for (int k = 0; k < kTokens / 32; ++k)
                   // at 64 dimensions the second half of the rows repeats the first: nobody reads it
-                  mma_e4m3_ss(tmem + L::kO + half * kN, operand(at_v + half * (kTokens * 128) + k * 32 * kRowBytes, 0, 8 * kRowBytes, swizzle_of<kDim>()),
-                              operand(at_p + (was & 1) * L::kPBytes + k * 512, 128, kTokens * 16, kNoSwizzle), kOutputs, j > 1 || k != 0);
-              commit(&sh.pv_done[was & 1]);
-              commit(&sh.empty[stage]);
+                  mma_e4m3_ss(tmem + L::kO + team * L::kOEach + half * kN, operand(at_v + half * (kTokens * 128) + k * 32 * kRowBytes, 0, 8 * kRowBytes, swizzle_of<kDim>()),
+                              operand(at_p + team * L::kPBytes + k * 512, 128, kTokens * 16, kNoSwizzle), kOutputs, j > 2 || k != 0);
+              commit(&sh.pv_done[team]);
+              commit(&sh.empty[slot]);
             }
           }
         }
       } else {
         // ---------------------------------------------------------------- workers
-        const uint32_t lanes = tmem + ((uint32_t)warp * 32 << 16);
+        const int team = warp >> 2, own = tid % kTeam;       // the token of a tile, and the dimension, that are this thread's
+        const uint32_t lanes = tmem + ((uint32_t)(warp & 3) * 32 << 16), at_o = lanes + L::kO + team * L::kOEach;
         // the rows' pieces, factors and lengths
         constexpr int kLanes = kDim / 16;
         for (int e = tid; e < kRows * kLanes; e += kWorkers) {
@@ -293,39 +319,41 @@ __global__ void __launch_bounds__(kThreads, few_ctas(kDim, kRows)) kv8_attention
           if (c == 0) {
             sh.factor[r] = p.scale * kLog2e * exp2i(ex);
             sh.see[r] = live ? seq.visible(p, row) : 0;
-            sh.ref[r] = kNone;
+            sh.ref[0][r] = sh.ref[1][r] = kNone;
             // rows that are not there, or see nothing, weigh nothing
             if (!kWithV) sh.base[r] = sh.see[r] > 0 ? p.lse[(int64_t)(seq.row0 + i) * p.q_heads + qh] * kLog2e : INFINITY;
           }
         }
         fence_to_async();
         if (steps > 0) bar_arrive(&sh.q_ready);
-        workers_sync();
+        ok = workers_all(true);
         float sum[kRows];
 #pragma unroll
         for (int r = 0; r < kRows; ++r) sum[r] = 0.f;
         float v_ref = 0.f;                     // 2^e_ref
 
-        for (int j = 0; j < steps; ++j) {
-          const uint32_t at = n_tiles + j, stage = at % kStages;
-          const int tok1 = tok0 + j * kTokens, tok = tok1 + tid;
-          ok = bar_wait(&sh.full[stage], at / kStages & 1, &sh.stalled);
-          if (kWithV && j > 1) ok = ok && bar_wait(&sh.pv_done[at & 1], (at - 2) >> 1 & 1, &sh.stalled);    // P's place is free
-          ok = ok && bar_wait(&sh.s_full[at & 1], at >> 1 & 1, &sh.stalled);
-          if (!(ok = workers_and(ok))) break;
+        uint32_t turn = n_of[team];                  // tiles that the team had before this one
+        for (int j = team; j < steps; j += 2, ++turn) {
+          // V's slot (of the weights: K's) is not filled again before this tile is done with, and its barrier says that the
+          // scales are there too.  The scores come first: once they are issued, so is the product of the tile two before, and
+          // what was in this slot before has been waited for, so that the barrier is in this tile's phase or behind it.
+          const uint32_t at = n_tiles + j, i_slot = L::kKv * at + L::kKv - 1, slot = i_slot % kSlots;
+          const int tok1 = tok0 + j * kTokens, tok = tok1 + own;
+          ok = bar_wait_warp(&sh.s_full[team], turn & 1, &sh.stalled);
+          ok = ok && bar_wait_warp(&sh.full[slot], i_slot / kSlots & 1, &sh.stalled);
+          if (kWithV && j > 1) ok = ok && bar_wait_warp(&sh.pv_done[team], (turn - 1) & 1, &sh.stalled);    // P's place is free, O at rest
           fence_after();
           const bool partly = tok1 + kTokens > least;      // some row does not see all of it
-          const int of_group = tid >> 4;
-          const bool gone = !(sh.there[stage] >> of_group & 1);
-          const float k_scale = gone ? 0.f : reinterpret_cast<const float *>(&sh.scale[stage][0][of_group])[head & 3];
-          const float v_scale = gone || !kWithV ? -1.f : reinterpret_cast<const float *>(&sh.scale[stage][1][of_group])[head & 3];
+          const int of_group = own >> 4;
+          const float k_scale = sh.scale[at % kRing][0][of_group], v_scale = kWithV ? sh.scale[at % kRing][1][of_group] : 0.f;
+          const bool gone = k_scale < 0.f;
           if (kWithV && partly) {
             // Rows behind the last token hold what the block held before.  A NaN reaches the rows that see its token and no
             // other: 0 * NaN would.  It is taken out, and the first such token remembered for each dimension.
 #pragma unroll 1
-            for (int e = tid; e < kTokens * kLanes; e += kWorkers) {
+            for (int e = own; e < kTokens * kLanes; e += kTeam) {
               const int row = e / kLanes, c = e % kLanes;
-              uint4 *chunk = reinterpret_cast<uint4 *>(smem + L::kFirst + stage * L::kStage + L::kTile + place<kDim>(row, c, kTokens));
+              uint4 *chunk = reinterpret_cast<uint4 *>(smem + L::kFirst + slot * L::kTile + place<kDim>(row, c, kTokens));
               if (tok1 + row >= seq.len) {
                 *chunk = make_uint4(0, 0, 0, 0);
                 continue;
@@ -342,7 +370,7 @@ __global__ void __launch_bounds__(kThreads, few_ctas(kDim, kRows)) kv8_attention
             }
           }
           __syncwarp();
-          const uint32_t at_s = lanes + (at & 1) * kN;
+          const uint32_t at_s = lanes + team * kN;
           auto scores = [&](int c, float (&x)[4]) {       // of rows 4 c .. 4 c + 3, for this thread's token
             uint32_t y[16];
             load16(y, at_s + 16 * c);
@@ -364,28 +392,30 @@ __global__ void __launch_bounds__(kThreads, few_ctas(kDim, kRows)) kv8_attention
               for (int r = 0; r < 4; ++r) w += exp2_fast(x[r] - sh.base[4 * c + r]);
             }
             fence_before();
-            bar_arrive(&sh.p_ready[at & 1]);
-            if (tiles > 1) sh.weight[j][tid] += w;
+            if (!ok) break;
+            bar_arrive(&sh.p_ready[team]);
+            if (tiles > 1) sh.weight[j][own] += w;
             else if (tok < tok_end && !gone) p.weights[s * p.w_seq + head * p.w_head + tok] += w;
           } else {
             float first[4];
-            bool over = v_scale > v_ref;
+            bool over = v_scale > v_ref || !ok;
 #pragma unroll
             for (int c = 0; c < kChunks; ++c) {
               float x[4];
               scores(c, x);
 #pragma unroll
               for (int r = 0; r < 4; ++r) {
-                over |= x[r] > sh.ref[4 * c + r] + kSlack;
+                over |= x[r] > sh.ref[team][4 * c + r] + kSlack;
                 if (c == 0) first[r] = x[r];
               }
             }
-            if (workers_or(over)) {
+            if (team_any(team, over)) {
+              if (!(ok = !team_any(team, !ok))) break;       // a wait of some warp ran out
               // new references: the largest scores of the tile, the largest of V's scales
               float v_top = v_scale;
 #pragma unroll
               for (int d = 1; d < 32; d <<= 1) v_top = fmaxf(v_top, __shfl_xor_sync(0xffffffffu, v_top, d));
-              if (lane == 0) sh.v_top[warp] = v_top;
+              if (lane == 0) sh.v_top[team][warp & 3] = v_top;
 #pragma unroll 1
               for (int c = 0; c < kChunks; ++c) {
                 float x[4];
@@ -394,33 +424,32 @@ __global__ void __launch_bounds__(kThreads, few_ctas(kDim, kRows)) kv8_attention
                 for (int r = 0; r < 4; ++r) {
 #pragma unroll
                   for (int d = 1; d < 32; d <<= 1) x[r] = fmaxf(x[r], __shfl_xor_sync(0xffffffffu, x[r], d));
-                  if (lane == 0) sh.top[warp][4 * c + r] = x[r];
+                  if (lane == 0) sh.top[team][warp & 3][4 * c + r] = x[r];
                 }
               }
-              if (j > 0) ok = bar_wait(&sh.pv_done[(at - 1) & 1], (at - 1) >> 1 & 1, &sh.stalled);
-              if (!(ok = workers_and(ok))) break;
-              fence_after();
-              v_top = fmaxf(fmaxf(fmaxf(sh.v_top[0], sh.v_top[1]), fmaxf(sh.v_top[2], sh.v_top[3])), fmaxf(v_ref, 0x1p-110f));
+              team_sync(team);
+              const float *tops = sh.v_top[team];
+              v_top = fmaxf(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])), fmaxf(v_ref, 0x1p-110f));
               const float v_down = v_ref / v_top;          // powers of two; 0 at the start
               v_ref = v_top;
-              if (tid < kRows) {
-                const float was = sh.ref[tid];
-                const float top = fmaxf(fmaxf(sh.top[0][tid], sh.top[1][tid]), fmaxf(sh.top[2][tid], sh.top[3][tid]));
+              if (own < kRows) {
+                const float was = sh.ref[team][own];
+                const float top = fmaxf(fmaxf(sh.top[team][0][own], sh.top[team][1][own]), fmaxf(sh.top[team][2][own], sh.top[team][3][own]));
                 const float now = top > was + kSlack ? top : was;
-                sh.ref[tid] = now;
-                sh.down[tid] = exp2_fast(was - now);
+                sh.ref[team][own] = now;
+                sh.down[team][own] = exp2_fast(was - now);
               }
-              workers_sync();
+              team_sync(team);
 #pragma unroll
-              for (int r = 0; r < kRows; ++r) sum[r] *= sh.down[r];
-              if (j > 0) {
+              for (int r = 0; r < kRows; ++r) sum[r] *= sh.down[team][r];
+              if (j > 1) {
 #pragma unroll 1
                 for (int c = 0; c < kHalves * kChunks; ++c) {
                   uint32_t y[16];
-                  load16(y, lanes + L::kO + 16 * c);
+                  load16(y, at_o + 16 * c);
 #pragma unroll
-                  for (int k = 0; k < 16; ++k) y[k] = __float_as_uint(__uint_as_float(y[k]) * (sh.down[4 * (c % kChunks) + k % 4] * v_down));
-                  store16(lanes + L::kO + 16 * c, y);
+                  for (int k = 0; k < 16; ++k) y[k] = __float_as_uint(__uint_as_float(y[k]) * (sh.down[team][4 * (c % kChunks) + k % 4] * v_down));
+                  store16(at_o + 16 * c, y);
                 }
                 wait_stores();
               }
@@ -434,7 +463,7 @@ __global__ void __launch_bounds__(kThreads, few_ctas(kDim, kRows)) kv8_attention
               else scores(c, x);
 #pragma unroll
               for (int r = 0; r < 4; ++r) {
-                x[r] = exp2_fast(x[r] - (sh.ref[4 * c + r] - kShift));
+                x[r] = exp2_fast(x[r] - (sh.ref[team][4 * c + r] - kShift));
                 sum[4 * c + r] += x[r];
               }
               uint32_t h[2] = {f16x2(x[0] * on_p, x[1] * on_p), f16x2(x[2] * on_p, x[3] * on_p)}, w[4];
@@ -450,84 +479,97 @@ __global__ void __launch_bounds__(kThreads, few_ctas(kDim, kRows)) kv8_attention
                   h[k] = *reinterpret_cast<const uint32_t *>(&left);
                 }
               }
-              *reinterpret_cast<uint4 *>(smem + L::kP + (at & 1) * L::kPBytes + c * (kTokens * 16) + tid * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+              *reinterpret_cast<uint4 *>(smem + L::kP + team * L::kPBytes + c * (kTokens * 16) + own * 16) = make_uint4(w[0], w[1], w[2], w[3]);
             }
             fence_to_async();
             fence_before();
-            bar_arrive(&sh.p_ready[at & 1]);
+            bar_arrive(&sh.p_ready[team]);
           }
         }
         if constexpr (kWithV) {
-          const uint32_t last = n_tiles + steps - 1;
-          if (steps > 0) ok = ok && bar_wait(&sh.pv_done[last & 1], last >> 1 & 1, &sh.stalled);
-          if ((ok = workers_and(ok))) {
+          if (steps > team) ok = ok && bar_wait_warp(&sh.pv_done[team], (turn - 1) & 1, &sh.stalled);
+          fence_after();
+          // row sums over the threads
+#pragma unroll
+          for (int r = 0; r < kRows; ++r) {
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], d);
+            if (lane == 0) sh.sum[team][warp & 3][r] = sum[r];
+          }
+          if (own == 0) sh.v_ref[team] = v_ref;
+          fence_before();
+          if ((ok = workers_all(ok))) {
             fence_after();
-            // row sums over the threads
-#pragma unroll
-            for (int r = 0; r < kRows; ++r) {
-#pragma unroll
-              for (int d = 1; d < 32; d <<= 1) sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], d);
-              if (lane == 0) sh.sum[warp][r] = sum[r];
-            }
-            workers_sync();
+            // the teams' parts together: team t writes row chunks t, t + 2, ...
             const bool whole = units == (int)seg.units, any_nan = sh.any_nan;
             const int slot = 2 * blockIdx.x + (first_segment ? 0 : 1);
 #pragma unroll 1
-            for (int half = 0; half < kHalves; ++half) {
-              const int d = half * 128 + tid;
-#pragma unroll 1
-              for (int c = 0; c < (live_rows + 3) / 4; ++c) {
-                uint32_t y[16];
-                load16(y, lanes + L::kO + half * kN + 16 * c);
+            for (int i = team; i < kHalves * ((live_rows + 3) / 4); i += 2) {
+              const int half = kHalves == 2 ? i & 1 : 0, c = kHalves == 2 ? i >> 1 : i, d = half * 128 + own;
+              uint32_t y[2][16];
+              load16(y[0], lanes + L::kO + half * kN + 16 * c);
+              load16(y[1], lanes + L::kO + L::kOEach + half * kN + 16 * c);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                  const int r = 4 * c + k;
-                  if (r >= live_rows || d >= kDim) continue;
-                  const float l = sh.sum[0][r] + sh.sum[1][r] + sh.sum[2][r] + sh.sum[3][r];
-                  const float lo = fmaf(__uint_as_float(y[12 + k]), 1.f / 16, __uint_as_float(y[8 + k]));
-                  float a = fmaf(fmaf(lo, 1.f / 16, __uint_as_float(y[4 + k])), 1.f / 16, __uint_as_float(y[k])) * v_ref;
-                  if (steps == 0 || l == 0.f) a = 0.f;
-                  if (any_nan && sh.nan_from[d] < sh.see[r]) a = __int_as_float(0x7fffffff);
-                  const int row = row_first + r, i = row / p.group, qh = head * p.group + row % p.group;
-                  const float base = sh.ref[r] - kShift;
-                  if (whole) {
-                    a = l == 0.f ? a : a / l;
-                    uint16_t *dst = p.out + (int64_t)(seq.row0 + i) * p.out_row + qh * p.out_head + d;
-                    *dst = kBf16 ? __bfloat16_as_ushort(__float2bfloat16_rn(a)) : __half_as_ushort(__float2half_rn(a));
-                    if (d == 0 && p.lse) p.lse[(int64_t)(seq.row0 + i) * p.q_heads + qh] = lse_of(base, l);
-                  } else {
-                    p.part_o[((int64_t)slot * kRows + r) * kDim + d] = a;
-                    if (d == 0) p.part_ml[slot * kRows + r] = make_float2(base, l);
-                  }
+              for (int k = 0; k < 4; ++k) {
+                const int r = 4 * c + k;
+                if (r >= live_rows || d >= kDim) continue;
+                const float base = fmaxf(sh.ref[0][r], sh.ref[1][r]);
+                float a = 0.f, l = 0.f;
+#pragma unroll
+                for (int of = 0; of < 2; ++of) {
+                  if (steps <= of) continue;               // that team had no tile: its O is not written
+                  const float down = exp2_fast(sh.ref[of][r] - base);
+                  const float lo = fmaf(__uint_as_float(y[of][12 + k]), 1.f / 16, __uint_as_float(y[of][8 + k]));
+                  a += fmaf(fmaf(lo, 1.f / 16, __uint_as_float(y[of][4 + k])), 1.f / 16, __uint_as_float(y[of][k])) * sh.v_ref[of] * down;
+                  l += (sh.sum[of][0][r] + sh.sum[of][1][r] + sh.sum[of][2][r] + sh.sum[of][3][r]) * down;
+                }
+                if (l == 0.f) a = 0.f;
+                if (any_nan && sh.nan_from[d] < sh.see[r]) a = __int_as_float(0x7fffffff);
+                const int row = row_first + r, i = row / p.group, qh = head * p.group + row % p.group;
+                if (whole) {
+                  a = l == 0.f ? a : a / l;
+                  uint16_t *dst = p.out + (int64_t)(seq.row0 + i) * p.out_row + qh * p.out_head + d;
+                  *dst = kBf16 ? __bfloat16_as_ushort(__float2bfloat16_rn(a)) : __half_as_ushort(__float2half_rn(a));
+                  if (d == 0 && p.lse) p.lse[(int64_t)(seq.row0 + i) * p.q_heads + qh] = lse_of(base - kShift, l);
+                } else {
+                  p.part_o[((int64_t)slot * kRows + r) * kDim + d] = a;
+                  if (d == 0) p.part_ml[slot * kRows + r] = make_float2(base - kShift, l);
                 }
               }
             }
             fence_before();
-            workers_sync();
             if (any_nan) {
+              workers_all(true);
               for (int i = tid; i < kDim; i += kWorkers) sh.nan_from[i] = INT_MAX;
               if (tid == 0) sh.any_nan = 0;
             }
           }
         }
-        if ((ok = workers_and(ok)) && !kWithV && tiles > 1 && tile + 1 == tiles)
-          for (int j = 0; j < units; ++j) {
-            const int tok = (int)(unit0 + j) * kTokens + tid;
-            if (tok < min(seq.len, p.w_capacity)) p.weights[s * p.w_seq + head * p.w_head + tok] += sh.weight[j][tid];
+        // what the rows of this tile left in shared memory has been read
+        if ((ok = workers_all(ok)) && !kWithV && tiles > 1 && tile + 1 == tiles)
+          for (int j = team; j < units; j += 2) {
+            const int tok = (int)(unit0 + j) * kTokens + own;
+            if (tok < min(seq.len, p.w_capacity)) p.weights[s * p.w_seq + head * p.w_head + tok] += sh.weight[j][own];
           }
       }
       n_tiles += steps;
+      n_of[0] += (steps + 1) >> 1;
+      n_of[1] += steps >> 1;
       n_rows += steps > 0;
     }
     u += units;
     first_segment = false;
   }
+  // The tensor cores' last arrivals, at the slots that are not filled again, come before the block leaves.
+  if (warp == 8 && ok)
+    for (uint32_t i = L::kKv * n_tiles > (uint32_t)kSlots ? L::kKv * n_tiles - kSlots : 0; i < L::kKv * n_tiles && ok; ++i)
+      ok = bar_wait_warp(&sh.empty[i % kSlots], i / kSlots & 1, &sh.stalled);
   __syncwarp();
   fence_before();
   __syncthreads();
   fence_after();
   if (sh.stalled && tid == 0) p.batch.report(PF_KV8_STALLED);
-  if (warp == 5) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(L::kAlloc));
+  if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(L::kAlloc));
 }
 
 // The cache as [K or V][block][head][row][byte], tiles of 16 rows of (half) a head.
@@ -556,7 +598,7 @@ template <int kDim, int kRows, bool kWithV, bool kBf16>
 void launch(const AttnParams &p, int n_ctas, cudaStream_t stream) {
   using L = Few<kDim, kRows, kWithV>;
   auto kernel = kv8_attention_few<kDim, kRows, kWithV, kBf16>;
-  const size_t smem = 1024 + (size_t)L::kEnd + sizeof(FewShared<kDim, kRows, L::kStages, kWithV>) +
+  const size_t smem = 1024 + (size_t)L::kEnd + sizeof(FewShared<kDim, kRows, L::kSlots, kWithV>) +
                       Work<kRows, kTokens, !kWithV>::bytes(p.batch.n_seqs, p.row_tiles_most);
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
     throw Error::storage("cudaFuncSetAttribute failed");
@@ -569,13 +611,14 @@ void launch(const AttnParams &p, int rows, cudaStream_t stream) {
     case 4: return launch<kDim, 4, true, kBf16>(p, p.n_ctas, stream);
     case 8: return launch<kDim, 8, true, kBf16>(p, p.n_ctas, stream);
     case 16: return launch<kDim, 16, true, kBf16>(p, p.n_ctas, stream);
-    default: return launch<kDim, 32, true, kBf16>(p, p.n_ctas, stream);
+    default:
+      if constexpr (kDim != 256) launch<kDim, 32, true, kBf16>(p, p.n_ctas, stream);
   }
 }
 
 }  // namespace
 
-int kv8_few_rows(int64_t rows) { return rows <= 4 ? 4 : rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 32 ? 32 : 0; }
+int kv8_few_rows(int dim, int64_t rows) { return rows <= 4 ? 4 : rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 32 && dim != 256 ? 32 : 0; }
 int kv8_few_ctas(int dim, int rows) { return few_ctas(dim, rows); }
 
 void kv8_few_launch(const AttnParams &p, int rows, bool bf16, cudaStream_t stream) {
