@@ -248,6 +248,7 @@ int pf_kv8_attention(int device_id, const pf_kv8_cache *cache, const pf_kv8_batc
     p.vec_out = (uintptr_t)a.out % 8 == 0 && (a.out_row_stride | a.out_head_stride) % 4 == 0;
     p.scale = a.scale;
     p.n_ctas = plan.n_ctas;
+    p.device = device_id;
     DeviceGuard on_device(device_id);
     if (a.dtype == PF_KV8_BF16) launch<true>(p, plan, kv8_sm_count(device_id), (cudaStream_t)stream);
     else launch<false>(p, plan, kv8_sm_count(device_id), (cudaStream_t)stream);

@@ -3,6 +3,8 @@
 
 #include <cuda_fp16.h>
 
+#include <atomic>
+
 #include "kv8.h"
 
 namespace pf {
@@ -27,17 +29,23 @@ struct AttnParams {
   // part_ml holds (base, sum): the row's sum and its part_o are of terms 2^(score - base), scores in base 2.
   float *part_o;    // [slots][rows][dim]
   float2 *part_ml;  // [slots][rows]
-  int n_ctas;
+  int n_ctas, device;
 };
 
-// The work of all sequences, heads and row tiles laid end to end in units of some tokens; CTA c of n takes
-// [total c / n, total (c + 1) / n).  A segment is one (sequence, head, row tile).
+// The work of all sequences, heads and row tiles laid end to end in units of some tokens, in equal ranges for n CTAs (the first
+// ones one unit longer).  A segment is one (sequence, head, row tile).
 struct Split {
-  uint32_t total;
-  int n_ctas;       // at most total: every CTA that takes part has work
-  __device__ Split(uint32_t total, int n) : total(total), n_ctas((int)min((uint32_t)n, total)) {}
-  __device__ uint32_t begin(int c) const { return (uint32_t)((uint64_t)total * c / n_ctas); }
-  __device__ int owner(uint32_t u) const { return (int)((((uint64_t)u + 1) * n_ctas - 1) / total); }
+  uint32_t each, longer;   // units of a range; how many ranges have one more
+  int n_ctas;              // at most the units: every CTA that takes part has work
+  __device__ Split(uint32_t total, int n) : n_ctas((int)min((uint32_t)n, total)) {
+    each = n_ctas ? total / n_ctas : 0;
+    longer = total - each * n_ctas;
+  }
+  __device__ uint32_t begin(int c) const { return each * c + min((uint32_t)c, longer); }
+  __device__ int owner(uint32_t u) const {
+    const uint32_t in_longer = longer * (each + 1);
+    return (int)(u < in_longer ? u / (each + 1) : longer + (u - in_longer) / each);
+  }
 };
 
 // One sequence of a call: its rows (row = query * group + head of the group) in tiles of kRows, and its tokens.  kWhole:
@@ -50,11 +58,11 @@ struct Seq {
     p.batch.rows(s, row0, hi);
     rows = min(hi - row0, p.max_query);
     len = p.batch.length(s, p.cache.block_log2);
-    row_tiles = kWhole ? min(rows, 1) : (rows * p.group + kRows - 1) / kRows;
+    row_tiles = kWhole ? min(rows, 1) : (rows * p.group + kRows - 1) / kRows;     // kRows is a power of two
   }
   __device__ int all_rows(const AttnParams &p) const { return rows * p.group; }
   __device__ int visible(const AttnParams &p, int row) const {   // tokens that query row `row` sees
-    return p.causal ? min(max(len - rows + row / p.group + 1, 0), len) : len;
+    return p.causal && rows > 1 ? min(max(len - rows + row / p.group + 1, 0), len) : len;     // of one query: all
   }
   // Units of one row tile: those that its last row sees, one at least.
   __device__ uint32_t units(const AttnParams &p, int rt) const {
@@ -76,10 +84,11 @@ struct Work {
     const int entries = n_seqs * row_tiles_most, chunk = chunk_of(entries);
     return ((size_t)(entries + chunk - 1) / chunk + 1) * 4;
   }
-  __device__ uint32_t units_of(const AttnParams &p, int e) const {
-    const SeqT seq(p, e / p.row_tiles_most);
-    const int rt = e % p.row_tiles_most;
-    return rt < seq.row_tiles ? seq.units(p, rt) * (uint32_t)p.cache.heads : 0u;
+  static __device__ int seq_of(const AttnParams &p, int e) { return p.row_tiles_most == 1 ? e : e / p.row_tiles_most; }
+  __device__ uint32_t units_of(const AttnParams &p, int e) const {       // of one head
+    const int s = seq_of(p, e), rt = e - s * p.row_tiles_most;
+    const SeqT seq(p, s);
+    return rt < seq.row_tiles ? seq.units(p, rt) : 0u;
   }
   __device__ Work(const AttnParams &p, uint32_t *prefix) : prefix(prefix) {
     __shared__ uint32_t warp_sum[32];
@@ -91,7 +100,7 @@ struct Work {
     for (int c0 = 0; c0 < chunks; c0 += blockDim.x) {
       const int c = c0 + threadIdx.x;
       uint32_t mine = 0;
-      for (int e = c * chunk; c < chunks && e < min((c + 1) * chunk, entries); ++e) mine += units_of(p, e);
+      for (int e = c * chunk; c < chunks && e < min((c + 1) * chunk, entries); ++e) mine += units_of(p, e) * (uint32_t)p.cache.heads;
       uint32_t x = mine;
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) {
@@ -129,14 +138,13 @@ struct Segment {
     }
     int e = lo * work.chunk;
     begin = work.prefix[lo];
-    uint32_t all = work.units_of(p, e);
-    while (u - begin >= all) {
-      begin += all;
-      all = work.units_of(p, ++e);
+    units = work.units_of(p, e);
+    while (u - begin >= units * (uint32_t)p.cache.heads) {
+      begin += units * (uint32_t)p.cache.heads;
+      units = work.units_of(p, ++e);
     }
-    s = e / p.row_tiles_most;
-    rt = e % p.row_tiles_most;
-    units = all / (uint32_t)p.cache.heads;
+    s = work.seq_of(p, e);
+    rt = e - s * p.row_tiles_most;
     head = (int)((u - begin) / units);
     begin += head * units;
   }
@@ -172,6 +180,16 @@ __device__ __forceinline__ void check_batch(const AttnParams &p) {
 }
 
 __device__ __forceinline__ float lse_of(float base, float sum) { return sum == 0.f ? -INFINITY : (base + log2f(sum)) * kLn2; }
+
+// Lets a kernel have all of the shared memory; asked of the driver once for each device.
+template <class Kernel>
+void allow_smem(Kernel kernel, std::atomic<uint64_t> &asked, int device) {
+  const uint64_t bit = 1ull << (device & 63);
+  if (device < 64 && (asked.load(std::memory_order_relaxed) & bit)) return;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 - 1024) != cudaSuccess)
+    throw Error::storage("cudaFuncSetAttribute failed");
+  if (device < 64) asked.fetch_or(bit, std::memory_order_relaxed);
+}
 
 // Few query rows (kv8_attention_few.cu): tiles of 4, 8, 16 or (not at 256 dimensions) 32
 // rows, 0 when there are more.  And the accumulated weights.

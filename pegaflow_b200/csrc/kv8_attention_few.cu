@@ -69,7 +69,7 @@ struct FewShared {
   uint64_t full[kSlots], empty[kSlots], q_ready, s_full[2], p_ready[2], pv_done[2];
   uint32_t tmem;
   int stalled, any_nan;
-  float factor[kRows], base[kRows];
+  float factor[kRows], base[kRows], row_top[8];
   float ref[2][kRows], down[2][kRows], top[2][4][kRows], sum[2][4][kRows], v_top[2][4], v_ref[2];
   int see[kRows];
   int nan_from[kDim];
@@ -85,6 +85,35 @@ __device__ __forceinline__ int place(int r, int c, int panel_rows) {
 
 template <int kDim>
 constexpr __host__ __device__ uint32_t swizzle_of() { return kDim == 64 ? kSwizzle64 : kSwizzle128; }
+
+__device__ __forceinline__ float warp_max(float x) {      // leaves NaN out
+  float y;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
+  return y;
+}
+// Sums of v[r] over the warp, for all kRows rows: each step halves the rows that a lane holds, or, once it holds one, the lanes.
+// Lane 0, 32 / kRows, ... hold a row each, which is returned; the others' is meaningless.
+template <int kRows>
+__device__ __forceinline__ float warp_sums(float (&v)[kRows], int &row) {
+  const int lane = threadIdx.x & 31;
+  row = 0;
+#pragma unroll
+  for (int m = 16, n = kRows; m > 0; m >>= 1) {
+    if (n > 1) {
+      n /= 2;
+#pragma unroll
+      for (int r = 0; r < kRows / 2; ++r)
+        if (r < n) {
+          const float send = lane & m ? v[r] : v[r + n], keep = lane & m ? v[r + n] : v[r];
+          v[r] = keep + __shfl_xor_sync(0xffffffffu, send, m);
+        }
+      row += lane & m ? n : 0;
+    } else {
+      v[0] += __shfl_xor_sync(0xffffffffu, v[0], m);
+    }
+  }
+  return v[0];
+}
 
 // Barriers of a team (ids 1 and 2) and of both (3); whole warps come to them.
 __device__ __forceinline__ void team_sync(int team) {
@@ -268,53 +297,48 @@ __global__ void __launch_bounds__(kThreads, few_ctas(kDim, kRows)) kv8_attention
         const int team = warp >> 2, own = tid % kTeam;       // the token of a tile, and the dimension, that are this thread's
         const uint32_t lanes = tmem + ((uint32_t)(warp & 3) * 32 << 16), at_o = lanes + L::kO + team * L::kOEach;
         // the rows' pieces, factors and lengths
-        constexpr int kLanes = kDim / 16;
-        for (int e = tid; e < kRows * kLanes; e += kWorkers) {
-          const int r = e / kLanes, c = e % kLanes, row = row_first + r;
+        constexpr int kLanes = kDim / 16, kFours = kDim / 4;       // 16-byte chunks of a row of bytes; threads of a row of q
+        for (int e = tid; e < kRows * kFours; e += kWorkers) {     // whole warps: a row is 16 lanes, or a warp or two
+          const int r = e / kFours, c = e % kFours, row = row_first + r;
           const bool live = r < live_rows;
-          const int i = live ? row / p.group : 0, qh = head * p.group + (live ? row % p.group : 0);
-          const uint16_t *src = p.q + (int64_t)(seq.row0 + i) * p.q_row + qh * p.q_head + 16 * c;
-          float x[16], top = 0.f;
-#pragma unroll
-          for (int k = 0; k < 16; k += 8) {
-            uint4 w = make_uint4(0, 0, 0, 0);
-            if (live) {
-              if (p.vec_q) w = *reinterpret_cast<const uint4 *>(src + k);
-              else {
-                const uint16_t *at = src + k;
-                w = make_uint4(at[0] | at[1] << 16, at[2] | at[3] << 16, at[4] | at[5] << 16, at[6] | at[7] << 16);
-              }
-            }
-            const uint32_t y[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-            for (int m = 0; m < 4; ++m) {
-              const float2 f = kBf16 ? make_float2(__uint_as_float(y[m] << 16), __uint_as_float(y[m] & 0xffff0000u)) : f32x2_from_f16x2(y[m]);
-              x[k + 2 * m] = f.x, x[k + 2 * m + 1] = f.y;
-              top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
-            }
+          const int i = live ? row / p.group : 0, qh = head * p.group + (live ? row - i * p.group : 0);
+          const uint16_t *src = p.q + (int64_t)(seq.row0 + i) * p.q_row + qh * p.q_head + 4 * c;
+          uint2 y = make_uint2(0, 0);
+          if (live) {
+            if (p.vec_q) y = *reinterpret_cast<const uint2 *>(src);
+            else y = make_uint2(src[0] | src[1] << 16, src[2] | src[3] << 16);
           }
+          float x[4];
+          const float2 lo2 = kBf16 ? make_float2(__uint_as_float(y.x << 16), __uint_as_float(y.x & 0xffff0000u)) : f32x2_from_f16x2(y.x);
+          const float2 hi2 = kBf16 ? make_float2(__uint_as_float(y.y << 16), __uint_as_float(y.y & 0xffff0000u)) : f32x2_from_f16x2(y.y);
+          x[0] = lo2.x, x[1] = lo2.y, x[2] = hi2.x, x[3] = hi2.y;
+          float top = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
+          if (kDim == 64) {
 #pragma unroll
-          for (int d = 1; d < kLanes; d <<= 1) top = fmaxf(top, __shfl_xor_sync(__activemask(), top, d));
+            for (int d = 1; d < 16; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+          } else {
+            top = warp_max(top);
+          }
+          if (kDim == 256) {                 // the row's other warp is this warp's neighbour
+            if (lane == 0) sh.row_top[warp] = top;
+            if (!workers_all(true)) break;
+            top = fmaxf(top, sh.row_top[warp ^ 1]);
+            if (!workers_all(true)) break;   // and has read it
+          }
           int ex = (int)(__float_as_uint(top) >> 23) - 127 - 7;
           if (top == 0.f || top > 3.4e38f) ex = 0;
           ex = max(ex, -126);
           const float down = exp2i(-ex);
           // an infinity would become 448
 #pragma unroll
-          for (int k = 0; k < 16; ++k) x[k] = fabsf(x[k]) > 3.4e38f ? __int_as_float(0x7fffffff) : x[k] * down;
+          for (int k = 0; k < 4; ++k) x[k] = fabsf(x[k]) > 3.4e38f ? __int_as_float(0x7fffffff) : x[k] * down;
 #pragma unroll
           for (int piece = 0; piece < 4; ++piece) {
-            uint32_t w[4];
-#pragma unroll
-            for (int k = 0; k < 16; k += 4) {
-              const uint32_t lo = e4m3x2(x[k], x[k + 1]), hi = e4m3x2(x[k + 2], x[k + 3]);
-              w[k / 4] = lo | hi << 16;
-              const float2 a = f32x2_from_f16x2(f16x2_from_e4m3<0>(lo)), b = f32x2_from_f16x2(f16x2_from_e4m3<0>(hi));
-              x[k] = (x[k] - a.x) * 16.f, x[k + 1] = (x[k + 1] - a.y) * 16.f;
-              x[k + 2] = (x[k + 2] - b.x) * 16.f, x[k + 3] = (x[k + 3] - b.y) * 16.f;
-            }
+            const uint32_t lo = e4m3x2(x[0], x[1]), hi = e4m3x2(x[2], x[3]);
             const int n = 16 * (r / 4) + 4 * piece + r % 4;
-            *reinterpret_cast<uint4 *>(smem + L::kQ + place<kDim>(n, c, kN)) = make_uint4(w[0], w[1], w[2], w[3]);
+            *reinterpret_cast<uint32_t *>(smem + L::kQ + place<kDim>(n, c / 4, kN) + 4 * (c % 4)) = lo | hi << 16;
+            const float2 a = f32x2_from_f16x2(f16x2_from_e4m3<0>(lo)), b = f32x2_from_f16x2(f16x2_from_e4m3<0>(hi));
+            x[0] = (x[0] - a.x) * 16.f, x[1] = (x[1] - a.y) * 16.f, x[2] = (x[2] - b.x) * 16.f, x[3] = (x[3] - b.y) * 16.f;
           }
           if (c == 0) {
             sh.factor[r] = p.scale * kLog2e * exp2i(ex);
@@ -412,9 +436,7 @@ __global__ void __launch_bounds__(kThreads, few_ctas(kDim, kRows)) kv8_attention
             if (team_any(team, over)) {
               if (!(ok = !team_any(team, !ok))) break;       // a wait of some warp ran out
               // new references: the largest scores of the tile, the largest of V's scales
-              float v_top = v_scale;
-#pragma unroll
-              for (int d = 1; d < 32; d <<= 1) v_top = fmaxf(v_top, __shfl_xor_sync(0xffffffffu, v_top, d));
+              float v_top = warp_max(v_scale);
               if (lane == 0) sh.v_top[team][warp & 3] = v_top;
 #pragma unroll 1
               for (int c = 0; c < kChunks; ++c) {
@@ -422,8 +444,7 @@ __global__ void __launch_bounds__(kThreads, few_ctas(kDim, kRows)) kv8_attention
                 scores(c, x);
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-#pragma unroll
-                  for (int d = 1; d < 32; d <<= 1) x[r] = fmaxf(x[r], __shfl_xor_sync(0xffffffffu, x[r], d));
+                  x[r] = warp_max(x[r]);
                   if (lane == 0) sh.top[team][warp & 3][4 * c + r] = x[r];
                 }
               }
@@ -490,12 +511,9 @@ __global__ void __launch_bounds__(kThreads, few_ctas(kDim, kRows)) kv8_attention
           if (steps > team) ok = ok && bar_wait_warp(&sh.pv_done[team], (turn - 1) & 1, &sh.stalled);
           fence_after();
           // row sums over the threads
-#pragma unroll
-          for (int r = 0; r < kRows; ++r) {
-#pragma unroll
-            for (int d = 1; d < 32; d <<= 1) sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], d);
-            if (lane == 0) sh.sum[team][warp & 3][r] = sum[r];
-          }
+          int row_of;
+          const float row_sum = warp_sums<kRows>(sum, row_of);
+          if (lane % (32 / kRows) == 0) sh.sum[team][warp & 3][row_of] = row_sum;
           if (own == 0) sh.v_ref[team] = v_ref;
           fence_before();
           if ((ok = workers_all(ok))) {
@@ -600,8 +618,8 @@ void launch(const AttnParams &p, int n_ctas, cudaStream_t stream) {
   auto kernel = kv8_attention_few<kDim, kRows, kWithV, kBf16>;
   const size_t smem = 1024 + (size_t)L::kEnd + sizeof(FewShared<kDim, kRows, L::kSlots, kWithV>) +
                       Work<kRows, kTokens, !kWithV>::bytes(p.batch.n_seqs, p.row_tiles_most);
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
-    throw Error::storage("cudaFuncSetAttribute failed");
+  static std::atomic<uint64_t> asked;
+  allow_smem(kernel, asked, p.device);
   launch_after(kernel, n_ctas, kThreads, smem, stream, p, map_of(p.cache));
 }
 

@@ -469,8 +469,8 @@ template <int kDim, bool kBf16>
 void launch(const AttnParams &p, cudaStream_t stream) {
   auto kernel = kv8_attention_wide<kDim, kBf16>;
   const size_t smem = kv8_wide_plan(kDim).smem + Work<kGroupRows * groups_of(kDim), tokens_of(kDim)>::bytes(p.batch.n_seqs, p.row_tiles_most);
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
-    throw Error::storage("cudaFuncSetAttribute failed");
+  static std::atomic<uint64_t> asked;
+  allow_smem(kernel, asked, p.device);
   launch_after(kernel, p.n_ctas, threads_of(kDim), smem, stream, p);
 }
 

@@ -23,6 +23,8 @@ from . import _native as N
 _DTYPES = {torch.bfloat16: N.KV8_BF16, torch.float16: N.KV8_F16}
 _INT32, _FLOAT32 = torch.int32, torch.float32
 _byref = C.byref
+# handle of a device's current stream; torch's own shortcut where there is one, a tenth of the object's cost
+_stream_of = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 _append, _attention, _attention_workspace, _evict = (N.lib.pf_kv8_append, N.lib.pf_kv8_attention,
                                                      N.lib.pf_kv8_attention_workspace, N.lib.pf_kv8_evict)
 
@@ -153,7 +155,7 @@ class Kv8Cache:
             _refuse(f"k ({k.dtype} {tuple(k.shape)}) and v ({v.dtype} {tuple(v.shape)}) differ")
         batch = self._batch(block_tables, lens, starts)
         if stream is None:
-            stream = torch.cuda.current_stream(self.device).cuda_stream
+            stream = _stream_of(self._index)
         N.check(_append(self._index, self._desc_ref, _byref(batch), k.data_ptr(), v.data_ptr(), code, k.shape[0], ks[0], ks[1],
                         vs[0], vs[1], stream))
 
@@ -211,7 +213,7 @@ class Kv8Cache:
             need = self._workspaces[sizes] = size.value
         space = torch.empty(need, dtype=torch.uint8, device=self.device)
         N.check(_attention(self._index, self._desc_ref, _byref(batch), _byref(args), space.data_ptr(), need,
-                           torch.cuda.current_stream(self.device).cuda_stream))
+                           _stream_of(self._index)))
         return (out, lse_out) if lse else out
 
     def evict(self, block_tables, lens, weights, dst_tables, keep: int, *, recent: int = 0,
@@ -244,5 +246,5 @@ class Kv8Cache:
         args = N.Kv8EvictArgs(weights.data_ptr(), ws[0], ws[1], tokens, dst_ptr, dst_tables.stride(0), keep, recent,
                               new_lens.data_ptr(), new_weights.data_ptr(), capacity, kept.data_ptr())
         N.check(_evict(self._index, self._desc_ref, _byref(batch), _byref(args),
-                       torch.cuda.current_stream(self.device).cuda_stream))
+                       _stream_of(self._index)))
         return new_lens, new_weights, kept
