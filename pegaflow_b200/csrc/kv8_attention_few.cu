@@ -636,7 +636,12 @@ void launch(const AttnParams &p, int rows, cudaStream_t stream) {
 
 }  // namespace
 
-int kv8_few_rows(int dim, int64_t rows) { return rows <= 4 ? 4 : rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 32 && dim != 256 ? 32 : 0; }
+// Up to 64 rows go in tiles of up to 32 (at 256 dimensions 16), K and V read once for each: at 16 requests of 4000 tokens, 4
+// KV heads of 128, 64 rows take 90 us here and 119 us in the form for many rows; 96 rows 138 us and 124 us.
+int kv8_few_rows(int dim, int64_t rows) {
+  if (rows <= 16) return rows <= 4 ? 4 : rows <= 8 ? 8 : 16;
+  return rows <= 64 ? (dim == 256 ? 16 : 32) : 0;
+}
 int kv8_few_ctas(int dim, int rows) { return few_ctas(dim, rows); }
 
 void kv8_few_launch(const AttnParams &p, int rows, bool bf16, cudaStream_t stream) {
