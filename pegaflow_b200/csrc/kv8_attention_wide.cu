@@ -32,7 +32,7 @@ constexpr int kRing = 4;                      // steps of scales kept
 
 constexpr int tokens_of(int dim) { return dim == 256 ? 64 : 128; }
 constexpr int groups_of(int dim) { return dim == 256 ? 1 : 2; }
-constexpr int threads_of(int dim) { return 128 * groups_of(dim) + 128 + 32; }
+constexpr int threads_of(int dim) { return 128 * groups_of(dim) + 128 + 128; }   // whole warpgroups; the last one has the issuer
 
 // Offsets in shared memory, behind the first 1024-byte boundary.
 template <int kDim>
@@ -101,14 +101,36 @@ __global__ void __launch_bounds__(threads_of(kDim), 1) kv8_attention_wide(AttnPa
   uint32_t step = 0;          // steps done in earlier segments: all roles count alike
   uint32_t n_segment = 0;
   bool ok = true;
-  while (u < u_end && ok) {
-    const Segment seg(p, work, u);
-    const int s = seg.s;
-    const SeqT seq(p, s);
-    const uint32_t unit0 = u - seg.begin, units = min(seg.units - unit0, u_end - u);
-    const int row_first = seg.rt * kRows, live_rows = min(seq.all_rows(p) - row_first, kRows);
-    const int head = seg.head;
-    if (warp < kConvert) {
+  // Every role walks the CTA's segments by itself; behind each all threads meet.
+  auto walk = [&](auto &&role) {
+    while (u < u_end && ok) {
+      const Segment seg(p, work, u);
+      const uint32_t unit0 = u - seg.begin, units = min(seg.units - unit0, u_end - u);
+      const SeqT seq(p, seg.s);
+      const int row_first = seg.rt * kRows;
+      role(seg, seq, unit0, units, row_first, min(seq.all_rows(p) - row_first, kRows));
+      step += units;
+      ++n_segment;
+      u += units;
+      first_segment = false;
+      __syncwarp();
+      // every thread is through with this segment's marks before the next one sets them
+      if (u < u_end) {
+        if (__syncthreads_or(sh.stalled)) break;
+        if (sh.any_nan) {
+          __syncthreads();
+          for (int k = tid; k < kDim; k += blockDim.x) sh.nan_from[k] = INT_MAX;
+          if (tid == 0) sh.any_nan = 0;
+        }
+        __syncthreads();
+      }
+    }
+  };
+  // Two groups: 512 threads start with 128 registers each, and 256 x 184 + 128 x 104 + 128 x 40 are as many.
+  if (warp < kConvert) {
+    if (kGroups == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+    walk([&](const Segment &seg, const SeqT &seq, uint32_t unit0, uint32_t units, int row_first, int live_rows) {
+      const int head = seg.head;
       // ------------------------------------------------------------------ softmax: a thread holds a row
       const int g = warp >> 2, r = (warp & 3) * 32 + lane;
       const int row = row_first + g * kGroupRows + r;
@@ -172,35 +194,32 @@ __global__ void __launch_bounds__(threads_of(kDim), 1) kv8_attention_wide(AttnPa
         if (!(ok = bar_wait_warp(&sh.s_full[g], at & 1, &sh.stalled))) break;
         fence_after();
         if (!dead) {
-          float f[kBlocks];
-          int ve[kBlocks], e_top = kKv8MinExp;
-          bool hidden = tok + kTokens > group_least;
+          uint32_t x[kTokens];
+          load_all(x, s_col);
+          const float *ks = sh.k_scale[ring];
+          const int *ve = sh.v_exp[ring];
+          // Rows that do not see the tile whole, blocks that are not there: -infinity, before anything else.  The factors below
+          // are positive, so that it stays that.
+          int e_top = kKv8MinExp, gone = 0;
 #pragma unroll
           for (int b = 0; b < kBlocks; ++b) {
-            f[b] = factor * sh.k_scale[ring][b];
-            ve[b] = sh.v_exp[ring][b];
-            if (ve[b] == kHidden) hidden = true;
+            if (ve[b] == kHidden) gone |= 1 << b;
             else e_top = max(e_top, ve[b]);
           }
-          // largest score that the row sees
+          if (tok + kTokens > group_least || gone) {
+            const int n = see - tok;
+#pragma unroll
+            for (int k = 0; k < kTokens; ++k)
+              if (k >= n || (gone >> (k / 16) & 1)) x[k] = 0xff800000u;
+          }
+          auto factor_of = [&](int b) { return fmaxf(factor * ks[b], 1e-37f); };
           float top = kNone;
 #pragma unroll
-          for (int c = 0; c < kTokens / 32; ++c) {
-            uint32_t x[32];
-            load32(x, s_col + 32 * c);
-            if (!hidden) {
+          for (int b = 0; b < kBlocks; ++b) {
+            float m = __uint_as_float(x[16 * b]);
 #pragma unroll
-              for (int b = 0; b < 2; ++b) {
-                float m = __uint_as_float(x[16 * b]);
-#pragma unroll
-                for (int k = 1; k < 16; ++k) m = fmaxf(m, __uint_as_float(x[16 * b + k]));
-                top = fmaxf(top, m * f[2 * c + b]);
-              }
-            } else {
-#pragma unroll
-              for (int k = 0; k < 32; ++k)
-                if (tok + 32 * c + k < see && ve[2 * c + k / 16] != kHidden) top = fmaxf(top, __uint_as_float(x[k]) * f[2 * c + k / 16]);
-            }
+            for (int k = 1; k < 15; k += 2) m = fmaxf(fmaxf(m, __uint_as_float(x[16 * b + k])), __uint_as_float(x[16 * b + k + 1]));
+            top = fmaxf(top, fmaxf(m, __uint_as_float(x[16 * b + 15])) * factor_of(b));
           }
           // both references, and O with them
           const bool start = j == 0;
@@ -218,44 +237,39 @@ __global__ void __launch_bounds__(threads_of(kDim), 1) kv8_attention_wide(AttnPa
             e_ref = e_top;
           }
           if (__any_sync(0xffffffffu, change)) {
-            for (int c = 0; c < kDim / 32; ++c) {
-              uint32_t x[32];
-              load32(x, o_col + 32 * c);
-  #pragma unroll
-              for (int k = 0; k < 32; ++k) x[k] = __float_as_uint(__uint_as_float(x[k]) * down);
-              store32(o_col + 32 * c, x);
+#pragma unroll 1
+            for (int c = 0; c < kDim / 16; ++c) {
+              uint32_t y[16];
+              load16(y, o_col + 16 * c);
+#pragma unroll
+              for (int k = 0; k < 16; ++k) y[k] = __float_as_uint(__uint_as_float(y[k]) * down);
+              store16(o_col + 16 * c, y);
             }
           }
 #pragma unroll
+          for (int b = 0; b < kBlocks; ++b) {
+            // 2^-60 of the largest scale leaves nothing of P in f16; the row sum still has it
+            const int de = gone >> b & 1 ? 0 : max(ve[b] - e_ref, -60);
+            const float fb = factor_of(b), minus = kShift + (float)de - ref;
+            const uint64_t fb2 = pair(fb, fb), minus2 = pair(minus, minus);
+            uint64_t part = pair(0.f, 0.f);
+#pragma unroll
+            for (int k = 0; k < 16; k += 2) {
+              float lo, hi;
+              unpair(fma2(pair(__uint_as_float(x[16 * b + k]), __uint_as_float(x[16 * b + k + 1])), fb2, minus2), lo, hi);
+              lo = exp2_fast(lo), hi = exp2_fast(hi);
+              part = add2(part, pair(lo, hi));
+              x[8 * b + k / 2] = f16x2(lo, hi);
+            }
+            float lo, hi;
+            unpair(part, lo, hi);
+            sum = fmaf(lo + hi, exp2i(-de), sum);
+          }
+#pragma unroll
           for (int c = 0; c < kTokens / 32; ++c) {
-            uint32_t x[32], h[16];
-            load32(x, s_col + 32 * c);
-            uint32_t seen = 0xffffffffu;
-            if (hidden) {
-              const int n = see - (tok + 32 * c);
-              seen = n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1;
-              if (ve[2 * c] == kHidden) seen &= 0xffff0000u;
-              if (ve[2 * c + 1] == kHidden) seen &= 0x0000ffffu;
-            }
+            uint32_t h[16];
 #pragma unroll
-            for (int b = 0; b < 2; ++b) {
-              const int de = ve[2 * c + b] == kHidden ? 0 : ve[2 * c + b] - e_ref;
-              // so far below e_ref, P would leave fp32's range and the row sum with it: the factor then goes on afterwards
-              const bool far = de < -60;
-              const float fb = f[2 * c + b], minus = kShift + (far ? 0.f : (float)de) - ref;
-              float part = 0.f;
-              auto entry = [&](int k) {
-                const float y = fmaf(__uint_as_float(x[16 * b + k]), fb, minus);
-                return exp2_fast(!hidden || (seen >> (16 * b + k) & 1) ? y : -INFINITY);
-              };
-#pragma unroll
-              for (int k = 0; k < 16; k += 2) {
-                const float a = entry(k), d = entry(k + 1);
-                part += a + d;
-                h[8 * b + k / 2] = far ? f16x2(a * exp2i(de), d * exp2i(de)) : f16x2(a, d);
-              }
-              sum = fmaf(part, far ? 1.f : exp2i(-de), sum);
-            }
+            for (int k = 0; k < 16; ++k) h[k] = x[16 * c + k];
             store16(s_col + 16 * c, h);
           }
           wait_stores();
@@ -321,19 +335,31 @@ __global__ void __launch_bounds__(threads_of(kDim), 1) kv8_attention_wide(AttnPa
         }
         fence_before();
       }
-    } else if (warp < kIssue) {
+    });
+  } else if (warp < kIssue) {
+    if (kGroups == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+    walk([&](const Segment &seg, const SeqT &seq, uint32_t unit0, uint32_t units, int, int) {
+      const int s = seg.s, head = seg.head;
       // ------------------------------------------------------------------ converters
       constexpr int kLanes = kDim / 16, kVecs = kTokens * kLanes / 128;      // lanes of a row, 16-byte vectors of a thread
       const int ct = tid - kConvert * 32, sub = ct % kLanes, row_of = ct / kLanes;
       const int within = p.cache.block_size() - 1, tok_stop = seq.len;
-      auto fetch = [&](int kv, uint32_t j, uint4 (&x)[kVecs]) {
+      const int32_t *table = p.batch.tables + s * p.batch.table_stride;
+      const char *tile_of[2] = {p.cache.base + head * p.cache.tile_bytes() + 16 * sub, p.cache.base + p.cache.kv_stride + head * p.cache.tile_bytes() + 16 * sub};
+      auto look_up = [&](uint32_t j, uint32_t (&id)[kVecs]) {
 #pragma unroll
         for (int v = 0; v < kVecs; ++v) {
           const int tok = (int)((unit0 + j) * kTokens) + v * (128 / kLanes) + row_of;
-          uint32_t id;
+          id[v] = j < units && tok < tok_stop ? (uint32_t)table[tok >> p.cache.block_log2] : 0xffffffffu;
+        }
+      };
+      auto fetch = [&](int kv, uint32_t j, const uint32_t (&id)[kVecs], uint4 (&x)[kVecs]) {
+#pragma unroll
+        for (int v = 0; v < kVecs; ++v) {
+          const int tok = (int)((unit0 + j) * kTokens) + v * (128 / kLanes) + row_of;
           x[v] = make_uint4(0, 0, 0, 0);
-          if (tok < tok_stop && p.batch.block(p.cache, s, tok >> p.cache.block_log2, id))
-            x[v] = __ldg(reinterpret_cast<const uint4 *>(p.cache.tile(kv, id, head) + (tok & within) * kDim + 16 * sub));
+          if (id[v] < p.cache.num_blocks)
+            x[v] = __ldg(reinterpret_cast<const uint4 *>(tile_of[kv] + (uint64_t)id[v] * (uint32_t)p.cache.block_stride + (tok & within) * kDim));
         }
       };
       auto lay = [&](char *base, const uint4 (&x)[kVecs]) {
@@ -350,11 +376,15 @@ __global__ void __launch_bounds__(threads_of(kDim), 1) kv8_attention_wide(AttnPa
         }
         fence_to_async();
       };
+      // pages a tile ahead of K, which is a tile ahead of V
       uint4 kx[kVecs], vx[kVecs];
-      fetch(0, 0, kx);
+      uint32_t id[kVecs], next[kVecs];
+      look_up(0, id);
+      look_up(1, next);
+      fetch(0, 0, id, kx);
       for (uint32_t j = 0; j < units; ++j) {
         const uint32_t at = step + j, stage = at & 1;
-        fetch(1, j, vx);
+        fetch(1, j, id, vx);
         if (!(ok = bar_wait(&sh.k_empty[stage], (at >> 1 & 1) ^ 1, &sh.stalled))) break;
         if (ct < kBlocks) {
           const int tok = (int)((unit0 + j) * kTokens) + 16 * ct;
@@ -375,7 +405,10 @@ __global__ void __launch_bounds__(threads_of(kDim), 1) kv8_attention_wide(AttnPa
         }
         lay(smem + L::k + stage * L::kv_bytes, kx);
         bar_arrive(&sh.k_full[stage]);
-        if (j + 1 < units) fetch(0, j + 1, kx);
+#pragma unroll
+        for (int v = 0; v < kVecs; ++v) id[v] = next[v];
+        if (j + 1 < units) fetch(0, j + 1, id, kx);
+        look_up(j + 2, next);
         // A NaN in V reaches the rows that see its token and no other: it is taken out here and remembered.
         bool any = false;
 #pragma unroll
@@ -401,7 +434,11 @@ __global__ void __launch_bounds__(threads_of(kDim), 1) kv8_attention_wide(AttnPa
         lay(smem + L::v + stage * L::kv_bytes, vx);
         bar_arrive(&sh.v_full[stage]);
       }
-    } else if (lane == 0) {
+    });
+  } else {
+    if (kGroups == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    walk([&](const Segment &, const SeqT &, uint32_t, uint32_t units, int, int live_rows) {
+      if (warp != kIssue || lane != 0) return;
       // ------------------------------------------------------------------ issuer
       constexpr uint32_t kScores = shape_f16(kTokens, false), kOutput = shape_f16(kDim, true);
       auto scores = [&](int g, uint32_t stage) {
@@ -439,22 +476,7 @@ __global__ void __launch_bounds__(threads_of(kDim), 1) kv8_attention_wide(AttnPa
           }
         }
       }
-    }
-    step += units;
-    ++n_segment;
-    u += units;
-    first_segment = false;
-    __syncwarp();
-    // every thread is through with this segment's marks before the next one sets them
-    if (u < u_end) {
-      if (__syncthreads_or(sh.stalled)) break;
-      if (sh.any_nan) {
-        __syncthreads();
-        for (int k = tid; k < kDim; k += blockDim.x) sh.nan_from[k] = INT_MAX;
-        if (tid == 0) sh.any_nan = 0;
-      }
-      __syncthreads();
-    }
+    });
   }
   // Everything that was issued has completed (the last commit was waited for), or a wait ran out.
   __syncwarp();
