@@ -1,5 +1,5 @@
 // Attention over the KV cache held in 8 bits (pf_kv8_attention): the joining of partial results, and the host's side.  The
-// attention itself is in kv8_attention_few.cu (up to 64 query rows of a KV head) and kv8_attention_wide.cu (more).
+// attention itself is in kv8_attention_few.cu (up to 32 query rows of a KV head) and kv8_attention_wide.cu (more).
 #include <algorithm>
 
 #include "kv8_attention.h"

@@ -636,11 +636,11 @@ void launch(const AttnParams &p, int rows, cudaStream_t stream) {
 
 }  // namespace
 
-// Up to 64 rows go in tiles of up to 32 (at 256 dimensions 16), K and V read once for each: at 16 requests of 4000 tokens, 4
-// KV heads of 128, 64 rows take 90 us here and 119 us in the form for many rows; 96 rows 138 us and 124 us.
+// Up to 32 rows go in tiles of up to 32 (at 256 dimensions 16).  16 requests of 4000 tokens, 4 KV heads of 128: 32 rows take
+// 61 us here and 68 us in the form for many rows, 64 rows (two tiles, K and V read for each) 90 us and 68 us.
 int kv8_few_rows(int dim, int64_t rows) {
   if (rows <= 16) return rows <= 4 ? 4 : rows <= 8 ? 8 : 16;
-  return rows <= 64 ? (dim == 256 ? 16 : 32) : 0;
+  return rows <= 32 ? (dim == 256 ? 16 : 32) : 0;
 }
 int kv8_few_ctas(int dim, int rows) { return few_ctas(dim, rows); }
 

@@ -90,13 +90,6 @@ __device__ __forceinline__ void load32(uint32_t (&r)[32], uint32_t at) {
       : "r"(at)
       : "memory");
 }
-__device__ __forceinline__ void store32(uint32_t at, const uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,"
-      "%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(at),
-      PF_I16(r, 0), PF_I16(r, 16)
-      : "memory");
-}
 __device__ __forceinline__ void load16(uint32_t (&r)[16], uint32_t at) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
@@ -112,6 +105,7 @@ __device__ __forceinline__ void store16(uint32_t at, const uint32_t (&r)[16]) {
       : "memory");
 }
 
+// 64 columns
 #define PF_E4(r, i) "=&r"(r[i]), "=&r"(r[i + 1]), "=&r"(r[i + 2]), "=&r"(r[i + 3])
 #define PF_E16(r, i) PF_E4(r, i), PF_E4(r, i + 4), PF_E4(r, i + 8), PF_E4(r, i + 12)
 #define PF_E64(r, i) PF_E16(r, i), PF_E16(r, i + 16), PF_E16(r, i + 32), PF_E16(r, i + 48)
@@ -126,22 +120,7 @@ __device__ __forceinline__ void load_all(uint32_t (&r)[64], uint32_t at) {
       : "r"(at)
       : "memory");
 }
-__device__ __forceinline__ void load_all(uint32_t (&r)[128], uint32_t at) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {"
-      "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,"
-      "%30,%31,%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,"
-      "%58,%59,%60,%61,%62,%63"
-      "}, [%128];\n\t"
-      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {"
-      "%64,%65,%66,%67,%68,%69,%70,%71,%72,%73,%74,%75,%76,%77,%78,%79,%80,%81,%82,%83,%84,%85,%86,%87,%88,%89,%90,%91,"
-      "%92,%93,%94,%95,%96,%97,%98,%99,%100,%101,%102,%103,%104,%105,%106,%107,%108,%109,%110,%111,%112,%113,%114,%115,"
-      "%116,%117,%118,%119,%120,%121,%122,%123,%124,%125,%126,%127"
-      "}, [%129];\n\ttcgen05.wait::ld.sync.aligned;"
-      : PF_E64(r, 0), PF_E64(r, 64)
-      : "r"(at), "r"(at + 64)
-      : "memory");
-}
+__device__ __forceinline__ void load_all(uint32_t (&r)[32], uint32_t at) { load32(r, at); }
 // Two fp32 operations an instruction.
 __device__ __forceinline__ uint64_t pair(float lo, float hi) {
   uint64_t d;
