@@ -23,7 +23,9 @@ Other modes (each prints one JSON line of its own):
     --peer [--peer-pairs K | --peer-local]
                          NVLink block copy between instances (GPU pairs, or both on one GPU)
     --transfer-grid      the reference's descriptor-level transfer_h2d grid on three backends
-    --ttft               cold / warm time-to-first-token shape through the connector hooks
+    --ttft [--kv8 [--kv8-keep N]]
+                         cold / warm time-to-first-token shape through the connector hooks; with --kv8 over caches
+                         held in 8 bits, with --kv8-keep shortened to N tokens behind the first one
     --vllm-ttft [--after-forward]
                          the same shape under a real vLLM engine with this library as KV connector
     --pool-coldstart     pinned-pool allocation strategies
@@ -1868,7 +1870,11 @@ def run_ttft(args):
     fills in: every layer's save is queued behind an event recorded after that layer's compute, and the
     decode step waits per layer on the layer's load event.  For a cold request both the time to the first
     token and the time until the KV blocks are in the pool (when the request's blocks may be reused) are
-    reported; the save is never on the first token's path, it only finishes earlier."""
+    reported; the save is never on the first token's path, it only finishes earlier.
+
+    With --kv8 the caches are Kv8Cache: a layer appends its keys and values, the decode step reads them with
+    Kv8Cache.attention, and half the bytes cross the link.  --kv8-keep N then shortens every layer's cache to N tokens by
+    the weights of the first token, into other blocks, and times that and one more token."""
     import torch
     import torch.nn.functional as F
     import pegaflow_b200 as pf
@@ -1887,7 +1893,13 @@ def run_ttft(args):
 
     w_qkv, w_o, w_gu, w_d = rnd(H, (NQ + 2 * NKV) * D), rnd(NQ * D, H), rnd(H, 2 * FFN), rnd(FFN, H)
     names = [f"model.layers.{l}.self_attn.attn" for l in range(L)]
-    caches = {n: torch.zeros((2, nb, BS, NKV, D), dtype=torch.bfloat16, device=dev) for n in names}
+    kv8, keep = args.kv8, args.kv8_keep
+    if keep and not (kv8 and 0 < keep <= T):
+        raise SystemExit(f"--kv8-keep needs --kv8 and a length from 1 to {T}")
+    if kv8:
+        caches = {n: pf.Kv8Cache(nb, BS, NKV, D, device=dev) for n in names}
+    else:
+        caches = {n: torch.zeros((2, nb, BS, NKV, D), dtype=torch.bfloat16, device=dev) for n in names}
     eng = pf.PegaEngine((2 * n_req + 2) * (L * per * 2 * BS * NKV * D * 2) + (256 << 20))
     conn = connector.PegaWorkerConnector(connector.InProcEngineClient(eng), eng, instance_id="ttft", namespace="ttft-ns",
                                          device_id=0, block_size=BS)
@@ -1895,26 +1907,34 @@ def run_ttft(args):
     rng = np.random.default_rng(11)
     compute = torch.cuda.Stream()
 
+    none, whole = (torch.full((1,), n, dtype=torch.int32, device=dev) for n in (0, T))
+
     def layer_prefill(x, cache, ids):
         x = F.rms_norm(x, (H,))
         qkv = x @ w_qkv
         q, k, v = qkv.split([NQ * D, NKV * D, NKV * D], dim=-1)
-        cache[0][ids] = k.view(per, BS, NKV, D)          # the layer's attention writes its KV pages
-        cache[1][ids] = v.view(per, BS, NKV, D)
+        if kv8:
+            cache.append(k.view(T, NKV, D), v.view(T, NKV, D), ids[None].int(), none)
+        else:
+            cache[0][ids] = k.view(per, BS, NKV, D)      # the layer's attention writes its KV pages
+            cache[1][ids] = v.view(per, BS, NKV, D)
         a = F.scaled_dot_product_attention(q.view(1, T, NQ, D).transpose(1, 2), k.view(1, T, NKV, D).transpose(1, 2),
                                            v.view(1, T, NKV, D).transpose(1, 2), is_causal=True, enable_gqa=True)
         x = x + a.transpose(1, 2).reshape(T, NQ * D) @ w_o
         gate, up = (x @ w_gu).chunk(2, dim=-1)
         return x + (F.silu(gate) * up) @ w_d
 
-    def layer_decode(x, cache, ids):
+    def layer_decode(x, cache, ids, lens=None, weights=None):
         x = F.rms_norm(x, (H,))
         qkv = x @ w_qkv
         q, _k, _v = qkv.split([NQ * D, NKV * D, NKV * D], dim=-1)
-        k = cache[0][ids].view(1, T, NKV, D).transpose(1, 2)   # reads the pages the load brought in
-        v = cache[1][ids].view(1, T, NKV, D).transpose(1, 2)
-        a = F.scaled_dot_product_attention(q.view(1, 1, NQ, D).transpose(1, 2), k, v, enable_gqa=True)
-        x = x + a.transpose(1, 2).reshape(1, NQ * D) @ w_o
+        if kv8:
+            a = cache.attention(q.view(1, NQ, D), ids[None].int(), whole if lens is None else lens, weights=weights)
+        else:
+            k = cache[0][ids].view(1, T, NKV, D).transpose(1, 2)   # reads the pages the load brought in
+            v = cache[1][ids].view(1, T, NKV, D).transpose(1, 2)
+            a = F.scaled_dot_product_attention(q.view(1, 1, NQ, D).transpose(1, 2), k, v, enable_gqa=True).transpose(1, 2)
+        x = x + a.reshape(1, NQ * D) @ w_o
         gate, up = (x @ w_gu).chunk(2, dim=-1)
         return x + (F.silu(gate) * up) @ w_d
 
@@ -1944,12 +1964,36 @@ def run_ttft(args):
             conn.wait_for_save()
         return first_token_ms, (time.perf_counter() - t0) * 1e3, hashes, ids_np
 
+    evict_ms, next_ms = [], []
+
+    def shorten(src_np, x, weights):
+        """Every layer's cache to `keep` tokens, in blocks that the request does not use, and one token over them."""
+        used = np.zeros(nb, dtype=bool)
+        used[src_np] = True
+        dst = torch.from_numpy(np.flatnonzero(~used)[1:1 + -(-keep // BS)].astype(np.int64)).to(dev)
+        src = torch.from_numpy(src_np.astype(np.int32)).to(dev)
+        t0 = time.perf_counter()
+        with torch.cuda.stream(compute):
+            for name in names:
+                lens, _, _ = caches[name].evict(src[None], whole, weights[name], dst[None].int(), keep, recent=min(keep, 64))
+        compute.synchronize()
+        t1 = time.perf_counter()
+        with torch.cuda.stream(compute):
+            for name in names:
+                x = layer_decode(x, caches[name], dst, lens)
+        compute.synchronize()
+        evict_ms.append((t1 - t0) * 1e3)
+        next_ms.append((time.perf_counter() - t1) * 1e3)
+        if not bool(torch.isfinite(x).all()):
+            raise RuntimeError("the token over the shortened cache is not finite")
+
     def warm(mode, r, hashes):
         dst_np = (rng.permutation(nb - 1)[:per] + 1)
         dst = torch.from_numpy(dst_np.astype(np.int64)).to(dev)
         for c in caches.values():
-            c[:, dst] = 0
+            (c.tensor if kv8 else c)[:, dst] = 0
         x = rnd(1, H, scale=1.0)
+        weights = {n: torch.zeros((1, NKV, T), device=dev) for n in names} if keep else None
         torch.cuda.synchronize()
         t0 = time.perf_counter()
         q = conn.client.query_prefetch("ttft", hashes, f"{mode}-w{r}")
@@ -1966,9 +2010,11 @@ def run_ttft(args):
             for name in names:
                 if mode == "layerwise":
                     conn.wait_for_layer_load(name, compute.cuda_stream)
-                x = layer_decode(x, caches[name], dst)
+                x = layer_decode(x, caches[name], dst, weights=weights[name] if keep else None)
         compute.synchronize()
         ms = (time.perf_counter() - t0) * 1e3
+        if keep and mode == "layerwise":
+            shorten(dst_np, x.detach().clone(), weights)
         if mode == "layerwise":
             done = []
             while not done:
@@ -1981,6 +2027,7 @@ def run_ttft(args):
     _, _, h0, _ = cold("after_forward", 99)
     warm("after_forward", 99, h0)
     modes = ("after_forward", "layerwise")
+    evict_ms.clear(), next_ms.clear()
     first_token = {m_: [] for m_ in modes}
     saved_at = {m_: [] for m_ in modes}
     warm_ms = {m_: [] for m_ in modes}
@@ -2005,6 +2052,9 @@ def run_ttft(args):
         # bit patterns, not values: equal NaNs must count as equal
         same = same and torch.equal(outs["after_forward"].view(torch.int32), outs["layerwise"].view(torch.int32)) \
             and bool(torch.isfinite(outs["after_forward"]).all())
+    if kv8:
+        for c in caches.values():
+            c.check()
     m = eng.metrics()
     conn.unregister()
     eng.close()
@@ -2012,11 +2062,11 @@ def run_ttft(args):
     def summary(v):
         return {"mean_ms": round(float(np.mean(v)), 2), "max_ms": round(float(np.max(v)), 2)}
 
-    kv_gib = L * per * 2 * BS * NKV * D * 2 / 2**30
+    kv_gib = L * per * 2 * pf.Kv8Cache.record_bytes(BS, NKV, D) / 2**30 if kv8 else L * per * 2 * BS * NKV * D * 2 / 2**30
     print(json.dumps({
         "metric": "ttft_shape_ms", "unit": "ms", "higher_is_better": False, "n_gpus": 1, "data": "synthetic",
         "config": {"workload": "llama3.1-8b, prompts of 10240 tokens, 1-token decode", "requests": n_req,
-                   "kv_gib_per_request": round(kv_gib, 3), "layers": L,
+                   "kv_gib_per_request": round(kv_gib, 3), "layers": L, "kv_dtype": "e4m3" if kv8 else "bf16",
                    "model": "synthetic layers of the model's sizes (torch matmul + SDPA, random weights)"},
         "cold_first_token": {k: summary(v) for k, v in first_token.items()},
         "cold_kv_in_pool": {k: summary(v) for k, v in saved_at.items()},
@@ -2024,6 +2074,7 @@ def run_ttft(args):
         "cold_kv_in_pool_earlier_by_ms": round(float(np.mean(saved_at["after_forward"]) - np.mean(saved_at["layerwise"])), 2),
         "warm_first_token_earlier_by_ms": round(float(np.mean(warm_ms["after_forward"]) - np.mean(warm_ms["layerwise"])), 2),
         "warm_outputs_identical": bool(same), "load_failures": m["load_failures"],
+        **({"shortened": {"keep": keep, "evict": summary(evict_ms), "token": summary(next_ms)}} if keep else {}),
         "published_reference": {"cold_mean_ms": 572.5, "warm_mean_ms": 61.5,
                                 "note": "README.md:89-94: H800, real vLLM serving at 4 req/s; context only"}}))
 
@@ -2284,6 +2335,9 @@ def main():
     ap.add_argument("--ttft", action="store_true",
                     help="cold / warm time-to-first-token shape through the connector hooks, blocking vs layer-wise")
     ap.add_argument("--ttft-requests", type=int, default=8)
+    ap.add_argument("--kv8", action="store_true", help="with --ttft: KV caches held in 8 bits (Kv8Cache)")
+    ap.add_argument("--kv8-keep", type=int, default=0, metavar="N",
+                    help="with --ttft --kv8: shorten every cache to N tokens behind the first token")
     ap.add_argument("--pool-coldstart", action="store_true", help="time the pinned-pool allocation strategies")
     ap.add_argument("--pool-gib", type=int, default=16)
     ap.add_argument("--transfer-grid", action="store_true",
