@@ -168,15 +168,20 @@ def test_append_token_by_token_gives_the_scales_of_one_call(pf):
 
 # ------------------------------------------------------------------------------------------------ attention
 def check_attention(pf, cache, q, tables, lens, counts, *, causal=True, scale=None, weights=False, rows_behind=0, out=None,
-                    want_cache=None, **kw):
+                    want_cache=None, called_with=None, **kw):
+    """called_with: (tables, lens) of the call where they are not those of the reference, with pages that are not there."""
     starts = starts_of(counts)
     heads, dim = cache.kv_heads, cache.head_dim
     scale_ = dim ** -0.5 if scale is None else scale
     longest = max(lens)
     w = torch.rand((len(lens), heads, longest + 5), generator=gen(99), device="cuda") if weights else None
     w0 = w.clone().cpu().double() if weights else None
-    got, lse = cache.attention(q, tables.cuda(), ints(lens), starts=ints(starts), max_query=max(max(counts), 1), scale=scale,
-                               causal=causal, weights=w, lse=True, out=out, **kw)
+    call_tables, call_lens = called_with or (tables, lens)
+    got, lse = cache.attention(q, call_tables.cuda(), ints(call_lens), starts=ints(starts), max_query=max(max(counts), 1),
+                               scale=scale, causal=causal, weights=w, lse=True, out=out, **kw)
+    if called_with:
+        with pytest.raises(pf.PegaflowInvalidArgument, match="block id"):
+            cache.check()
     cache.check()
     rc = want_cache or ref.Cache(cache)
     want, want_lse, size, spread, want_w = ref.attention(q.cpu(), rc, tables, lens, starts, scale_, causal)
@@ -320,6 +325,44 @@ def test_attention_over_scales_far_apart(pf):
     check_attention(pf, cache, (q.float() * 2.0 ** 100).bfloat16(), tables, lens, [20], scale=2.0 ** -104)
     check_attention(pf, cache, q * 0, tables, lens, [20], weights=True)
     check_attention(pf, cache, q, tables, lens, [20], scale=0.0)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("order", [1, -1])
+def test_attention_of_many_rows_over_scales_and_scores_that_grow(pf, dim, order):
+    """Scales of K and V that rise (or fall) by 2^3 from block to block, so that nearly every step moves the unit of O, and
+    scores of some rows that rise by hundreds along the sequence, so that the reference moves too."""
+    lens = [400, 90]
+    blocks, tables = make_tables(lens, 16, 45)
+    cache = make_cache(pf, blocks, 16, 1, dim, 46)
+    for s in range(2):
+        for i, b in enumerate(tables[s].tolist()):
+            cache.scales[1, b] = 2.0 ** (3 * order * i - 20)
+            cache.scales[0, b] = 2.0 ** (order * i // 4 - 5)
+    q = torch.randn((60, 2, dim), generator=gen(47), device="cuda").bfloat16()
+    q[::3] *= 16
+    check_attention(pf, cache, q, tables, lens, [40, 20])
+    check_attention(pf, cache, q, tables, lens, [40, 20], causal=False)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("counts", [[2], [40]])
+def test_attention_leaves_out_pages_that_are_not_there(pf, dim, counts):
+    """Like the sequence without them, whatever block 0 and the place behind the sequence's end hold."""
+    n, size = 600, 16
+    blocks, tables = make_tables([n], size, 48)
+    cache = make_cache(pf, blocks, size, 2, dim, 49)
+    cache.values[:, 0] = torch.full((2, 2, size, dim), math.nan, device="cuda").to(torch.float8_e4m3fn)
+    last = int(tables[0, n // size])
+    cache.values[:, last, :, n % size:] = torch.full((2, 2, size - n % size, dim), math.nan, device="cuda").to(torch.float8_e4m3fn)
+    q = torch.randn((sum(counts), 4, dim), generator=gen(50), device="cuda").half()
+    called = tables.clone()
+    gone = [0, 1, 2, 3, 4, 5, 6, 7, 11, 12, 30]         # the first step as a whole
+    for i in gone:
+        called[0, i] = -1 if i % 2 else 2 ** 30
+    there = [i for i in range(-(-n // size)) if i not in gone]
+    check_attention(pf, cache, q, tables[:, there].contiguous(), [n - size * len(gone)], counts, causal=False,
+                    called_with=(called, [n]))
 
 
 def test_attention_is_the_same_on_every_run(pf):
