@@ -154,12 +154,17 @@ __global__ void __launch_bounds__(kSelectThreads) kv8_select_kernel(EvictParams 
   for (int i = m + tid; i < p.keep; i += kSelectThreads) kept[i] = -1;
 }
 
+__device__ __forceinline__ __half2 half2_of(uint32_t x) { return *reinterpret_cast<__half2 *>(&x); }
+
 // kWarps warps make one new block of one head, K and V: a warp 2048 bytes of each, in registers.  Lane r finds where the
 // warp's r-th row lies (three dependent loads, once for K and V); rows are then read 16 bytes a lane.  Where
 // every row comes from a block of the scale that the new block gets, which is the common case, bytes are copied as they
 // are; otherwise they are multiplied as f16, which is exact down to 2^-24 while e4m3 ends at 2^-9.
+// Bound by memory, through the latency of those loads: 64 registers a thread, so that 32 warps share an SM.  16 sequences of
+// 10240 tokens shortened to 4096, 8 heads of 128 (the choice included): 80 us; at 80 registers 83 us; at 128 registers, with
+// the largest value looked for in converted numbers, 98 us; a warp for K and one for V 108 us.
 template <int kWarps>
-__global__ void __launch_bounds__(32 * (kWarps < 8 ? 8 : kWarps)) kv8_gather_kernel(EvictParams p) {
+__global__ void __launch_bounds__(32 * (kWarps < 8 ? 8 : kWarps), kWarps < 16 ? 4 : 2) kv8_gather_kernel(EvictParams p) {
   constexpr int kCta = kWarps < 8 ? 8 : kWarps, kTiles = kCta / kWarps;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = warp % kWarps;
   const int64_t tile = (int64_t)blockIdx.x * kTiles + warp / kWarps;
@@ -169,21 +174,14 @@ __global__ void __launch_bounds__(32 * (kWarps < 8 ? 8 : kWarps)) kv8_gather_ker
   after_previous();
   const bool mine = s < p.batch.n_seqs;
   const int m = mine ? min(p.length(s), p.keep) : 0, rows = min(m - (b << bl), 1 << bl);
-  uint32_t id = 0;
-  bool write = rows > 0;
-  if (write) {
-    id = (uint32_t)p.dst_tables[s * p.dst_stride + b];
-    if (id >= p.cache.num_blocks) {
-      if (lane == 0) p.batch.report(PF_KV8_BAD_BLOCK);
-      write = false;
-    }
-  }
-  // where row `lane` of this warp's share lies
+  // where row `lane` of this warp's share lies, and where the block goes
+  const bool has = lane < rows_held && row_first + lane < rows;
+  const int j = has ? p.kept[(int64_t)sh * p.keep + (b << bl) + row_first + lane] : 0;
+  const uint32_t id = rows > 0 ? (uint32_t)p.dst_tables[s * p.dst_stride + b] : 0xffffffffu;
   uint32_t src = 0;
   int at = 0, e_k = kKv8MinExp, e_v = kKv8MinExp;
   bool there = false;
-  if (write && lane < rows_held && row_first + lane < rows) {
-    const int j = p.kept[(int64_t)sh * p.keep + (b << bl) + row_first + lane];
+  if (has) {
     there = p.batch.block(p.cache, s, j >> bl, src);
     if (there) {
       at = j & ((1 << bl) - 1);
@@ -193,6 +191,8 @@ __global__ void __launch_bounds__(32 * (kWarps < 8 ? 8 : kWarps)) kv8_gather_ker
       p.batch.report(PF_KV8_BAD_BLOCK);
     }
   }
+  const bool write = id < p.cache.num_blocks;
+  if (rows > 0 && !write && lane == 0) p.batch.report(PF_KV8_BAD_BLOCK);
   uint4 x[2][4];
   int e_row[2][4];
 #pragma unroll
@@ -214,15 +214,27 @@ __global__ void __launch_bounds__(32 * (kWarps < 8 ? 8 : kWarps)) kv8_gather_ker
     uint32_t t = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
+      // magnitudes of e4m3 are ordered like their bits
       const uint32_t w[4] = {x[kv][i].x, x[kv][i].y, x[kv][i].z, x[kv][i].w};
-      __half2 h = __half2half2(__ushort_as_half(0));
+      uint32_t even = 0, odd = 0;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {       // max leaves a NaN out
-        const uint32_t a = f16x2_from_e4m3<0>(w[k]), c = f16x2_from_e4m3<1>(w[k]);
-        h = __hmax2(h, __hmax2(__habs2(*reinterpret_cast<const __half2 *>(&a)), __habs2(*reinterpret_cast<const __half2 *>(&c))));
+      for (int k = 0; k < 4; ++k) {
+        even = __vmaxu2(even, w[k] & 0x007f007fu);
+        odd = __vmaxu2(odd, w[k] >> 8 & 0x007f007fu);
       }
-      const float f = fmaxf(__low2float(h), __high2float(h)) * exp2i(e_row[kv][i]);
-      t = max(t, f == f ? __float_as_uint(f) : 0u);
+      even = __vmaxu2(even, odd);
+      uint32_t most = max(even & 0xffff, even >> 16);
+      if (most == 0x7f) {       // a NaN among them does not count
+        most = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+          for (int b8 = 0; b8 < 32; b8 += 8) {
+            const uint32_t m = w[k] >> b8 & 0x7f;
+            if (m != 0x7f) most = max(most, m);
+          }
+      }
+      t = max(t, __float_as_uint(__low2float(half2_of(f16x2_from_e4m3<0>(most))) * exp2i(e_row[kv][i])));
     }
     top[kv] = __reduce_max_sync(0xffffffffu, t);
     if (kWarps > 1 && lane == 0) sh_top[kv][warp] = top[kv];
