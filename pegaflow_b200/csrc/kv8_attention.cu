@@ -17,7 +17,8 @@ __device__ __forceinline__ uint32_t narrow2(float lo, float hi) {
 
 // Joins the parts of segments that several CTAs shared, in the order of the tokens.  CTA (b, y) looks at the boundary
 // between the ranges of CTAs b and b + 1: if it is the first one within a segment, it joins rows of it, a team of threads
-// for each.  kDim / 4 threads hold a row of a part as float4; a team of more reads several parts at once.
+// for each.  kDim / 4 threads hold a row of a part as float4; a team of more reads several parts at once.  Bound by latency:
+// some 5 us behind the last CTA of the attention.
 constexpr int kJoinThreads = 256;
 template <int kDim, int kRows, int kUnits, bool kBf16>
 __global__ void __launch_bounds__(kJoinThreads) kv8_attention_join(AttnParams p, int team) {

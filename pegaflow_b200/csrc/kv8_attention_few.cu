@@ -21,7 +21,10 @@
 //        that exactly down to 2^-11, that is 2^-17 of the largest, and smaller ones to 2^-28 of it
 //   V's scale goes on p: 2^(e - e_ref), e_ref the largest so far, and the sums are in units of it; the row sum leaves it out
 //   sums fp32, the tensor cores' and the row sum's; it takes p before it is rounded
-// Other forms were measured at 48 requests of 700 to 16001 tokens, 8 heads of 128 (75 us at the copy rate): K and V converted
+// What it measured: 48 requests of 700 to 16001 tokens, 8 heads of 128, groups of 4: 117 us (75 us at the copy rate), 8 of 10240
+// tokens 39 us (26 us).  Long tiles stream at 6.2 TB/s; a segment's beginning and end cost some 3 us and the call 14 to 20 us.
+// The pass for the weights reads K once more, 26 us for the 8 of 10240 tokens.
+// Other forms were measured at the 48 requests: K and V converted
 // to f16 in registers for m16n8k16 104 us, the same from rings in shared memory 108 us, m16n8k32 on e4m3 (which sm_100
 // does not have: it is converted and issued as f16) 109 us: bound by the issue of conversions with few warps to hide them.
 #include <cuda.h>
