@@ -273,25 +273,18 @@ __global__ void __launch_bounds__(threads_of(kDim), 1) kv8_attention_wide(AttnPa
           for (bool again = false;; again = true) {
             const uint64_t minus2 = pair(kShift - ref, kShift - ref);
             uint64_t part[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
-            auto columns = [&](auto &x, int c0) {
-              load_all(x, s_col + c0);
 #pragma unroll
-              for (int k = 0; k < (int)(sizeof(x) / 4); k += 2) {
+            for (int c0 = 0; c0 < kTokens; c0 += 32) {
+              uint32_t x[32];
+              load32(x, s_col + c0);
+#pragma unroll
+              for (int k = 0; k < 32; k += 2) {
                 float lo, hi;
                 unpair(fma2(pair(__uint_as_float(x[k]), __uint_as_float(x[k + 1])), unit2, minus2), lo, hi);
                 lo = exp2_fast(lo), hi = exp2_fast(hi);
                 part[k / 2 & 1] = add2(part[k / 2 & 1], pair(lo, hi));
                 h[(c0 + k) / 2] = f16x2(lo, hi);
               }
-            };
-            {
-              uint32_t x[64];
-              columns(x, 0);
-            }
-#pragma unroll
-            for (int c = 64; c < kTokens; c += 32) {
-              uint32_t x[32];
-              columns(x, c);
             }
             float lo, hi;
             unpair(add2(part[0], part[1]), lo, hi);

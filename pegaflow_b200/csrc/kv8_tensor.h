@@ -105,22 +105,6 @@ __device__ __forceinline__ void store16(uint32_t at, const uint32_t (&r)[16]) {
       : "memory");
 }
 
-// 64 columns
-#define PF_E4(r, i) "=&r"(r[i]), "=&r"(r[i + 1]), "=&r"(r[i + 2]), "=&r"(r[i + 3])
-#define PF_E16(r, i) PF_E4(r, i), PF_E4(r, i + 4), PF_E4(r, i + 8), PF_E4(r, i + 12)
-#define PF_E64(r, i) PF_E16(r, i), PF_E16(r, i + 16), PF_E16(r, i + 32), PF_E16(r, i + 48)
-__device__ __forceinline__ void load_all(uint32_t (&r)[64], uint32_t at) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {"
-      "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,"
-      "%30,%31,%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,"
-      "%58,%59,%60,%61,%62,%63"
-      "}, [%64];\n\ttcgen05.wait::ld.sync.aligned;"
-      : PF_E64(r, 0)
-      : "r"(at)
-      : "memory");
-}
-__device__ __forceinline__ void load_all(uint32_t (&r)[32], uint32_t at) { load32(r, at); }
 // Two fp32 operations an instruction.
 __device__ __forceinline__ uint64_t pair(float lo, float hi) {
   uint64_t d;
