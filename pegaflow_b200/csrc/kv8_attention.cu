@@ -49,8 +49,8 @@ __global__ void __launch_bounds__(kJoinThreads) kv8_attention_join(AttnParams p,
   const uint32_t u = split.begin(c0 + 1);
   const Segment seg(p, work, u);
   const SeqT seq(p, seg.s);
-  if (seg.begin == u || split.owner(seg.begin) != c0) return;
-  const int parts = split.owner(seg.begin + seg.units - 1) - c0 + 1, slot0 = 2 * c0 + (split.begin(c0) < seg.begin ? 1 : 0);
+  if (u <= seg.begin || split.owner(seg.begin) != c0) return;
+  const int parts = split.owner(seg.begin + seg.units - 1) - c0 + 1, slot0 = 2 * c0 + (split.begin(c0) < seg.from ? 1 : 0);
   const int teams = kJoinThreads / team, lane = threadIdx.x % team, part0 = lane / kSpan, at_once = team / kSpan, d = lane % kSpan * 4;
   const int live_rows = min(seq.all_rows(p) - seg.rt * kRows, kRows);
   auto slot_of = [&](int k) { return k == 0 ? slot0 : 2 * (c0 + k); };

@@ -191,11 +191,13 @@ __global__ void __launch_bounds__(kThreads, few_ctas(kDim, kRows)) kv8_attention
     const Segment seg(p, work, u);
     const int s = seg.s, head = seg.head;
     const SeqT seq(p, s);
-    const uint32_t unit0 = u - seg.begin;
+    uint32_t unit0, next = u;
+    int units = (int)seg.take(next, u_end, unit0);
+    if (units == 0) break;                 // the range ends within a segment's cost
     const int all_rows = seq.all_rows(p);
     // Attention: one row tile.  Weights: all of them, one after the other, each over all units.
     const int tiles = kWithV ? 1 : (all_rows + kRows - 1) / kRows;
-    const int units = (int)min(min(seg.units - unit0, u_end - u), tiles > 1 ? (uint32_t)kPass : 0xffffffffu);
+    if (tiles > 1 && units > kPass) units = kPass, next = seg.begin + unit0 + kPass;
     if (!kWithV && tiles > 1 && warp < 8)
       for (int j = warp >> 2; j < units; j += 2) sh.weight[j][tid % kTeam] = 0.f;         // a thread's own
     for (int tile = 0; tile < tiles && ok; ++tile) {
@@ -578,7 +580,7 @@ __global__ void __launch_bounds__(kThreads, few_ctas(kDim, kRows)) kv8_attention
       n_of[1] += steps >> 1;
       n_rows += steps > 0;
     }
-    u += units;
+    u = next;
     first_segment = false;
   }
   // The tensor cores' last arrivals, at the slots that are not filled again, come before the block leaves.

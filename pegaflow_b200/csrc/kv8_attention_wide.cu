@@ -510,13 +510,13 @@ __global__ void __launch_bounds__(threads_of(kDim), 1) kv8_attention_wide(AttnPa
       part.units = 0;
       if (u >= u_end) return;
       const Segment seg(p, work, u);
+      uint32_t unit0;
+      const uint32_t units = seg.take(u, u_end, unit0);
       const SeqT seq(p, seg.s);
-      const uint32_t unit0 = u - seg.begin, units = min(seg.units - unit0, u_end - u);
       part.s = seg.s, part.head = seg.head, part.row0 = seq.row0, part.rows = seq.rows, part.len = seq.len;
       part.row_first = seg.rt * kRows, part.live_rows = min(seq.all_rows(p) - seg.rt * kRows, kRows);
       part.unit0 = unit0, part.units = units;
       part.whole = units == seg.units, part.slot = 2 * blockIdx.x + (first ? 0 : 1);
-      u += units;
       first = false;
     };
     if (looks) {
