@@ -21,9 +21,10 @@
 //        that exactly down to 2^-11, that is 2^-17 of the largest, and smaller ones to 2^-28 of it
 //   V's scale goes on p: 2^(e - e_ref), e_ref the largest so far, and the sums are in units of it; the row sum leaves it out
 //   sums fp32, the tensor cores' and the row sum's; it takes p before it is rounded
-// What it measured: 48 requests of 700 to 16001 tokens, 8 heads of 128, groups of 4: 117 us (75 us at the copy rate), 8 of 10240
-// tokens 39 us (26 us).  Long tiles stream at 6.2 TB/s; a segment's beginning and end cost some 3 us and the call 14 to 20 us.
-// The pass for the weights reads K once more, 26 us for the 8 of 10240 tokens.
+// What it measured: 48 requests of 700 to 16001 tokens, 8 heads of 128, groups of 4: 99 us with the join (75 us at the copy rate; 119 us
+// with a split that does not count what a segment costs), 8 of 10240 tokens 37 us (26 us).  Long segments stream at 6.2 TB/s;
+// a segment's beginning and end cost 8000 cycles of one CTA, the call 14 to 20 us.  The pass for the weights reads K once
+// more, 26 us for the 8 of 10240 tokens.
 // Other forms were measured at the 48 requests: K and V converted
 // to f16 in registers for m16n8k16 104 us, the same from rings in shared memory 108 us, m16n8k32 on e4m3 (which sm_100
 // does not have: it is converted and issued as f16) 109 us: bound by the issue of conversions with few warps to hide them.
@@ -209,7 +210,7 @@ __global__ void __launch_bounds__(kThreads, few_ctas(kDim, kRows)) kv8_attention
       if (warp == 8) {
         // ---------------------------------------------------------------- feeding: lane = (values or scale, K or V, group)
         const int32_t *table = p.batch.tables + s * p.batch.table_stride;
-        const int group = lane & 7, kv = lane >> 3 & 1;
+        const int group = lane & 7, kv = lane >> 3 & 1, box = p.cache.block_size() / 16;      // groups of a block, and of a copy
         const char *scale_of = p.cache.base + kv * p.cache.kv_stride + p.cache.heads * p.cache.tile_bytes() + 4 * head;
         auto look_up = [&](int j) {
           const int tok = tok0 + j * kTokens + 16 * group;
@@ -226,7 +227,7 @@ __global__ void __launch_bounds__(kThreads, few_ctas(kDim, kRows)) kv8_attention
           const int tok = tok0 + j * kTokens + 16 * group;
           const bool there = id < p.cache.num_blocks;
           if (!there && tok < tok_end && lane < 8) p.batch.report(PF_KV8_BAD_BLOCK);
-          // a group that is not there lies behind the last block: the copy fills it with zeros
+          // a block that is not there lies behind the last one: the copy fills it with zeros
           const int row = tok & (p.cache.block_size() - 1), block = there ? (int)id : (int)p.cache.num_blocks;
           id = next;
           next = look_up(j + 2);
@@ -241,7 +242,7 @@ __global__ void __launch_bounds__(kThreads, few_ctas(kDim, kRows)) kv8_attention
             if (lane == 0)
               asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(shared_of(&sh.full[slot])), "r"(L::kTile) : "memory");
             __syncwarp();
-            if (lane < 16 && kv == of) {
+            if (lane < 16 && kv == of && (group & (box - 1)) == 0) {
 #pragma unroll
               for (int half = 0; half < kHalves; ++half)
                 asm volatile(
@@ -595,7 +596,8 @@ __global__ void __launch_bounds__(kThreads, few_ctas(kDim, kRows)) kv8_attention
   if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(L::kAlloc));
 }
 
-// The cache as [K or V][block][head][row][byte], tiles of 16 rows of (half) a head.
+// The cache as [K or V][block][head][row][byte], copied by the rows of a block of (half) a head: the copies' rate is one in 45 to
+// 60 cycles of an SM.  48 requests of 25600 tokens, 8 heads of 64, blocks of 64: 237 us, by copies of 16 rows 261 us.
 CUtensorMap map_of(const Kv8View &c) {
   using Encode = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
                               const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -608,7 +610,7 @@ CUtensorMap map_of(const Kv8View &c) {
   if (!encode) throw Error::cuda_init("cuTensorMapEncodeTiled is not available");
   const cuuint64_t dims[5] = {(cuuint64_t)c.dim, (cuuint64_t)c.block_size(), (cuuint64_t)c.heads, c.num_blocks, 2};
   const cuuint64_t strides[4] = {(cuuint64_t)c.dim, c.tile_bytes(), c.block_stride, c.kv_stride};
-  const cuuint32_t box[5] = {(cuuint32_t)std::min(c.dim, 128), 16, 1, 1, 1}, ones[5] = {1, 1, 1, 1, 1};
+  const cuuint32_t box[5] = {(cuuint32_t)std::min(c.dim, 128), (cuuint32_t)c.block_size(), 1, 1, 1}, ones[5] = {1, 1, 1, 1, 1};
   CUtensorMap map;
   if (encode(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 5, c.base, dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
              c.dim == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
