@@ -151,8 +151,8 @@ void check_args(const pf_kv8_attention_args *a, const Kv8View &c, const Kv8Batch
   if (rows_of_group > 0x3fffffffu) throw Error::invalid("too many query rows");
   if (!b.starts && b.n_seqs && a->max_query < (size_t)b.rows_each)
     throw Error::invalid(strf("max_query=%zu is below the %d rows of each sequence", a->max_query, b.rows_each));
-  // units are counted in 32 bits: (segments) x (units of a segment), summed over the sequences
-  const uint64_t units = ((uint64_t)b.max_blocks << c.block_log2) / 64 + 1;
+  // units are counted in 32 bits: (segments) x (units of a segment and its cost), summed over the sequences
+  const uint64_t units = ((uint64_t)b.max_blocks << c.block_log2) / 64 + 1 + 4;
   const uint64_t tiles = ((uint64_t)a->n_rows * (a->q_heads / c.heads) + 3) / 4 + b.n_seqs;
   if (units * tiles > 0xffffffffull / c.heads) throw Error::invalid("too many query rows for tables of this width: split the call");
 }
