@@ -116,16 +116,58 @@ __global__ void __launch_bounds__(kJoinThreads) kv8_attention_join(AttnParams p,
   }
 }
 
+// Each token's probability from the scores that the attention kept, added to the weights: a thread a token, rows in order.
+// Bound by memory, 4 bytes for each score and 8 for each weight.
+constexpr int kAddThreads = 256;
+template <int kRows>
+__global__ void __launch_bounds__(kAddThreads) kv8_weights_add(AttnParams p) {
+  after_previous();
+  const int s = blockIdx.x / p.cache.heads, head = blockIdx.x % p.cache.heads;
+  if (head == 0 && blockIdx.y == 0 && threadIdx.x == 0 && p.batch.lens[s] > p.w_capacity) p.batch.report(PF_KV8_BAD_LENGTH);
+  const Seq<kRows, 128> seq(p, s);
+  const int live_rows = min(seq.all_rows(p), kRows);
+  if (live_rows <= 0) return;
+  const int end = min(min(seq.visible(p, live_rows - 1), p.score_tokens), p.w_capacity);
+  float base[kRows];
+#pragma unroll
+  for (int r = 0; r < kRows; ++r) {
+    base[r] = INFINITY;        // a row that sees nothing weighs nothing
+    if (r < live_rows) {
+      const float lse = p.lse[(int64_t)(seq.row0 + r / p.group) * p.q_heads + head * p.group + r % p.group];
+      if (lse != -INFINITY) base[r] = lse * kLog2e;
+    }
+  }
+  const float *scores = p.scores + (int64_t)blockIdx.x * p.score_tokens * kRows;
+  float *weights = p.weights + s * p.w_seq + head * p.w_head;
+  for (int tok = blockIdx.y * kAddThreads + threadIdx.x; tok < end; tok += gridDim.y * kAddThreads) {
+    float w = 0.f;
+#pragma unroll
+    for (int c = 0; c < kRows / 4; ++c) {
+      const float4 x = *reinterpret_cast<const float4 *>(scores + (int64_t)tok * kRows + 4 * c);
+      const float y[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+      for (int r = 0; r < 4; ++r) w += 4 * c + r < live_rows ? exp2_fast(y[r] - base[4 * c + r]) : 0.f;
+    }
+    weights[tok] += w;
+  }
+}
+
 // ---------------------------------------------------------------------------------------------- host
 struct Plan {
   bool wide;            // rows by the hundred
   int n_ctas, rows;     // rows of a tile, and of a part
-  size_t part_o, part_ml, lse, bytes;   // offsets in the workspace
+  size_t part_o, part_ml, lse, scores, bytes;   // offsets in the workspace
+  int score_tokens;     // 0: scores are not kept
 };
 
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
-Plan make_plan(int device_id, const Kv8View &c, const pf_kv8_attention_args &a) {
+// The weights need every score once more, when the row's lse is known.  Of few rows the scores are kept, 8 bytes written and
+// read for each, where K is dim bytes and four products a row: for 8 sequences of 10240 tokens, 8 heads of 128, groups of 4, the
+// pass over the scores takes 12 us, the one over K 26 us (a call 55 and 67 us).  More rows, or more than this much workspace, read K again.
+constexpr uint64_t kMostScores = 256 << 20;
+
+Plan make_plan(int device_id, const Kv8View &c, const Kv8Batch &b, const pf_kv8_attention_args &a) {
   const size_t group = a.q_heads / c.heads;
   Plan plan{};
   const size_t rows = std::min(a.max_query, a.n_rows) * group;
@@ -137,7 +179,13 @@ Plan make_plan(int device_id, const Kv8View &c, const pf_kv8_attention_args &a) 
   plan.part_o = 0;
   plan.part_ml = up256(slots * c.dim * 4);
   plan.lse = plan.part_ml + up256(slots * 8);
-  plan.bytes = plan.lse + (a.weights && !a.lse ? up256(a.n_rows * a.q_heads * 4) : 0);
+  plan.scores = plan.lse + (a.weights && !a.lse ? up256(a.n_rows * a.q_heads * 4) : 0);
+  plan.bytes = plan.scores;
+  if (a.weights && !plan.wide && rows <= (size_t)plan.rows && plan.rows <= c.dim / 16) {      // one row tile
+    const uint64_t tokens = std::min<uint64_t>((uint64_t)b.max_blocks << c.block_log2, std::min<size_t>(a.weights_capacity, 0x7fffffff));
+    const uint64_t bytes = (uint64_t)b.n_seqs * c.heads * tokens * plan.rows * 4;
+    if (bytes <= kMostScores) plan.score_tokens = (int)tokens, plan.bytes += up256(bytes);
+  }
   return plan;
 }
 
@@ -188,7 +236,15 @@ void launch(const AttnParams &p, const Plan &plan, int n_sms, cudaStream_t strea
   if (p.cache.dim == 64) launch<64, kBf16>(p, plan, stream);
   else if (p.cache.dim == 128) launch<128, kBf16>(p, plan, stream);
   else launch<256, kBf16>(p, plan, stream);
-  if (p.weights && p.batch.n_seqs) kv8_weights_launch(p, kBf16, n_sms, stream);
+  if (!p.weights || !p.batch.n_seqs) return;
+  if (!p.scores) return kv8_weights_launch(p, kBf16, n_sms, stream);
+  auto add = [&](auto kernel) {
+    launch_after(kernel, dim3((unsigned)(p.batch.n_seqs * p.cache.heads), (unsigned)std::min((p.score_tokens + 1023) / 1024, 16)), kAddThreads, 0,
+                 stream, p);
+  };
+  if (plan.rows == 4) add(kv8_weights_add<4>);
+  else if (plan.rows == 8) add(kv8_weights_add<8>);
+  else add(kv8_weights_add<16>);
 }
 
 }  // namespace
@@ -206,7 +262,7 @@ int pf_kv8_attention_workspace(int device_id, const pf_kv8_cache *cache, const p
     const Kv8View c = kv8_check_cache(cache);
     const Kv8Batch b = kv8_check_batch(batch, args->n_rows);
     check_args(args, c, b);
-    *bytes = make_plan(device_id, c, *args).bytes;
+    *bytes = make_plan(device_id, c, b, *args).bytes;
   });
 }
 
@@ -221,7 +277,7 @@ int pf_kv8_attention(int device_id, const pf_kv8_cache *cache, const pf_kv8_batc
     if (a.n_rows == 0 || (b.n_seqs == 0 && !a.clear_tail)) return;
     if (!a.q || !a.out) throw Error::invalid("null q or out");
     if ((uintptr_t)a.q % 2 || (uintptr_t)a.out % 2) throw Error::invalid("q and out must be aligned to their elements");
-    const Plan plan = make_plan(device_id, c, a);
+    const Plan plan = make_plan(device_id, c, b, a);
     if (!workspace || workspace_bytes < plan.bytes)
       throw Error::invalid(strf("workspace of %zu bytes, the call needs %zu", workspace ? workspace_bytes : 0, plan.bytes));
     if ((uintptr_t)workspace % 256) throw Error::invalid("the workspace must be 256-byte aligned");
@@ -235,6 +291,8 @@ int pf_kv8_attention(int device_id, const pf_kv8_cache *cache, const pf_kv8_batc
     p.part_ml = (float2 *)(ws + plan.part_ml);
     p.lse = a.lse ? a.lse : a.weights ? (float *)(ws + plan.lse) : nullptr;
     p.weights = a.weights;
+    p.scores = plan.score_tokens ? (float *)(ws + plan.scores) : nullptr;
+    p.score_tokens = plan.score_tokens;
     p.q_row = (int64_t)a.q_row_stride, p.q_head = (int64_t)a.q_head_stride;
     p.out_row = (int64_t)a.out_row_stride, p.out_head = (int64_t)a.out_head_stride;
     p.w_seq = (int64_t)a.weights_seq_stride, p.w_head = (int64_t)a.weights_head_stride;

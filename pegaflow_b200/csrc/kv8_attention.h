@@ -29,6 +29,9 @@ struct AttnParams {
   // part_ml holds (base, sum): the row's sum and its part_o are of terms 2^(score - base), scores in base 2.
   float *part_o;    // [slots][rows][dim]
   float2 *part_ml;  // [slots][rows]
+  // Scores in base 2, kept for the weights, or null: [sequence][KV head][score_tokens][rows of the tile].
+  float *scores;
+  int score_tokens;
   int n_ctas, device;
 };
 

@@ -23,8 +23,8 @@
 //   sums fp32, the tensor cores' and the row sum's; it takes p before it is rounded
 // What it measured: 48 requests of 700 to 16001 tokens, 8 heads of 128, groups of 4: 99 us with the join (75 us at the copy rate; 119 us
 // with a split that does not count what a segment costs), 8 of 10240 tokens 37 us (26 us).  Long segments stream at 6.2 TB/s;
-// a segment's beginning and end cost 8000 cycles of one CTA, the call 14 to 20 us.  The pass for the weights reads K once
-// more, 26 us for the 8 of 10240 tokens.
+// a segment's beginning and end cost 8000 cycles of one CTA, the call 14 to 20 us.  The pass for the weights of
+// more rows than scores are kept for reads K once more, 26 us for the 8 of 10240 tokens.
 // Other forms were measured at the 48 requests: K and V converted
 // to f16 in registers for m16n8k16 104 us, the same from rings in shared memory 108 us, m16n8k32 on e4m3 (which sm_100
 // does not have: it is converted and issued as f16) 109 us: bound by the issue of conversions with few warps to hide them.
@@ -488,6 +488,9 @@ __global__ void __launch_bounds__(kThreads, few_ctas(kDim, kRows)) kv8_attention
               float x[4];
               if (c == 0) x[0] = first[0], x[1] = first[1], x[2] = first[2], x[3] = first[3];
               else scores(c, x);
+              if (p.scores && tok < min(tok_end, p.score_tokens))
+                *reinterpret_cast<float4 *>(p.scores + (((int64_t)s * p.cache.heads + head) * p.score_tokens + tok) * kRows + 4 * c) =
+                    make_float4(x[0], x[1], x[2], x[3]);
 #pragma unroll
               for (int r = 0; r < 4; ++r) {
                 x[r] = exp2_fast(x[r] - (sh.ref[team][4 * c + r] - kShift));

@@ -203,7 +203,7 @@ class Kv8Cache:
         args = N.Kv8AttentionArgs(q.data_ptr(), out.data_ptr(), lse_out.data_ptr() if lse else None, w_ptr, n_rows, max_query,
                                   qs[0], qs[1], os[0], os[1], w_seq, w_head, capacity, q_heads, code, 1 if causal else 0, clear,
                                   dim ** -0.5 if scale is None else scale)
-        sizes = (n_rows, q_heads, max_query, batch.n_seqs, batch.max_blocks, starts is None, lse, w_ptr is None)
+        sizes = (n_rows, q_heads, max_query, batch.n_seqs, batch.max_blocks, starts is None, lse, w_ptr is None, capacity)
         need = self._workspaces.get(sizes)
         if need is None:
             size = N.sz()

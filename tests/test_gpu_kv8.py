@@ -365,6 +365,38 @@ def test_attention_leaves_out_pages_that_are_not_there(pf, dim, counts):
                     called_with=(called, [n]))
 
 
+def test_weights_of_few_rows_with_and_without_room_for_their_scores(pf):
+    """Tables and weights so wide that the scores of all their tokens are not kept: the same weights as in narrow ones."""
+    lens, size = [70, 400], 16
+    blocks, tables = make_tables(lens, size, 55)
+    cache = make_cache(pf, blocks, size, 1, 128, 56)
+    q = torch.randn((2, 4, 128), generator=gen(57), device="cuda").bfloat16()
+    w = torch.zeros((2, 1, 400), device="cuda")
+    check_attention(pf, cache, q, tables, lens, [1, 1], weights=True)
+    cache.attention(q, tables.cuda(), ints(lens), weights=w)
+    width = 600_000
+    wide_t = torch.zeros((2, width), dtype=torch.int32, device="cuda")
+    wide_t[:, :tables.shape[1]] = tables.cuda()
+    wide_w = torch.zeros((2, 1, width * size), device="cuda")
+    cache.attention(q, wide_t, ints(lens), weights=wide_w)
+    cache.check()
+    # the scores come from the same products, the exponentials from the same function of the same numbers but for their
+    # rounding: 2^-20 of each, and 4 rows added
+    assert torch.allclose(wide_w[:, :, :400], w, rtol=2.0 ** -19, atol=0) and (wide_w[:, :, 400:] == 0).all()
+
+
+def test_weights_of_rows_whose_pages_are_not_there(pf):
+    """A sequence of which nothing is there weighs nothing; the other's weights are as ever."""
+    cache = make_cache(pf, 6, 16, 2, 128, 58)
+    q = torch.randn((2, 4, 128), generator=gen(59), device="cuda").half()
+    w = torch.zeros((2, 2, 32), device="cuda")
+    cache.attention(q, ints([[77, -1], [1, 2]]), ints([30, 20]), weights=w)
+    with pytest.raises(pf.PegaflowInvalidArgument, match="block id"):
+        cache.check()
+    assert (w[0] == 0).all() and torch.allclose(w[1].sum(-1), torch.full((2,), 2.0, device="cuda"), atol=2.0 ** -16)
+    assert (w[1, :, 20:] == 0).all()
+
+
 def test_attention_is_the_same_on_every_run(pf):
     lens = [700, 5000, 33]
     blocks, tables = make_tables(lens, 16, 51)
