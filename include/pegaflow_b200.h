@@ -613,8 +613,9 @@ typedef struct pf_kv8_attention_args {
   int clear_tail;              /* 1: rows behind the last sequence get out = 0, lse = -infinity */
   float scale;
 } pf_kv8_attention_args;
-/* Workspace bytes for a call of these sizes (pointers are not looked at).  The workspace is device memory, 256-byte
- * aligned, used by one call at a time. */
+/* Workspace bytes for a call of these sizes: rows, heads, table width, weights_capacity and which of lse and weights are
+ * given count, what pointers point at does not.  The workspace is device memory, 256-byte aligned, used by one call at
+ * a time. */
 int pf_kv8_attention_workspace(int device_id, const pf_kv8_cache *cache, const pf_kv8_batch *batch,
                                const pf_kv8_attention_args *args, size_t *bytes);
 int pf_kv8_attention(int device_id, const pf_kv8_cache *cache, const pf_kv8_batch *batch,
