@@ -93,11 +93,6 @@ __device__ __forceinline__ int kv8_scale_exponent(float scale) {
   const int e = (int)((__float_as_uint(scale) >> 23) & 255) - 127;
   return min(max(e, kKv8MinExp), kKv8MaxExp);
 }
-// |x| as ordered bits; infinities and NaN do not count (they would make every other value 0).
-__device__ __forceinline__ uint32_t kv8_magnitude(float x) {
-  const uint32_t b = __float_as_uint(x) & 0x7fffffffu;
-  return b < 0x7f800000u ? b : 0u;
-}
 
 // Round to nearest even, saturating: an infinity becomes +-448 steps, a NaN stays NaN.
 __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {

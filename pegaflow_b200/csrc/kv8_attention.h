@@ -177,10 +177,6 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return d;
 }
 template <bool kBf16>
-__device__ __forceinline__ float widen1(uint16_t x) {
-  return kBf16 ? __uint_as_float((uint32_t)x << 16) : __half2float(__ushort_as_half(x));
-}
-template <bool kBf16>
 __device__ __forceinline__ uint32_t narrow2(float lo, float hi) {
   if (!kBf16) return f16x2(lo, hi);
   uint32_t d;
