@@ -21,7 +21,7 @@ NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-lineinfo", "-O3", "-std=c++17",
     "-Xcompiler", "-fPIC,-g,-Wall,-Wextra,-Wno-unused-parameter",
-    "--shared",
+    "--shared", "--threads", "0",      # files side by side
 ]
 LINK_FLAGS = ["-lpthread", "-ldl", "-lrt"]
 
