@@ -350,8 +350,11 @@ __global__ void __launch_bounds__(kThreads, few_ctas(kDim, kRows)) kv8_attention
             sh.factor[r] = p.scale * kLog2e * exp2i(ex);
             sh.see[r] = live ? seq.visible(p, row) : 0;
             sh.ref[0][r] = sh.ref[1][r] = kNone;
-            // rows that are not there, or see nothing, weigh nothing
-            if (!kWithV) sh.base[r] = sh.see[r] > 0 ? p.lse[(int64_t)(seq.row0 + i) * p.q_heads + qh] * kLog2e : INFINITY;
+            // Rows that are not there, or see nothing (no token, or missing pages only: lse is -inf), weigh nothing.
+            if (!kWithV) {
+              const float lse = sh.see[r] > 0 ? p.lse[(int64_t)(seq.row0 + i) * p.q_heads + qh] : -INFINITY;
+              sh.base[r] = lse == -INFINITY ? INFINITY : lse * kLog2e;
+            }
           }
         }
         fence_to_async();

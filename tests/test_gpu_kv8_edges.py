@@ -1,0 +1,84 @@
+"""The 8-bit KV cache on a GPU at the edges of what its calls allow: pages that are missing, rows of no sequence, tensors
+of other streams, caches in slices of a buffer, sizes beyond the other tests'."""
+import math
+
+import pytest
+import torch
+
+from tests import kv8_reference as ref
+from tests.test_gpu_kv8 import bytes_of, gen, ints, make_cache, make_tables, pf, same_bytes, starts_of  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+def rows_of(cache, kv, table, n):
+    """float64 [kv_heads, n, dim] on the GPU: what the first n tokens of a block table hold; 0 for pages that are not there."""
+    size = cache.block_size
+    ids = torch.tensor(table[: -(-n // size)], dtype=torch.long, device="cuda")
+    there = (ids >= 0) & (ids < cache.num_blocks)
+    at = torch.where(there, ids, torch.zeros_like(ids))
+    x = cache.values[kv, at].double() * cache.scales[kv, at].double()[:, :, None, None]
+    x = torch.where(there[:, None, None, None], x, torch.zeros_like(x))
+    return x.transpose(0, 1).reshape(cache.kv_heads, -1, cache.head_dim)[:, :n], there.repeat_interleave(size)[:n]
+
+
+def plain(cache, q, table, n, scale, causal=True):
+    """64 bits, one sequence: (out, lse, weights, sum p |v|, spread); a row that sees nothing gives 0, -infinity and no weight."""
+    rows, q_heads, dim = q.shape
+    heads, group = cache.kv_heads, q_heads // cache.kv_heads
+    (k, there), (v, _) = rows_of(cache, 0, table, n), rows_of(cache, 1, table, n)
+    last = n - rows + torch.arange(rows, device="cuda") if causal else torch.full((rows,), n, device="cuda")
+    see = (torch.arange(n, device="cuda")[None] <= last[:, None]) & there
+    x = torch.einsum("ihgd,hjd->ihgj", q.double().view(rows, heads, group, dim), k) * scale
+    x = x.masked_fill(~see[:, None, None], -math.inf)
+    lse = torch.logsumexp(x, -1)
+    p = torch.where(torch.isneginf(lse)[..., None], torch.zeros_like(x), torch.exp(x - lse[..., None]))
+    spread = (torch.einsum("ihgd,hjd->ihgj", q.double().abs().view(rows, heads, group, dim), k.abs()) * abs(scale) * see[:, None, None]).amax(-1)
+    back = lambda t: t.reshape(rows, q_heads, dim)  # noqa: E731
+    return (back(torch.einsum("ihgj,hjd->ihgd", p, v)), lse.reshape(rows, q_heads), p.sum((0, 2)),
+            back(torch.einsum("ihgj,hjd->ihgd", p, v.abs())), spread.reshape(rows, q_heads))
+
+
+def close(cache, q, got, lse, weights, before, want, n):
+    """The bounds of tests/test_gpu_kv8.py: ds of a score, p to 2^-21 and, for the product with V, 2^-11, sums of n terms."""
+    out, want_lse, w, size, spread = want
+    dim, rows = q.shape[2], q.shape[0] * q.shape[1] // cache.kv_heads
+    ds = (dim + 8) * 2.0 ** -23 * spread
+    rel = 2 * (ds + 2.0 ** -21) + 2.0 ** -11 + 2 * n * 2.0 ** -24
+    big = float((cache.values.double().abs().nan_to_num() * cache.scales.double()[..., None, None]).max())
+    half = 2.0 ** -8 if q.dtype == torch.bfloat16 else 2.0 ** -11
+    tol = size * rel[..., None] + half * out.abs() + big * n * (2.0 ** -27 if rows <= 32 else 2.0 ** -30) + 1e-30
+    assert ((got.double() - out).abs() <= tol).all()
+    if lse is not None:
+        none = torch.isneginf(want_lse)
+        assert torch.equal(torch.isneginf(lse.double()), none)
+        assert ((lse.double() - want_lse).abs() <= 2 * ds + 2.0 ** -20 + 2.0 ** -22 * want_lse.abs() + n * 2.0 ** -24)[~none].all()
+    if weights is not None:
+        # score and lse are off by ds each, twice where they are computed twice; rows terms are added, then one more
+        worst = 4 * float(ds.max()) + 2.0 ** -19 + n * 2.0 ** -23 + rows * 2.0 ** -24
+        total = before.double() + w
+        assert ((weights.double() - total).abs() <= w * worst + 2.0 ** -23 * total).all()
+
+
+# ------------------------------------------------------------------------------------------------ pages that are missing
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("rows", [1, 2, 5, 40])
+@pytest.mark.parametrize("missing", ["first", "all", "from the fourth on"])
+def test_weights_of_rows_that_see_missing_pages_only(pf, dim, rows, missing):
+    """One row or several row tiles, scores kept or taken again: rows of which every visible page is missing weigh nothing, and
+    tokens that other rows see get those rows' weights."""
+    size, heads, group, n = 16, 2, 4, 16 + rows - 1 if missing == "first" else 90      # row 0 sees the first page alone
+    blocks, tables = make_tables([n], size, 201)
+    cache = make_cache(pf, blocks, size, heads, dim, 202)
+    table = tables[0].tolist()
+    gone = {"first": [0], "all": range(len(table)), "from the fourth on": range(3, len(table))}[missing]
+    for i in gone:
+        table[i] = -1 if i % 2 else blocks
+    q = torch.randn((rows, heads * group, dim), generator=gen(203), device="cuda").bfloat16()
+    w = torch.rand((1, heads, n + 3), generator=gen(204), device="cuda")
+    before = w.clone()
+    out, lse = cache.attention(q, ints([table]), ints([n]), weights=w, lse=True)
+    with pytest.raises(pf.PegaflowInvalidArgument, match="block id"):
+        cache.check()
+    assert torch.isfinite(w).all() and torch.equal(w[..., n:], before[..., n:])
+    close(cache, q, out, lse, w[0, :, :n], before[0, :, :n], plain(cache, q, table, n, dim ** -0.5), n)
