@@ -132,14 +132,17 @@ class InProcEngineClient:
 
     def register_context_batch(self, instance_id, namespace, tp_rank, pp_rank, tp_size, world_size, device_id,
                                layer_names, tensors, num_blocks_list, bytes_per_block_list, kv_stride_bytes_list,
-                               segments_list, transfer_backend, page_first, layer_group_ids=None):
+                               segments_list, transfer_backend, page_first, layer_group_ids=None,
+                               block_stride_bytes_list=None):
+        """``block_stride_bytes_list`` (additive): from block to block of each layer, where blocks do not follow each other."""
         if transfer_backend not in ("direct", "kernel"):
             raise ValueError(f"unknown transfer_backend {transfer_backend!r}")
         regions = [_region_of(t) for t in tensors]
         return self._reply(lambda: self._engine.register_context_layer_batch_strided(
             instance_id, namespace, device_id, tp_rank, pp_rank, tp_size, world_size, list(layer_names),
             [r[0] for r in regions], [r[1] for r in regions], list(num_blocks_list), list(bytes_per_block_list),
-            list(kv_stride_bytes_list), list(segments_list), None,
+            list(kv_stride_bytes_list), list(segments_list),
+            list(block_stride_bytes_list) if block_stride_bytes_list is not None else None,
             list(layer_group_ids) if layer_group_ids is not None else None, transfer_backend, page_first))
 
     def unregister_context(self, instance_id):
@@ -392,10 +395,17 @@ class PegaWorkerConnector:
     def register_kv_caches(self, kv_caches: Dict[str, object]):
         if not kv_caches:
             raise RuntimeError("No KV cache layers were selected for registration")
-        names, tensors, nb, bpb, kvs, segs = [], [], [], [], [], []
+        names, tensors, nb, bpb, kvs, segs, strides = [], [], [], [], [], [], []
+        in_slices = False
         for name, t in kv_caches.items():
-            t = getattr(t, "tensor", t)          # a Kv8Cache registers the tensor that it lies in
-            info = infer_kv_cache_registration(t, self.block_size, is_mla=self.is_mla)
+            if hasattr(t, "registration"):       # a Kv8Cache knows its records, which other layers' may lie between
+                t, blocks, segment, kv_stride, stride = t.registration()
+                in_slices |= stride is not None
+                info = KVCacheRegistrationInfo("KV-first", blocks, segment, kv_stride, 2, 1)
+            else:
+                info, stride = infer_kv_cache_registration(t, self.block_size, is_mla=self.is_mla), None
+            # the engine's own default where none is given: segments that follow each other, or whole blocks
+            strides.append(stride or info.bytes_per_block * (1 if info.kv_stride_bytes > info.bytes_per_block else info.segments))
             self.registrations[name] = info
             names.append(name)
             tensors.append(t)
@@ -403,6 +413,11 @@ class PegaWorkerConnector:
             bpb.append(info.bytes_per_block)
             kvs.append(info.kv_stride_bytes)
             segs.append(info.segments)
+        more = {}
+        if in_slices:
+            if not isinstance(self.client, InProcEngineClient):
+                raise ValueError("8-bit caches in slices of a larger buffer register with an engine of this process only")
+            more["block_stride_bytes_list"] = strides
         if not isinstance(self.client, InProcEngineClient):
             # an engine in another process gets the tensors as pickled CUDA IPC wrappers (worker.py:326-349)
             from .ipc import CudaIPCWrapper
@@ -410,7 +425,7 @@ class PegaWorkerConnector:
             tensors = [CudaIPCWrapper(t).to_bytes() for t in tensors]
         ok, msg = self.client.register_context_batch(self.instance_id, self.namespace, self.tp_rank, self.pp_rank,
                                                      self.tp_size, self.world_size, self.device_id, names, tensors,
-                                                     nb, bpb, kvs, segs, self.transfer_backend, self.page_first)
+                                                     nb, bpb, kvs, segs, self.transfer_backend, self.page_first, **more)
         if not ok:
             raise RuntimeError(f"Register context batch failed for layers {names}: {msg}")
         self.registered_layers = names

@@ -1,10 +1,11 @@
 """KV cache of one layer held in 8 bits: write, attention, eviction by accumulated attention weight.
 
 ``Kv8Cache.tensor`` is a uint8 tensor ``[2 (K, V), num_blocks, record]``; a record holds ``kv_heads x block_size x
-head_dim`` e4m3 values and one power-of-two fp32 scale for each head (include/pegaflow_b200.h, section 5).  It registers
-like any KV tensor whose first dimension is 2 (``PegaWorkerConnector.register_kv_caches({name: cache.tensor})``, or the
-cache itself), so that saves, loads and peer copies move half the bytes of a 16-bit cache and a block's
-scales travel with it.
+head_dim`` e4m3 values and one power-of-two fp32 scale for each head (include/pegaflow_b200.h, section 5).  A cache registers
+like any KV tensor whose first dimension is 2 (``PegaWorkerConnector.register_kv_caches({name: cache})``), so that saves, loads
+and peer copies move half the bytes of a 16-bit cache and a block's scales travel with it.  Of a cache in a slice of a larger
+buffer its records alone are registered, with an engine of the same process; ``cache.tensor`` in its place would be taken to own
+all bytes from one block to the next.
 
 The calls only enqueue work, on the current torch stream of the cache's device unless ``stream`` (a cudaStream_t value)
 says otherwise, and may be captured into a CUDA graph.  Block tables, lengths and row starts are int32 tensors on
@@ -83,6 +84,17 @@ class Kv8Cache:
         self.values = t[:, :, :n].view(torch.float8_e4m3fn).view(2, t.shape[1], kv_heads, block_size, head_dim)
         #: View of the scales: [2, num_blocks, kv_heads], float32.
         self.scales = t[:, :, n:n + 4 * kv_heads].view(torch.float32)
+
+    def registration(self):
+        """What an engine needs to know of the layer: (tensor, or (address, bytes) where it is a slice of a larger buffer; number
+        of blocks; bytes of a segment; from K to V of a block; from block to block, None where blocks are dense)."""
+        t = self.tensor
+        n, width = t.shape[1], t.shape[2]
+        if t.storage_offset() == 0 and t.stride(1) == width:
+            return t, n, width, t.stride(0), None
+        behind = t.untyped_storage().nbytes() - t.storage_offset()
+        record = self.record_bytes(self.block_size, self.kv_heads, self.head_dim)
+        return (t.data_ptr(), behind), n, record, t.stride(0), max(t.stride(1), record)
 
     def check(self):
         """Raise if a call since the last check met a block id, a length or row starts that it had to leave out.  Waits

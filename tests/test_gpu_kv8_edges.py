@@ -82,3 +82,59 @@ def test_weights_of_rows_that_see_missing_pages_only(pf, dim, rows, missing):
         cache.check()
     assert torch.isfinite(w).all() and torch.equal(w[..., n:], before[..., n:])
     close(cache, q, out, lse, w[0, :, :n], before[0, :, :n], plain(cache, q, table, n, dim ** -0.5), n)
+
+
+# ------------------------------------------------------------------------------------------------ caches in slices of a buffer
+SLICES = {
+    # shape of the buffer (2: K and V, 12 blocks, 3 layers), a layer's cache in it
+    "layers within a block": (lambda r: (2, 12, 3, r), lambda t, i: t[:, :, i]),
+    "layers outermost": (lambda r: (3, 2, 12, r), lambda t, i: t[i]),
+    "K and V of a block together": (lambda r: (12, 3, 2, r), lambda t, i: t[:, i].transpose(0, 1)),
+    "records with room behind them": (lambda r: (2, 12, 3, r + 48), lambda t, i: t[:, :, i]),
+}
+
+
+@pytest.mark.parametrize("only", [None, 0])
+@pytest.mark.parametrize("layout", SLICES)
+def test_caches_in_a_slice_of_a_larger_buffer_are_saved_and_loaded_alone(pf, layout, only):
+    """A load writes the records of its own layer, block and all, and leaves every other byte of the buffer as it was; so
+    does a peer copy."""
+    from pegaflow_b200 import connector
+
+    size, heads, dim = 16, 2, 64
+    shape, slice_of = SLICES[layout]
+    record = pf.Kv8Cache.record_bytes(size, heads, dim)
+    buffers = [torch.randint(0, 256, shape(record), dtype=torch.uint8, device="cuda", generator=gen(210 + i)) for i in range(2)]
+    use = [0, 1, 2] if only is None else [only]
+    caches = [{f"l{i}": pf.Kv8Cache.from_tensor(slice_of(b, i), size, heads, dim) for i in use} for b in buffers]
+    eng = pf.PegaEngine(64 << 20)
+    client = connector.InProcEngineClient(eng)
+    conns = [connector.PegaWorkerConnector(client, eng, instance_id=who, namespace="kv8", device_id=0, block_size=size) for who in "ab"]
+    for conn, c in zip(conns, caches):
+        conn.register_kv_caches(c)
+        assert all(conn.registrations[n].bytes_per_block == record for n in c)
+    src, home = [2, 7, 11], [5, 1, 9]
+    hashes = [b"slice-%d" % i for i in range(3)]
+    torch.cuda.synchronize()
+    conns[0].wait_for_save([(n, src, hashes) for n in caches[0]])
+    want = buffers[1].clone()
+    for i in use:
+        slice_of(want, i)[:, home, :record] = slice_of(buffers[0], i)[:, src, :record]
+    hit = client.query_prefetch("b", hashes, "r")
+    assert hit.num_hit_blocks == 3
+    torch.cuda.synchronize()
+    conns[1].start_load_kv([("r", hit.lease, home)])
+    done = []
+    while not done:
+        done, failed = conns[1].get_finished()
+        assert not failed
+    torch.cuda.synchronize()
+    assert torch.equal(buffers[1], want)
+    eng.peer_load("a", 0, "b", 0, src, [4, 3, 0])
+    for i in use:
+        slice_of(want, i)[:, [4, 3, 0], :record] = slice_of(buffers[0], i)[:, src, :record]
+    torch.cuda.synchronize()
+    assert torch.equal(buffers[1], want)
+    for conn in conns:
+        conn.unregister()
+    eng.close()

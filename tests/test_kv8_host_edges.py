@@ -1,0 +1,50 @@
+"""Host side of the 8-bit KV cache at the edges: registration of caches in slices, refusals (no GPU needed)."""
+import pytest
+import torch
+
+
+class _Sliced:
+    """What a Kv8Cache in a slice says of itself."""
+
+    def registration(self):
+        return (0x70000, 8 * 6192 * 2 - 2064), 8, 2064, 8 * 6192, 6192
+
+
+def _worker(client):
+    from pegaflow_b200.connector import PegaWorkerConnector
+
+    return PegaWorkerConnector(client, None, instance_id="i", namespace="n", device_id=0, block_size=16)
+
+
+def test_a_cache_in_a_slice_registers_its_records_and_their_stride():
+    import pegaflow_b200 as pf
+
+    seen = {}
+
+    class Client(pf.InProcEngineClient):
+        def __init__(self):
+            pass
+
+        def register_context_batch(self, *a, **kw):
+            seen["args"], seen["kw"] = a, kw
+            return True, ""
+
+    w = _worker(Client())
+    w.register_kv_caches({"a": _Sliced(), "b": torch.zeros((2, 8, 100), dtype=torch.uint8), "c": torch.zeros((8, 100), dtype=torch.uint8),
+                          "d": torch.zeros((2, 1, 100), dtype=torch.uint8)})
+    _, tensors, blocks, per_block, kv, segments = seen["args"][7:13]
+    assert tensors[0] == (0x70000, 8 * 6192 * 2 - 2064) and blocks == [8, 8, 8, 1]
+    assert per_block == [2064, 100, 100, 100] and kv == [8 * 6192, 800, 0, 100] and segments == [2, 2, 1, 2]
+    assert seen["kw"] == {"block_stride_bytes_list": [6192, 100, 100, 200]}     # the others': what an engine takes by itself
+    assert w.registrations["a"].bytes_per_block == 2064
+    w.register_kv_caches({"b": torch.zeros((2, 8, 100), dtype=torch.uint8)})
+    assert seen["kw"] == {}
+
+
+def test_a_cache_in_a_slice_does_not_register_over_a_wire():
+    class Client:
+        def register_context_batch(self, *a, **kw):
+            raise AssertionError("must not be called")
+
+    with pytest.raises(ValueError, match="this process only"):
+        _worker(Client()).register_kv_caches({"a": _Sliced()})
