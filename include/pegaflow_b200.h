@@ -577,8 +577,8 @@ typedef struct pf_kv8_batch {
   uint32_t max_blocks;
   uint32_t n_seqs;             /* at most PF_KV8_MAX_SEQS */
   const int32_t *lens;         /* [n_seqs] tokens of each sequence */
-  const int32_t *starts;       /* [n_seqs + 1]: rows starts[s] .. starts[s + 1] belong to sequence s; rows behind the
-                                  last are not read and not written.  NULL: the rows are divided evenly */
+  const int32_t *starts;       /* [n_seqs + 1]: rows starts[s] .. starts[s + 1] belong to sequence s; rows before the
+                                  first and behind the last are not read and not written.  NULL: the rows are divided evenly */
   uint32_t *status;            /* device word, or NULL */
 } pf_kv8_batch;
 #define PF_KV8_MAX_SEQS 8192
@@ -597,6 +597,7 @@ int pf_kv8_append(int device_id, const pf_kv8_cache *cache, const pf_kv8_batch *
  * p = exp(scale * q.K - lse) over the visible tokens; a row that sees nothing gives out = 0, lse = -infinity.
  * weights (may be NULL) [n_seqs][kv_heads][weights_capacity]: the sum of p over the sequence's rows and the
  * query heads of the group is added for each token, in an order that does not vary. */
+enum { PF_KV8_CLEAR_ALL = 1, PF_KV8_CLEAR_LSE = 2 };
 typedef struct pf_kv8_attention_args {
   const void *q;               /* [n_rows][q_heads][head_dim], q_heads a multiple of kv_heads */
   void *out;                   /* the same shape and type */
@@ -610,7 +611,8 @@ typedef struct pf_kv8_attention_args {
   uint32_t q_heads;
   int dtype;
   int causal;
-  int clear_tail;              /* 1: rows behind the last sequence get out = 0, lse = -infinity */
+  int clear_tail;              /* PF_KV8_CLEAR_ALL: rows of no sequence (before starts[0], behind the last one) get out = 0 and lse =
+                                  -infinity; PF_KV8_CLEAR_LSE: lse alone; 0: both stay as they are */
   float scale;
 } pf_kv8_attention_args;
 /* Workspace bytes for a call of these sizes: rows, heads, table width, weights_capacity and which of lse and weights are

@@ -240,6 +240,7 @@ class Kv8EvictArgs(C.Structure):
 KV8_BF16, KV8_F16 = 0, 1
 KV8_BAD_BLOCK, KV8_BAD_LENGTH, KV8_BAD_ROWS, KV8_STALLED = 1, 2, 4, 8
 KV8_MAX_SEQS = 8192
+KV8_CLEAR_ALL, KV8_CLEAR_LSE = 1, 2
 _sig("pf_kv8_record_bytes", sz, u32, u32, u32)
 _sig("pf_kv8_append", C.c_int, C.c_int, P(Kv8CacheDesc), P(Kv8Batch), vp, vp, C.c_int, sz, sz, sz, sz, sz, vp)
 _sig("pf_kv8_attention_workspace", C.c_int, C.c_int, P(Kv8CacheDesc), P(Kv8Batch), P(Kv8AttentionArgs), P(sz))

@@ -31,15 +31,20 @@ __global__ void __launch_bounds__(kJoinThreads) kv8_attention_join(AttnParams p,
   const int n_seqs = p.batch.n_seqs;
   const Work<kRows, kUnits> work(p, prefix);
   after_previous();
-  if (p.clear_tail) {
-    int lo, hi = 0;
-    if (n_seqs) p.batch.rows(n_seqs - 1, lo, hi);
+  if (p.clear_tail) {          // rows [0, first) and [last, n_rows) belong to no sequence
+    int first = 0, last = 0, ignored;
+    if (n_seqs) {
+      p.batch.rows(0, first, ignored);
+      p.batch.rows(n_seqs - 1, ignored, last);
+      first = min(first, last);
+    }
+    const int64_t per_row = (int64_t)p.q_heads * kDim, all = (first + p.batch.n_rows - last) * per_row;
     const int64_t id = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * kJoinThreads + threadIdx.x;
-    for (int64_t e = (int64_t)hi * p.q_heads * kDim + id; e < (int64_t)p.batch.n_rows * p.q_heads * kDim;
-         e += (int64_t)gridDim.x * gridDim.y * kJoinThreads) {
-      const int64_t row = e / (p.q_heads * kDim);
+    for (int64_t e = id; e < all; e += (int64_t)gridDim.x * gridDim.y * kJoinThreads) {
+      int64_t row = e / per_row;
+      if (row >= first) row += last - first;
       const int qh = (int)(e / kDim % p.q_heads), d = (int)(e % kDim);
-      p.out[row * p.out_row + qh * p.out_head + d] = 0;
+      if (p.clear_tail == PF_KV8_CLEAR_ALL) p.out[row * p.out_row + qh * p.out_head + d] = 0;
       if (d == 0 && p.lse) p.lse[row * p.q_heads + qh] = -INFINITY;
     }
   }
@@ -195,6 +200,7 @@ void check_args(const pf_kv8_attention_args *a, const Kv8View &c, const Kv8Batch
   if (a->q_heads == 0 || a->q_heads % c.heads || a->q_heads > 65536)
     throw Error::invalid(strf("%u query heads are not a multiple of %d KV heads", a->q_heads, c.heads));
   if (a->n_rows && b.n_seqs && a->max_query == 0) throw Error::invalid("max_query must not be 0");
+  if (a->clear_tail < 0 || a->clear_tail > PF_KV8_CLEAR_LSE) throw Error::invalid(strf("unknown clear_tail %d", a->clear_tail));
   const uint64_t rows_of_group = (uint64_t)std::min<size_t>(a->max_query, a->n_rows) * (a->q_heads / c.heads);
   if (rows_of_group > 0x3fffffffu) throw Error::invalid("too many query rows");
   if (!b.starts && b.n_seqs && a->max_query < (size_t)b.rows_each)
@@ -302,7 +308,7 @@ int pf_kv8_attention(int device_id, const pf_kv8_cache *cache, const pf_kv8_batc
     p.max_query = (int)std::min<size_t>(a.max_query, a.n_rows);
     p.row_tiles_most = std::max(1, (p.max_query * p.group + plan.rows - 1) / plan.rows);
     p.causal = a.causal != 0;
-    p.clear_tail = a.clear_tail != 0;
+    p.clear_tail = a.clear_tail;
     p.vec_q = (uintptr_t)a.q % 16 == 0 && (a.q_row_stride | a.q_head_stride) % 8 == 0;
     p.vec_out = (uintptr_t)a.out % 8 == 0 && (a.out_row_stride | a.out_head_stride) % 4 == 0;
     p.scale = a.scale;

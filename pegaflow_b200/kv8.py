@@ -180,8 +180,9 @@ class Kv8Cache:
         token lens - n + i and sees, unless ``causal=False``, the tokens up to itself.  A row that sees none
         gives 0 and lse = -inf.  max_query: the most rows of any sequence (needed with starts).  scale: head_dim ** -0.5
         unless given.  weights, float32 [sequences, kv_heads, >= longest]: each token's probability, summed over the
-        sequence's rows and the query heads of the KV head, is added in place.  Rows behind the last sequence are
-        left as they were in a given ``out``, and 0 in one that the call allocates."""
+        sequence's rows and the query heads of the KV head, is added in place.  Rows of no sequence, in front of starts[0]
+        and behind the last one, are left as they were in a given ``out``, and 0 in one that the call allocates; their
+        lse is -inf."""
         code, qs = self._rows("q", q)
         n_rows, q_heads, dim = q.shape
         if q_heads == 0 or q_heads % self.kv_heads:
@@ -202,8 +203,8 @@ class Kv8Cache:
             self._rows("out", out)
             if out.shape != q.shape or out.dtype != q.dtype:
                 _refuse(f"out ({out.dtype} {tuple(out.shape)}) and q ({q.dtype} {tuple(q.shape)}) differ")
-        elif starts is not None:
-            clear = 1
+        if starts is not None and (out is None or lse):        # what the call allocates has no row that nobody writes
+            clear = N.KV8_CLEAR_ALL if out is None else N.KV8_CLEAR_LSE
         if stream is not None:
             with self._on(stream):     # what the call allocates belongs to the stream that uses it
                 return self.attention(q, block_tables, lens, starts=starts, max_query=max_query, scale=scale, causal=causal,

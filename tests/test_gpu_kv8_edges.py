@@ -138,3 +138,48 @@ def test_caches_in_a_slice_of_a_larger_buffer_are_saved_and_loaded_alone(pf, lay
     for conn in conns:
         conn.unregister()
     eng.close()
+
+
+# ------------------------------------------------------------------------------------------------ rows of no sequence
+def leave_behind(*shapes):
+    """Fills memory that the allocator gives out next for tensors of these shapes and types, and returns it."""
+    torch.cuda.synchronize()
+    for shape, dtype in shapes:
+        keep = [torch.full(shape, 7.0, dtype=dtype, device="cuda") for _ in range(64)]
+        del keep
+    torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("given", [False, True])
+@pytest.mark.parametrize("before,counts,behind", [(3, [1, 1], 0), (0, [1, 1], 3), (2, [3, 0, 2], 2), (5, [], 0), (4, [0, 0], 1), (1, [40, 3], 2)])
+def test_rows_in_front_of_and_behind_the_sequences(pf, before, counts, behind, given):
+    """0 and -infinity where the call allocates the output, left as they were in a given one; lse is the call's own always."""
+    n_seqs, rows = len(counts), before + sum(counts) + behind
+    lens = [70, 33, 50][:n_seqs]
+    blocks, tables = make_tables(lens, 16, 220) if n_seqs else (4, torch.zeros((0, 2), dtype=torch.int32))
+    cache = make_cache(pf, blocks, 16, 2, 64, 221)
+    q = torch.randn((rows, 8, 64), generator=gen(222), device="cuda").half()
+    none = torch.ones(rows, dtype=torch.bool, device="cuda")
+    none[before:before + sum(counts)] = False
+    q[none] = math.nan
+    starts = [before + n for n in starts_of(counts)]
+    out = torch.full_like(q, 3.0) if given else None
+    leave_behind((q.shape, q.dtype), ((rows, 8), torch.float32))
+    got, lse = cache.attention(q, tables.cuda(), ints(lens), starts=ints(starts), max_query=max([1] + counts), lse=True, out=out)
+    cache.check()
+    assert (got[none] == (3.0 if given else 0.0)).all() and torch.isneginf(lse[none]).all()
+    for s, n in enumerate(counts):
+        if n:
+            a = slice(starts[s], starts[s] + n)
+            close(cache, q[a], got[a], lse[a], None, None, plain(cache, q[a], tables[s].tolist(), lens[s], 0.125), lens[s])
+
+
+def test_append_takes_the_rows_behind_its_first_start(pf):
+    """Rows in front of starts[0], a batch's other part, are not read: their NaN reach nothing."""
+    cache, same = make_cache(pf, 6, 16, 2, 64, 223), make_cache(pf, 6, 16, 2, 64, 223)
+    x = torch.randn((9, 2, 64), generator=gen(224), device="cuda").half()
+    x[:4] = math.nan
+    cache.append(x, -x, ints([[1], [4]]), ints([3, 0]), starts=ints([4, 6, 9]))
+    same.append(x[4:], -x[4:], ints([[1], [4]]), ints([3, 0]), starts=ints([0, 2, 5]))
+    cache.check()
+    assert torch.equal(cache.tensor, same.tensor)

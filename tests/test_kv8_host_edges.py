@@ -1,6 +1,11 @@
 """Host side of the 8-bit KV cache at the edges: registration of caches in slices, refusals (no GPU needed)."""
+import ctypes as C
+
 import pytest
 import torch
+
+from pegaflow_b200 import _native as N
+from tests.test_kv8_host import PTR, attention, batch, cache, refused
 
 
 class _Sliced:
@@ -48,3 +53,8 @@ def test_a_cache_in_a_slice_does_not_register_over_a_wire():
 
     with pytest.raises(ValueError, match="this process only"):
         _worker(Client()).register_kv_caches({"a": _Sliced()})
+
+
+def test_clear_tail_is_one_of_its_values():
+    for bad in (-1, 3):
+        refused(N.lib.pf_kv8_attention(0, C.byref(cache()), C.byref(batch()), C.byref(attention(clear_tail=bad)), PTR, 1 << 40, None), "clear_tail")
