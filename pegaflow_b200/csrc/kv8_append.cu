@@ -43,6 +43,8 @@ Kv8Batch kv8_check_batch(const pf_kv8_batch *b, size_t n_rows) {
   if (b->n_seqs > PF_KV8_MAX_SEQS)
     throw Error::invalid(strf("%u sequences exceed the limit of %d", b->n_seqs, PF_KV8_MAX_SEQS));
   if (n_rows > 0x7fffffffu) throw Error::invalid(strf("%zu rows exceed 2^31 - 1", n_rows));
+  if (!b->n_seqs && !b->starts && n_rows)
+    throw Error::invalid(strf("%zu rows cannot be divided evenly among 0 sequences: row starts are needed", n_rows));
   if (b->n_seqs) {
     if (!b->block_tables || !b->lens) throw Error::invalid("null block_tables or lens");
     if (b->max_blocks == 0 || b->max_blocks > 0x800000u)

@@ -183,3 +183,19 @@ def test_append_takes_the_rows_behind_its_first_start(pf):
     same.append(x[4:], -x[4:], ints([[1], [4]]), ints([3, 0]), starts=ints([0, 2, 5]))
     cache.check()
     assert torch.equal(cache.tensor, same.tensor)
+
+
+def test_rows_without_a_sequence_are_refused(pf):
+    """Rows cannot be divided among no sequences; with starts they are rows of no sequence."""
+    cache = pf.Kv8Cache(4, 16, 2, 64)
+    x = torch.ones((3, 2, 64), dtype=torch.bfloat16, device="cuda")
+    none, nothing = torch.zeros((0, 2), dtype=torch.int32, device="cuda"), ints([])
+    for call in (lambda: cache.attention(x, none, nothing), lambda: cache.attention(x, none, nothing, lse=True, out=torch.empty_like(x)),
+                 lambda: cache.append(x, x, none, nothing)):
+        with pytest.raises(pf.PegaflowInvalidArgument, match="evenly"):
+            call()
+    assert cache.attention(x[:0], none, nothing).shape == (0, 2, 64)
+    cache.append(x[:0], x[:0], none, nothing)
+    cache.append(x, x, none, nothing, starts=ints([0]))
+    cache.check()
+    assert (cache.tensor == 0).all()

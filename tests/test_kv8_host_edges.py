@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from pegaflow_b200 import _native as N
-from tests.test_kv8_host import PTR, attention, batch, cache, refused
+from tests.test_kv8_host import PTR, attention, batch, cache, evict, refused
 
 
 class _Sliced:
@@ -58,3 +58,14 @@ def test_a_cache_in_a_slice_does_not_register_over_a_wire():
 def test_clear_tail_is_one_of_its_values():
     for bad in (-1, 3):
         refused(N.lib.pf_kv8_attention(0, C.byref(cache()), C.byref(batch()), C.byref(attention(clear_tail=bad)), PTR, 1 << 40, None), "clear_tail")
+
+
+def test_rows_are_not_divided_among_no_sequences():
+    c, none = C.byref(cache()), C.byref(batch(n_seqs=0, starts=None))
+    need = N.sz()
+    refused(N.lib.pf_kv8_append(0, c, none, PTR, PTR, 0, 2, 128, 64, 128, 64, None), "evenly among 0")
+    refused(N.lib.pf_kv8_attention_workspace(0, c, none, C.byref(attention()), C.byref(need)), "evenly among 0")
+    refused(N.lib.pf_kv8_attention(0, c, none, C.byref(attention(clear_tail=1)), PTR, 1 << 40, None), "evenly among 0")
+    assert N.lib.pf_kv8_append(0, c, none, None, None, 0, 0, 128, 64, 128, 64, None) == 0        # no rows: nothing to do
+    assert N.lib.pf_kv8_append(0, c, C.byref(batch(n_seqs=0)), PTR, PTR, 0, 2, 128, 64, 128, 64, None) == 0
+    assert N.lib.pf_kv8_evict(0, c, none, C.byref(evict()), None) == 0
