@@ -31,9 +31,10 @@ __global__ void __launch_bounds__(kJoinThreads) kv8_attention_join(AttnParams p,
   const int n_seqs = p.batch.n_seqs;
   const Work<kRows, kUnits> work(p, prefix);
   after_previous();
-  if (p.clear_tail) {          // rows [0, first) and [last, n_rows) belong to no sequence
+  const bool none = work.total() == 0;         // no rows, or row starts that claim more than there can be: no row is computed
+  if (p.clear_tail || (none && p.weights)) {   // rows [0, first) and [last, n_rows) belong to no sequence
     int first = 0, last = 0, ignored;
-    if (n_seqs) {
+    if (!none) {
       p.batch.rows(0, first, ignored);
       p.batch.rows(n_seqs - 1, ignored, last);
       first = min(first, last);
@@ -163,6 +164,8 @@ struct Plan {
   int n_ctas, rows;     // rows of a tile, and of a part
   size_t part_o, part_ml, lse, scores, bytes;   // offsets in the workspace
   int score_tokens;     // 0: scores are not kept
+  int row_tiles;        // of a sequence, at most
+  uint32_t units;       // of all its rows, at most
 };
 
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
@@ -179,6 +182,14 @@ Plan make_plan(int device_id, const Kv8View &c, const Kv8Batch &b, const pf_kv8_
   plan.rows = kv8_few_rows(c.dim, (int64_t)rows);
   plan.wide = plan.rows == 0;
   if (plan.wide) plan.rows = kv8_wide_plan(c.dim).rows;
+  // As the kernels count them: row tiles of all sequences x (units of tokens and a segment's cost) x heads.
+  const uint64_t unit = plan.wide ? kv8_wide_plan(c.dim).tokens : 128;
+  const uint64_t units = (((uint64_t)b.max_blocks << c.block_log2) / unit + 1 + Work<4, 128>::kCost) *
+                         (((uint64_t)a.n_rows * group) / plan.rows + b.n_seqs) * c.heads;
+  const uint64_t row_tiles = std::max<uint64_t>(1, (rows + plan.rows - 1) / plan.rows);
+  if (units > 0xffffffffull || row_tiles * b.n_seqs > 1u << 29) throw Error::invalid("too many query rows for tables of this width: split the call");
+  plan.units = (uint32_t)units;
+  plan.row_tiles = (int)row_tiles;
   plan.n_ctas = kv8_sm_count(device_id) * (plan.wide ? 1 : kv8_few_ctas(c.dim, plan.rows));
   const size_t slots = 2 * (size_t)plan.n_ctas * plan.rows;
   plan.part_o = 0;
@@ -306,7 +317,8 @@ int pf_kv8_attention(int device_id, const pf_kv8_cache *cache, const pf_kv8_batc
     p.q_heads = (int)a.q_heads;
     p.group = (int)a.q_heads / c.heads;
     p.max_query = (int)std::min<size_t>(a.max_query, a.n_rows);
-    p.row_tiles_most = std::max(1, (p.max_query * p.group + plan.rows - 1) / plan.rows);
+    p.row_tiles_most = plan.row_tiles;
+    p.units_most = plan.units;
     p.causal = a.causal != 0;
     p.clear_tail = a.clear_tail;
     p.vec_q = (uintptr_t)a.q % 16 == 0 && (a.q_row_stride | a.q_head_stride) % 8 == 0;

@@ -23,6 +23,7 @@ struct AttnParams {
   int w_capacity;
   int q_heads, group, max_query;
   int row_tiles_most;   // of a sequence
+  uint32_t units_most;  // units (see Work) that n_rows rows can be, however they fall on the sequences
   int causal, clear_tail, vec_q, vec_out;
   float scale;
   // Partial results: slot 2 c + k of CTA c (k = 0: the segment that its range starts in, 1: the one that it ends in).
@@ -76,7 +77,8 @@ struct Seq {
 // The units of all (sequence, row tile) entries in order, kCost of them in front of each head's for what a segment costs at its
 // beginning and end, as sums before every chunk of entries (one, unless there are more
 // than kMost).  Every CTA of every kernel computes them for itself: lens stay on the device, and no launch and no
-// workspace is spent on it.
+// workspace is spent on it.  Row starts that fall and rise again can claim rows more than once: sums stay at the largest number
+// instead of wrapping, and where they exceed what the call's rows can be there is no work at all.
 template <int kRows, int kUnit, bool kWhole = false>
 struct Work {
   using SeqT = Seq<kRows, kUnit, kWhole>;
@@ -90,6 +92,10 @@ struct Work {
   static __host__ size_t bytes(int n_seqs, int row_tiles_most) {
     const int entries = n_seqs * row_tiles_most, chunk = chunk_of(entries);
     return ((size_t)(entries + chunk - 1) / chunk + 1) * 4;
+  }
+  static __device__ uint32_t add(uint32_t a, uint32_t b) {
+    const uint32_t sum = a + b;
+    return sum < a ? 0xffffffffu : sum;
   }
   static __device__ int seq_of(const AttnParams &p, int e) { return p.row_tiles_most == 1 ? e : e / p.row_tiles_most; }
   __device__ uint32_t units_of(const AttnParams &p, int e) const {       // of one head
@@ -107,25 +113,25 @@ struct Work {
     for (int c0 = 0; c0 < chunks; c0 += blockDim.x) {
       const int c = c0 + threadIdx.x;
       uint32_t mine = 0;
-      for (int e = c * chunk; c < chunks && e < min((c + 1) * chunk, entries); ++e) mine += units_of(p, e) * (uint32_t)p.cache.heads;
+      for (int e = c * chunk; c < chunks && e < min((c + 1) * chunk, entries); ++e) mine = add(mine, units_of(p, e) * (uint32_t)p.cache.heads);
       uint32_t x = mine;
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) {
         const uint32_t y = __shfl_up_sync(0xffffffffu, x, d);
-        if (lane >= d) x += y;
+        if (lane >= d) x = add(x, y);
       }
       if (lane == 31) warp_sum[warp] = x;
       __syncthreads();
       uint32_t before = base, all = 0;
       for (int w = 0; w < n_warps; ++w) {
-        if (w < warp) before += warp_sum[w];
-        all += warp_sum[w];
+        if (w < warp) before = add(before, warp_sum[w]);
+        all = add(all, warp_sum[w]);
       }
       if (c < chunks) prefix[c] = before + x - mine;
-      base += all;
+      base = add(base, all);
       __syncthreads();
     }
-    if (threadIdx.x == 0) prefix[chunks] = base;
+    if (threadIdx.x == 0) prefix[chunks] = base > p.units_most ? 0 : base;
     __syncthreads();
   }
   __device__ uint32_t total() const { return prefix[chunks]; }
@@ -146,7 +152,7 @@ struct Segment {
     int e = lo * work.chunk;
     begin = work.prefix[lo];
     units = work.units_of(p, e);
-    while (u - begin >= units * (uint32_t)p.cache.heads) {
+    while (e + 1 < work.entries && u - begin >= units * (uint32_t)p.cache.heads) {
       begin += units * (uint32_t)p.cache.heads;
       units = work.units_of(p, ++e);
     }
@@ -211,7 +217,7 @@ void kv8_few_launch(const AttnParams &p, int rows, bool bf16, cudaStream_t strea
 void kv8_weights_launch(const AttnParams &p, bool bf16, int n_sms, cudaStream_t stream);
 // Query rows by the hundred (kv8_attention_wide.cu).
 struct WidePlan {
-  int rows, threads;
+  int rows, tokens, threads;
   size_t smem;
 };
 WidePlan kv8_wide_plan(int dim);

@@ -600,7 +600,7 @@ static_assert(Layout<256>::end <= Layout<128>::end && Layout<64>::end <= Layout<
 
 WidePlan kv8_wide_plan(int dim) {
   const int end = dim == 64 ? Layout<64>::end : dim == 128 ? Layout<128>::end : Layout<256>::end;
-  return WidePlan{kGroupRows * groups_of(dim), threads_of(dim), 1024 + (size_t)end + sizeof(Shared)};
+  return WidePlan{kGroupRows * groups_of(dim), tokens_of(dim), threads_of(dim), 1024 + (size_t)end + sizeof(Shared)};
 }
 
 void kv8_wide_launch(const AttnParams &p, bool bf16, cudaStream_t stream) {

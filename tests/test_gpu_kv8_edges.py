@@ -199,3 +199,19 @@ def test_rows_without_a_sequence_are_refused(pf):
     cache.append(x, x, none, nothing, starts=ints([0]))
     cache.check()
     assert (cache.tensor == 0).all()
+
+
+# ------------------------------------------------------------------------------------------------ sizes
+@pytest.mark.parametrize("seqs,n,width,heads", [(64, 512, 64, 2), (8192, 4096, 8192, 64)])
+def test_row_starts_that_fall_again_and_again_do_no_harm(pf, seqs, n, width, heads):
+    """Starts 0, n, 0, n, ... claim all rows for every second sequence, more work than these rows can be (in the second
+    case more than 32 bits count): no row is computed, and the call says why."""
+    cache = make_cache(pf, 8, 16, heads, 64, 260)
+    q = torch.randn((n, 8 * heads, 64), generator=gen(261), device="cuda").half()
+    tables = ints([[1, 2]]).repeat(1, width // 2).expand(seqs, width)
+    lens = torch.full((seqs,), 16 * width, dtype=torch.int32, device="cuda")
+    starts = ints([0, n] * (seqs // 2) + [0])
+    out, lse = cache.attention(q, tables, lens, starts=starts, max_query=n, causal=False, lse=True)
+    with pytest.raises(pf.PegaflowInvalidArgument, match="row starts"):
+        cache.check()
+    assert (out == 0).all() and torch.isneginf(lse).all()

@@ -69,3 +69,10 @@ def test_rows_are_not_divided_among_no_sequences():
     assert N.lib.pf_kv8_append(0, c, none, None, None, 0, 0, 128, 64, 128, 64, None) == 0        # no rows: nothing to do
     assert N.lib.pf_kv8_append(0, c, C.byref(batch(n_seqs=0)), PTR, PTR, 0, 2, 128, 64, 128, 64, None) == 0
     assert N.lib.pf_kv8_evict(0, c, none, C.byref(evict()), None) == 0
+
+
+def test_more_row_tiles_than_can_be_numbered_are_refused():
+    rows = 1 << 24
+    a = attention(n_rows=rows, max_query=rows)
+    c, b = cache(), batch(n_seqs=8192)
+    refused(N.lib.pf_kv8_attention(0, C.byref(c), C.byref(b), C.byref(a), PTR, 1 << 40, None), "too many query rows")
