@@ -182,7 +182,7 @@ Plan make_plan(int device_id, const Kv8View &c, const Kv8Batch &b, const pf_kv8_
   plan.rows = kv8_few_rows(c.dim, (int64_t)rows);
   plan.wide = plan.rows == 0;
   if (plan.wide) plan.rows = kv8_wide_plan(c.dim).rows;
-  // As the kernels count them: row tiles of all sequences x (units of tokens and a segment's cost) x heads.
+  // As the kernels count them, in 32 bits: row tiles of all sequences x (units of tokens and a segment's cost) x heads.
   const uint64_t unit = plan.wide ? kv8_wide_plan(c.dim).tokens : 128;
   const uint64_t units = (((uint64_t)b.max_blocks << c.block_log2) / unit + 1 + Work<4, 128>::kCost) *
                          (((uint64_t)a.n_rows * group) / plan.rows + b.n_seqs) * c.heads;
@@ -216,10 +216,6 @@ void check_args(const pf_kv8_attention_args *a, const Kv8View &c, const Kv8Batch
   if (rows_of_group > 0x3fffffffu) throw Error::invalid("too many query rows");
   if (!b.starts && b.n_seqs && a->max_query < (size_t)b.rows_each)
     throw Error::invalid(strf("max_query=%zu is below the %d rows of each sequence", a->max_query, b.rows_each));
-  // units are counted in 32 bits: (segments) x (units of a segment and its cost), summed over the sequences
-  const uint64_t units = ((uint64_t)b.max_blocks << c.block_log2) / 64 + 1 + 4;
-  const uint64_t tiles = ((uint64_t)a->n_rows * (a->q_heads / c.heads) + 3) / 4 + b.n_seqs;
-  if (units * tiles > 0xffffffffull / c.heads) throw Error::invalid("too many query rows for tables of this width: split the call");
 }
 
 template <int kDim, int kRows, int kUnits, bool kBf16>

@@ -215,3 +215,17 @@ def test_row_starts_that_fall_again_and_again_do_no_harm(pf, seqs, n, width, hea
     with pytest.raises(pf.PegaflowInvalidArgument, match="row starts"):
         cache.check()
     assert (out == 0).all() and torch.isneginf(lse).all()
+
+
+def test_prompts_over_wide_tables_are_counted_by_their_own_tiles(pf):
+    """8 prompts of 300 rows with tables for 2^24 tokens, of which they use 400."""
+    size, heads, group, dim, rows = 16, 2, 16, 64, 300
+    lens = [400] * 8
+    blocks, tables = make_tables(lens, size, 265, width=1 << 20)
+    cache = make_cache(pf, blocks, size, heads, dim, 263)
+    q = torch.randn((8 * rows, heads * group, dim), generator=gen(264), device="cuda").bfloat16()
+    out, lse = cache.attention(q, tables.cuda(), ints(lens), lse=True)
+    cache.check()
+    for s in (0, 7):
+        a = slice(s * rows, (s + 1) * rows)
+        close(cache, q[a], out[a], lse[a], None, None, plain(cache, q[a], tables[s].tolist(), lens[s], 0.125), lens[s])

@@ -76,3 +76,17 @@ def test_more_row_tiles_than_can_be_numbered_are_refused():
     a = attention(n_rows=rows, max_query=rows)
     c, b = cache(), batch(n_seqs=8192)
     refused(N.lib.pf_kv8_attention(0, C.byref(c), C.byref(b), C.byref(a), PTR, 1 << 40, None), "too many query rows")
+
+
+@pytest.mark.parametrize("rows,q_heads,max_blocks,fits", [(8 * 10240, 128, 8192, True), (8 * 10240, 128, 1 << 20, False), (8, 128, 1 << 20, True)])
+def test_work_is_counted_in_the_tiles_that_the_rows_go_in(rows, q_heads, max_blocks, fits):
+    """8 prompts of 10240 rows, 128 query and 8 KV heads: tables for 131072 tokens are 80 tiles of 256 rows x 1029 units of a head,
+    not 20480 of 4 rows.  Where there is no device the call ends behind its checks, with that error."""
+    need = N.sz()
+    c = cache(kv_heads=8, head_dim=128, block_stride_bytes=16 * 8 * 128 + 32, kv_stride_bytes=8 * (16 * 8 * 128 + 32))
+    a = attention(n_rows=rows, max_query=rows // 8, q_heads=q_heads)
+    status = N.lib.pf_kv8_attention_workspace(0, C.byref(c), C.byref(batch(n_seqs=8, max_blocks=max_blocks)), C.byref(a), C.byref(need))
+    if fits:
+        assert status == (0 if torch.cuda.is_available() else 4)
+    else:
+        refused(status, "too many query rows")
