@@ -8,7 +8,10 @@ buffer its records alone are registered, with an engine of the same process; ``c
 all bytes from one block to the next.
 
 The calls only enqueue work, on the current torch stream of the cache's device unless ``stream`` (a cudaStream_t value)
-says otherwise, and may be captured into a CUDA graph.  Block tables, lengths and row starts are int32 tensors on
+says otherwise, and may be captured into a CUDA graph.  Work on a given stream comes behind what the current stream holds at
+the call, and the memory of the call's tensors and outputs is not given out again before either stream is through with
+them; to use the outputs, the current stream has to wait for the given one.  (A stream that is being captured while the current
+one is not cannot wait for it: order that capture beforehand.)  Block tables, lengths and row starts are int32 tensors on
 the device.  What the host cannot check (block ids, lengths, row starts) the kernels check: they leave the access out and
 set a bit that ``check()`` raises for.  None of the calls has a backward pass.
 """
@@ -152,8 +155,29 @@ class Kv8Cache:
             _refuse(f"{name}: a float32 tensor [{n}, {self.kv_heads}, tokens] on {self.device} with a dense last dimension is "
                     f"needed, not {t.dtype} {tuple(t.shape)} on {t.device}")
 
-    def _on(self, stream):
-        return torch.cuda.stream(torch.cuda.ExternalStream(stream, device=self.device))
+    def _hand_over(self, stream, *tensors):
+        """The given stream as torch's, behind the current one and known to the allocator as a user of the call's tensors;
+        None where it is the current one."""
+        current = torch.cuda.current_stream(self.device)
+        if stream == current.cuda_stream:
+            return None
+        given = torch.cuda.ExternalStream(stream, device=self.device)
+        with torch.cuda.stream(given):
+            alone = torch.cuda.is_current_stream_capturing()
+        with torch.cuda.stream(current):
+            alone = alone and not torch.cuda.is_current_stream_capturing()
+        if not alone:
+            given.wait_stream(current)
+        for t in (self.tensor, self._status) + tensors:
+            if t is not None:
+                t.record_stream(given)
+        return given
+
+    def _hand_back(self, outputs):
+        """What a call on a given stream has allocated is used on the current one."""
+        current = torch.cuda.current_stream(self.device)
+        for t in outputs:
+            t.record_stream(current)
 
     # ------------------------------------------------------------------ operators
     def append(self, k, v, block_tables, lens, *, starts=None, stream: Optional[int] = None) -> None:
@@ -168,6 +192,8 @@ class Kv8Cache:
         batch = self._batch(block_tables, lens, starts)
         if stream is None:
             stream = _stream_of(self._index)
+        else:
+            self._hand_over(stream, k, v, block_tables, lens, starts)
         N.check(_append(self._index, self._desc_ref, _byref(batch), k.data_ptr(), v.data_ptr(), code, k.shape[0], ks[0], ks[1],
                         vs[0], vs[1], stream))
 
@@ -206,9 +232,13 @@ class Kv8Cache:
         if starts is not None and (out is None or lse):        # what the call allocates has no row that nobody writes
             clear = N.KV8_CLEAR_ALL if out is None else N.KV8_CLEAR_LSE
         if stream is not None:
-            with self._on(stream):     # what the call allocates belongs to the stream that uses it
-                return self.attention(q, block_tables, lens, starts=starts, max_query=max_query, scale=scale, causal=causal,
-                                      weights=weights, lse=lse, out=out)
+            given = self._hand_over(stream, q, block_tables, lens, starts, weights, out)
+            if given is not None:
+                with torch.cuda.stream(given):     # what the call allocates belongs to the stream that uses it
+                    result = self.attention(q, block_tables, lens, starts=starts, max_query=max_query, scale=scale, causal=causal,
+                                            weights=weights, lse=lse, out=out)
+                self._hand_back(result if lse else (result,))
+                return result
         if out is None:
             out = torch.empty(q.shape, dtype=q.dtype, device=self.device)
         os = out.stride()
@@ -249,8 +279,12 @@ class Kv8Cache:
             _refuse(f"dst_tables {tuple(dst_tables.shape)} does not hold {keep} tokens of {n} sequences")
         self._per_token("weights", weights, n)
         if stream is not None:
-            with self._on(stream):
-                return self.evict(block_tables, lens, weights, dst_tables, keep, recent=recent)
+            given = self._hand_over(stream, block_tables, lens, weights, dst_tables)
+            if given is not None:
+                with torch.cuda.stream(given):
+                    result = self.evict(block_tables, lens, weights, dst_tables, keep, recent=recent)
+                self._hand_back(result)
+                return result
         ws, tokens = weights.stride(), weights.shape[2]
         capacity = max(tokens, keep)
         new_lens = torch.empty(n, dtype=_INT32, device=self.device)

@@ -229,3 +229,108 @@ def test_prompts_over_wide_tables_are_counted_by_their_own_tiles(pf):
     for s in (0, 7):
         a = slice(s * rows, (s + 1) * rows)
         close(cache, q[a], out[a], lse[a], None, None, plain(cache, q[a], tables[s].tolist(), lens[s], 0.125), lens[s])
+
+
+# ------------------------------------------------------------------------------------------------ streams
+LONG = 200_000_000       # cycles, a tenth of a second: longer than the host takes for everything behind it
+
+
+def operators(cache, x, t, n, w):
+    """Each operator as a call with `stream`, on tensors that the call alone holds: temporaries of the current stream."""
+    starts, dst = ints([0, 1, 2]), ints([[7], [8]])
+    return {
+        "append": lambda s: cache.append(x.half(), (-x).half(), t + 0, n + 0, starts=starts + 0, stream=s),
+        "attention": lambda s: cache.attention(x.repeat(1, 2, 1).half(), t + 0, n + 0, starts=starts + 0, max_query=1, weights=w, lse=True, stream=s),
+        "evict": lambda s: cache.evict(t + 0, n + 0, w + 0, dst + 0, 9, recent=2, stream=s),
+    }
+
+
+def overwrite():
+    """What the allocator gives out next for tensors like the calls' is full of ones."""
+    for like in ((2, 2, 64), (2, 4, 64), (2, 2, 30), (2, 2), (2,), (3,), (2, 1)):
+        for dtype in (torch.float32, torch.float16, torch.int32):
+            keep = [torch.full(like, 1, dtype=dtype, device="cuda") for _ in range(4)]
+            del keep
+
+
+@pytest.mark.parametrize("late", ["caller", "stream"])
+@pytest.mark.parametrize("name", ["append", "attention", "evict"])
+def test_a_given_stream_takes_temporaries_of_the_current_one(pf, name, late):
+    """The work on `stream` comes behind what the current stream was given before the call, and the call's tensors are not
+    given out again before it has read them: whichever of the two streams is far behind."""
+    results = []
+    for own_stream in (False, True):
+        cache = make_cache(pf, 9, 16, 2, 64, 230)
+        x = torch.randn((2, 2, 64), generator=gen(231), device="cuda")
+        t, n, w = ints([[1, 2], [3, 4]]), ints([20, 17]), torch.rand((2, 2, 30), generator=gen(232), device="cuda")
+        call = operators(cache, x, t, n, w)[name]
+        side = torch.cuda.Stream()
+        overwrite()
+        torch.cuda.synchronize()
+        if own_stream:
+            with torch.cuda.stream(side if late == "stream" else torch.cuda.current_stream()):
+                torch.cuda._sleep(LONG)
+            got = call(side.cuda_stream)
+            overwrite()
+        else:
+            got = call(None)
+        torch.cuda.synchronize()
+        cache.check()
+        results.append((cache.tensor.clone(), w.clone(), got if isinstance(got, tuple) else ()))
+    (a, wa, oa), (b, wb, ob) = results
+    assert torch.equal(a, b) and torch.equal(wa, wb) and len(oa) == len(ob)
+    assert all(torch.equal(p, q) for p, q in zip(oa, ob))
+
+
+def test_outputs_made_on_a_given_stream_outlive_their_use_on_the_current_one(pf):
+    """The current stream, which waits for the other one, still reads an output after its last name is gone."""
+    cache = make_cache(pf, 9, 16, 2, 64, 233)
+    q = torch.randn((2, 8, 64), generator=gen(234), device="cuda").half()
+    t, n = ints([[1, 2], [3, 4]]), ints([20, 17])
+    want = cache.attention(q, t, n)
+    side = torch.cuda.Stream()
+
+    def others():
+        with torch.cuda.stream(side):
+            keep = [torch.full(q.shape, 1, dtype=q.dtype, device="cuda") for _ in range(4)]
+            del keep
+
+    others()                                   # what is loaded at its first use waits for the whole device
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    got = cache.attention(q, t, n, stream=side.cuda_stream)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda._sleep(LONG)
+    copy = got.clone()
+    del got
+    others()
+    torch.cuda.synchronize()
+    assert torch.equal(copy, want)
+
+
+def test_a_given_stream_joins_the_capture_of_the_current_one(pf):
+    """Calls on another stream while the current one is captured: they become part of the graph, which the caller joins; a stream
+    that is captured alone takes calls too."""
+    cache = make_cache(pf, 9, 16, 2, 64, 240)
+    q = torch.randn((2, 8, 64), generator=gen(241), device="cuda").half()
+    t, n = ints([[1, 2], [3, 4]]), ints([20, 17])
+    want = cache.attention(q, t, n)
+    side, torch_graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(torch_graph):
+        got = cache.attention(q + 0, t, n, stream=side.cuda_stream)
+        torch.cuda.current_stream().wait_stream(side)
+        got = got + 0
+    alone = torch.cuda.CUDAGraph()
+    capturing, current = torch.cuda.Stream(), torch.cuda.current_stream()
+    out = torch.zeros_like(q)
+    with torch.cuda.graph(alone, stream=capturing):
+        with torch.cuda.stream(current):
+            handle = capturing.cuda_stream
+            cache.attention(q, t, n, out=out, stream=handle)
+    for _ in range(2):
+        torch_graph.replay()
+        alone.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want) and torch.equal(out, want)
+        got.zero_(), out.zero_()
