@@ -39,7 +39,8 @@ def _refuse(text: str):
 
 class Kv8Cache:
     def __init__(self, num_blocks: int, block_size: int, kv_heads: int, head_dim: int, device="cuda"):
-        """A cache of zeros.  block_size 16, 32, 64 or 128 tokens, head_dim 64, 128 or 256."""
+        """A cache of zeros, there when the constructor returns (it waits for the device's current stream, like
+        ``from_tensor``).  block_size 16, 32, 64 or 128 tokens, head_dim 64, 128 or 256."""
         record = self.record_bytes(block_size, kv_heads, head_dim)
         self._bind(torch.zeros((2, num_blocks, record), dtype=torch.uint8, device=device), block_size, kv_heads, head_dim)
 
@@ -80,6 +81,10 @@ class Kv8Cache:
         self._desc = N.Kv8CacheDesc(t.data_ptr(), block_stride, t.stride(0), t.shape[1], block_size, kv_heads, head_dim)
         self._desc_ref = _byref(self._desc)
         self._status = torch.zeros(1, dtype=torch.int32, device=t.device)
+        # any stream may be the first to use the cache: the status, which nobody else can wait for, is there before that
+        with torch.cuda.device(t.device):
+            if not torch.cuda.is_current_stream_capturing():
+                torch.cuda.current_stream().synchronize()
         self._status_ptr = self._status.data_ptr()
         self._workspaces = {}      # sizes of a call -> workspace bytes
         n = kv_heads * block_size * head_dim

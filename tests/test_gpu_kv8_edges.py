@@ -334,3 +334,22 @@ def test_a_given_stream_joins_the_capture_of_the_current_one(pf):
         torch.cuda.synchronize()
         assert torch.equal(got, want) and torch.equal(out, want)
         got.zero_(), out.zero_()
+
+
+def test_a_new_cache_is_ready_for_every_stream(pf):
+    """Its zeros and its status are there when the constructor returns, however far behind the current stream is."""
+    side = torch.cuda.Stream()
+    x = torch.ones((1, 2, 64), dtype=torch.float16, device="cuda")
+    t, n = ints([[9]]), ints([0])
+    warm = pf.Kv8Cache(4, 16, 2, 64)
+    del warm
+    torch.cuda.synchronize()
+    torch.cuda._sleep(LONG)
+    cache = pf.Kv8Cache(4, 16, 2, 64)
+    with torch.cuda.stream(side):
+        cache.append(x, x, t, n)               # a block that is not there
+    side.synchronize()
+    torch.cuda.synchronize()
+    with pytest.raises(pf.PegaflowInvalidArgument, match="block id"):
+        cache.check()
+    assert (cache.tensor == 0).all()
