@@ -13,7 +13,7 @@ the call, and the memory of the call's tensors and outputs is not given out agai
 them; to use the outputs, the current stream has to wait for the given one.  (A stream that is being captured while the current
 one is not cannot wait for it: order that capture beforehand.)  Block tables, lengths and row starts are int32 tensors on
 the device.  What the host cannot check (block ids, lengths, row starts) the kernels check: they leave the access out and
-set a bit that ``check()`` raises for.  None of the calls has a backward pass.
+set a bit that ``check()`` raises for.  None of the calls has a backward pass or a forward-mode rule: tensors that carry a derivative are refused.
 """
 from __future__ import annotations
 
@@ -21,6 +21,7 @@ import ctypes as C
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native as N
 
@@ -31,6 +32,13 @@ _byref = C.byref
 _stream_of = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 _append, _attention, _attention_workspace, _evict = (N.lib.pf_kv8_append, N.lib.pf_kv8_attention,
                                                      N.lib.pf_kv8_attention_workspace, N.lib.pf_kv8_evict)
+
+
+def _no_derivative(name, t):
+    """Refuses a tensor that autograd would have to know of: neither mode has a rule for these calls."""
+    if (t.requires_grad and torch.is_grad_enabled()) or \
+            (getattr(forward_ad, "_current_level", 0) >= 0 and forward_ad.unpack_dual(t).tangent is not None):
+        _refuse(f"{name} requires a gradient or carries a tangent: the 8-bit cache has no backward pass and no forward-mode rule")
 
 
 def _refuse(text: str):
@@ -150,8 +158,7 @@ class Kv8Cache:
             _refuse(f"{name}: shape {tuple(shape)} does not fit kv_heads={self.kv_heads}, head_dim={self.head_dim}")
         if strides[2] != 1:
             _refuse(f"{name}: the last dimension must be dense")
-        if t.requires_grad and torch.is_grad_enabled():
-            _refuse(f"{name} requires a gradient: the 8-bit cache has no backward pass")
+        _no_derivative(name, t)
         return code, strides
 
     def _per_token(self, name, t, n):
@@ -159,6 +166,7 @@ class Kv8Cache:
                 t.shape[1] != self.kv_heads or (t.stride(2) != 1 and t.shape[2] > 1):
             _refuse(f"{name}: a float32 tensor [{n}, {self.kv_heads}, tokens] on {self.device} with a dense last dimension is "
                     f"needed, not {t.dtype} {tuple(t.shape)} on {t.device}")
+        _no_derivative(name, t)
 
     def _hand_over(self, stream, *tensors):
         """The given stream as torch's, behind the current one and known to the allocator as a user of the call's tensors;

@@ -353,3 +353,30 @@ def test_a_new_cache_is_ready_for_every_stream(pf):
     with pytest.raises(pf.PegaflowInvalidArgument, match="block id"):
         cache.check()
     assert (cache.tensor == 0).all()
+
+
+# ------------------------------------------------------------------------------------------------ refusals
+def test_tangents_and_gradients_are_refused(pf):
+    """There is neither a backward pass nor a forward-mode rule: nothing that carries a derivative is taken."""
+    import torch.autograd.forward_ad as fwad
+
+    cache = pf.Kv8Cache(6, 16, 2, 64)
+    t, n, dst = ints([[1, 2]]), ints([20]), ints([[3]])
+    x, w = torch.zeros((1, 2, 64), dtype=torch.bfloat16, device="cuda"), torch.zeros((1, 2, 32), device="cuda")
+    calls = [lambda x, w: cache.append(x, torch.zeros_like(x), t, n), lambda x, w: cache.append(torch.zeros_like(x), x, t, n),
+             lambda x, w: cache.attention(x, t, n), lambda x, w: cache.attention(torch.zeros_like(x), t, n, out=x),
+             lambda x, w: cache.attention(torch.zeros_like(x), t, n, weights=w), lambda x, w: cache.evict(t, n, w, dst, 8)]
+    uses_x = [True, True, True, True, False, False]
+    for call, of_x in zip(calls, uses_x):
+        with fwad.dual_level():
+            a = fwad.make_dual(x.clone(), torch.ones_like(x)) if of_x else x.clone()
+            b = w.clone() if of_x else fwad.make_dual(w.clone(), torch.ones_like(w))
+            with pytest.raises(pf.PegaflowInvalidArgument, match="backward"):
+                call(a, b)
+        with pytest.raises(pf.PegaflowInvalidArgument, match="backward"):
+            call(x.clone().requires_grad_() if of_x else x, w if of_x else w.clone().requires_grad_())
+        with torch.no_grad():
+            call(x.clone().requires_grad_() if of_x else x.clone(), w.clone() if of_x else w.clone().requires_grad_())
+    with fwad.dual_level():
+        cache.attention(x, t, n, weights=w)          # nothing here carries a tangent
+    cache.check()
