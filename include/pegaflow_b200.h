@@ -601,7 +601,8 @@ int pf_kv8_append(int device_id, const pf_kv8_cache *cache, const pf_kv8_batch *
 enum { PF_KV8_CLEAR_ALL = 1, PF_KV8_CLEAR_LSE = 2 };
 typedef struct pf_kv8_attention_args {
   const void *q;               /* [n_rows][q_heads][head_dim], q_heads a multiple of kv_heads */
-  void *out;                   /* the same shape and type */
+  void *out;                   /* the same shape and type; may be q itself where weights are NULL or of few rows whose scores
+                                  are kept, and must not overlap it (or itself) otherwise */
   float *lse;                  /* [n_rows][q_heads] dense, or NULL */
   float *weights;
   size_t n_rows;

@@ -205,6 +205,33 @@ Plan make_plan(int device_id, const Kv8View &c, const Kv8Batch &b, const pf_kv8_
   return plan;
 }
 
+// Whether two elements of an array of outer x inner dense rows of n elements can be one; of a single row any stride will do.
+bool overlaps_itself(size_t outer, size_t outer_stride, size_t inner, size_t inner_stride, size_t n) {
+  if (outer * inner <= 1) return false;
+  if (outer > 1 && (inner == 1 || inner_stride > outer_stride)) std::swap(outer, inner), std::swap(outer_stride, inner_stride);
+  // now outer_stride is the larger one, or outer is 1
+  const size_t whole = outer == 1 || inner > 1 ? (inner - 1) * inner_stride + n : n;
+  return (inner > 1 && inner_stride < n) || (outer > 1 && outer_stride < whole);
+}
+
+// Whether out can share an element with q where the two are not one and the same: their ranges are apart, or the rests of their
+// offsets modulo one of the strides are (heads or rows of one buffer that belong to q and to out in turn).
+bool shares(const pf_kv8_attention_args &a, int dim) {
+  const uint64_t q = (uint64_t)a.q, out = (uint64_t)a.out;
+  auto bytes = [&](size_t row, size_t head) { return 2 * ((a.n_rows - 1) * row + (a.q_heads - 1) * head + dim); };
+  if (q + bytes(a.q_row_stride, a.q_head_stride) <= out || out + bytes(a.out_row_stride, a.out_head_stride) <= q) return false;
+  if ((out - q) % 2) return true;
+  for (const size_t m : {a.q_row_stride, a.q_head_stride, a.out_row_stride, a.out_head_stride}) {
+    if (!m) continue;
+    auto rest = [&](size_t row, size_t head) {       // elements from the first one on that an offset's rest can be
+      return (row % m ? (a.n_rows - 1) * row : 0) + (head % m ? (a.q_heads - 1) * head : 0) + dim;
+    };
+    const size_t apart = out >= q ? (out - q) / 2 % m : (m - (q - out) / 2 % m) % m;
+    if (apart >= rest(a.q_row_stride, a.q_head_stride) && apart + rest(a.out_row_stride, a.out_head_stride) <= m) return false;
+  }
+  return true;
+}
+
 void check_args(const pf_kv8_attention_args *a, const Kv8View &c, const Kv8Batch &b) {
   if (!a) throw Error::invalid("null attention arguments");
   if (a->dtype != PF_KV8_BF16 && a->dtype != PF_KV8_F16) throw Error::invalid(strf("unknown dtype %d", a->dtype));
@@ -290,7 +317,14 @@ int pf_kv8_attention(int device_id, const pf_kv8_cache *cache, const pf_kv8_batc
     if (a.n_rows == 0 || (b.n_seqs == 0 && !a.clear_tail)) return;
     if (!a.q || !a.out) throw Error::invalid("null q or out");
     if ((uintptr_t)a.q % 2 || (uintptr_t)a.out % 2) throw Error::invalid("q and out must be aligned to their elements");
+    if (overlaps_itself(a.n_rows, a.out_row_stride, a.q_heads, a.out_head_stride, c.dim)) throw Error::invalid("elements of out overlap");
+    if (a.weights && overlaps_itself(b.n_seqs, a.weights_seq_stride, c.heads, a.weights_head_stride, a.weights_capacity))
+      throw Error::invalid("elements of weights overlap");
+    // a row tile of q has been read when its part of out is written
+    const bool in_place = a.q == a.out && a.q_row_stride == a.out_row_stride && a.q_head_stride == a.out_head_stride;
+    if (!in_place && shares(a, c.dim)) throw Error::invalid("out overlaps q");
     const Plan plan = make_plan(device_id, c, b, a);
+    if (in_place && a.weights && !plan.score_tokens) throw Error::invalid("out overlaps q, which these weights are computed from again");
     if (!workspace || workspace_bytes < plan.bytes)
       throw Error::invalid(strf("workspace of %zu bytes, the call needs %zu", workspace ? workspace_bytes : 0, plan.bytes));
     if ((uintptr_t)workspace % 256) throw Error::invalid("the workspace must be 256-byte aligned");

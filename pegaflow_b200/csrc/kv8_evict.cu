@@ -306,6 +306,7 @@ extern "C" int pf_kv8_evict(int device_id, const pf_kv8_cache *cache, const pf_k
     p.keep = (int)a.keep, p.recent = (int)a.recent;
     p.n_dst = (int)((a.keep + (1 << c.block_log2) - 1) >> c.block_log2);
     p.new_lens = a.new_lens, p.new_weights = a.new_weights, p.new_capacity = (int64_t)a.new_capacity, p.kept = a.kept;
+    if (b.n_seqs > 1 && a.dst_table_stride < (size_t)p.n_dst) throw Error::invalid("rows of dst_tables overlap: every sequence needs blocks of its own");
     const uint64_t tiles = (uint64_t)b.n_seqs * c.heads * p.n_dst;
     if (tiles > 0x7fffffffu) throw Error::invalid("too many blocks for one call: split the batch");
     kv8_sm_count(device_id);

@@ -380,3 +380,42 @@ def test_tangents_and_gradients_are_refused(pf):
     with fwad.dual_level():
         cache.attention(x, t, n, weights=w)          # nothing here carries a tangent
     cache.check()
+
+
+def test_outputs_that_overlap_themselves_or_the_queries_are_refused(pf):
+    """Several CTAs would write one element, or one would read what another has written."""
+    cache = pf.Kv8Cache(6, 16, 2, 64)
+    t, n = ints([[1, 2], [3, 4]]), ints([20, 7])
+    q = torch.randn((2, 4, 64), generator=gen(250), device="cuda").half()
+    w = torch.zeros((2, 2, 32), device="cuda")
+    many = q.repeat(20, 1, 1)               # 40 rows of a KV head: their weights take the queries a second time
+    buffer = torch.zeros(4096, dtype=torch.float16, device="cuda")
+    E = pf.PegaflowInvalidArgument
+    for bad in (lambda: cache.attention(q, t, n, out=q.new_zeros((1, 4, 64)).expand(2, 4, 64)),
+                lambda: cache.attention(q, t, n, out=q.new_zeros((2, 1, 64)).expand(2, 4, 64)),
+                lambda: cache.attention(q, t, n, out=buffer.as_strided((2, 4, 64), (200, 64, 1))),
+                lambda: cache.attention(q, t, n, weights=w[:1].expand(2, 2, 32)), lambda: cache.attention(q, t, n, weights=w[:, :1].expand(2, 2, 32)),
+                lambda: cache.evict(t, n, w, ints([[5]]).expand(2, 1), 8),
+                lambda: cache.attention(buffer[:512].view(2, 4, 64), t, n, out=buffer[64:576].view(2, 4, 64)),
+                lambda: cache.attention(many, t, n, out=many, weights=w)):
+        with pytest.raises(E, match="overlap"):
+            bad()
+    cache.check()
+    # in place, and between the queries: as before
+    want = cache.attention(q, t, n)
+    fused = torch.zeros((2, 12, 64), dtype=torch.float16, device="cuda")
+    fused[:, 4:8] = q
+    cache.attention(fused[:, 4:8], t, n, out=fused[:, :4])
+    assert torch.equal(fused[:, :4], want) and torch.equal(fused[:, 4:8], q) and (fused[:, 8:] == 0).all()
+    apart = torch.zeros((2, 4, 2, 64), dtype=torch.float16, device="cuda")
+    apart[:, :, 1] = q
+    cache.attention(apart[:, :, 1], t, n, out=apart[:, :, 0])
+    assert torch.equal(apart[:, :, 0], want)
+    mine = q.clone()
+    assert torch.equal(cache.attention(mine, t, n, out=mine), want)
+    mine = q.clone()
+    assert torch.equal(cache.attention(mine, t, n, out=mine, weights=w), want)
+    mine = many.clone()
+    assert torch.equal(cache.attention(mine, t, n, out=mine), cache.attention(many, t, n))
+    one = cache.attention(q[:1], t[:1], n[:1], out=q.new_zeros((1, 4, 64)).expand(1, 4, 64))      # of one row any stride
+    assert torch.equal(one, want[:1])

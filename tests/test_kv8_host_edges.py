@@ -90,3 +90,64 @@ def test_work_is_counted_in_the_tiles_that_the_rows_go_in(rows, q_heads, max_blo
         assert status == (0 if torch.cuda.is_available() else 4)
     else:
         refused(status, "too many query rows")
+
+
+CLEAN = dict(n_rows=4, max_query=2, q_heads=4, q=PTR, out=PTR + (1 << 20), q_row_stride=256, q_head_stride=64, out_row_stride=256, out_head_stride=64)
+
+
+def attended(**kw):
+    d = dict(CLEAN, **kw)
+    return N.lib.pf_kv8_attention(0, C.byref(cache()), C.byref(batch(starts=None)), C.byref(attention(**d)), None, 0, None)
+
+
+@pytest.mark.parametrize("kw,word", [
+    (dict(out_row_stride=0), "out"), (dict(out_head_stride=0), "out"), (dict(out_row_stride=255), "out"), (dict(out_head_stride=63), "out"),
+    (dict(out_row_stride=64, out_head_stride=255), "out"), (dict(out_row_stride=64, out_head_stride=64), "out"),
+    (dict(weights=PTR, weights_seq_stride=0, weights_head_stride=32, weights_capacity=32), "weights"),
+    (dict(weights=PTR, weights_seq_stride=64, weights_head_stride=31, weights_capacity=32), "weights"),
+    (dict(out=PTR + 128), "q"), (dict(out=PTR + 2), "q"), (dict(out=PTR - 512), "q"), (dict(out=PTR, out_row_stride=512), "q"),
+    (dict(q_row_stride=512, out_row_stride=512, out=PTR + 2 * 256 - 2), "q"), (dict(q_row_stride=512, out_row_stride=512, out=PTR + 2 * 256 + 1), "aligned")])
+def test_outputs_that_overlap_are_refused(kw, word):
+    refused(attended(**kw), word)
+
+
+@pytest.mark.parametrize("kw", [
+    {}, dict(out=PTR), dict(out_row_stride=64, out_head_stride=256),                       # apart, in place, heads outermost
+    dict(q_row_stride=512, out_row_stride=512, out=PTR + 2 * 256), dict(q_row_stride=512, out_row_stride=512, out=PTR - 2 * 256),   # rows in turn
+    dict(q_row_stride=512, q_head_stride=128, out_row_stride=512, out_head_stride=128, out=PTR + 128),                          # heads in turn
+    dict(n_rows=2, max_query=1, q_heads=2, out_row_stride=192, out_head_stride=64),
+    dict(weights=PTR, weights_seq_stride=64, weights_head_stride=32, weights_capacity=32),
+    dict(weights=PTR, weights_seq_stride=32, weights_head_stride=64, weights_capacity=32)])
+def test_outputs_that_do_not_overlap_get_past_the_checks(kw):
+    """What comes next is the device, or (where there is one) the workspace that this call does not have."""
+    status = attended(**kw)
+    assert status == 4 or (status == 3 and b"workspace" in N.lib.pf_last_error()), (status, N.lib.pf_last_error())
+
+
+def test_the_overlap_checks_agree_with_a_search_of_all_elements():
+    """Small random layouts: whatever shares an element is refused, but for q itself; most of what does not is let through."""
+    g = torch.Generator().manual_seed(3)
+    among = lambda x: x[int(torch.randint(0, len(x), (1,), generator=g))]  # noqa: E731
+    steps = [0, 32, 64, 96, 128, 160, 192, 256, 288, 384]
+    seen = {True: 0, False: 0}
+    for _ in range(800):
+        rows, heads, delta = among([2, 4]), among([2, 4]), 32 * among(range(-24, 25))
+        q_strides, strides = (among(steps), among(steps)), (among(steps), among(steps))
+        if among([True, False]):
+            strides = q_strides
+        status = attended(n_rows=rows, max_query=rows // 2, q_heads=heads, out=PTR + 2 * delta, q_row_stride=q_strides[0], q_head_stride=q_strides[1],
+                          out_row_stride=strides[0], out_head_stride=strides[1])
+        told = status == 3 and b"overlap" in N.lib.pf_last_error()
+        places = lambda at, s: [at + i * s[0] + j * s[1] + d for i in range(rows) for j in range(heads) for d in range(64)]  # noqa: E731
+        q, out = places(0, q_strides), places(delta, strides)
+        shared = len(set(out)) < len(out) or (not set(q).isdisjoint(out) and not (delta == 0 and strides == q_strides))
+        assert told or not shared, (rows, heads, delta, q_strides, strides)
+        if not shared:
+            seen[told] += 1
+    assert seen[False] > 2 * seen[True]
+
+
+def test_eviction_into_rows_that_overlap_is_refused():
+    for stride in (0, 1):
+        refused(N.lib.pf_kv8_evict(0, C.byref(cache()), C.byref(batch()), C.byref(evict(dst_table_stride=stride)), None), "overlap")
+    assert N.lib.pf_kv8_evict(0, C.byref(cache()), C.byref(batch(n_seqs=0)), C.byref(evict(dst_table_stride=0)), None) == 0
