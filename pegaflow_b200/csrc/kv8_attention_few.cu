@@ -70,9 +70,9 @@ constexpr int kRing = 16;
 template <int kDim, int kRows, int kSlots, bool kWithV>
 struct FewShared {
   float scale[kRing][2][kGroups];             // of K, of V; -1: the group's block is not in the cache
-  uint64_t full[kSlots], empty[kSlots], q_ready, s_full[2], p_ready[2], pv_done[2];
-  uint32_t tmem;
-  int stalled, any_nan;
+  uint64_t full[kSlots], empty[kSlots], q_ready, s_full[2], p_ready[2], pv_done[2], drained;
+  uint32_t tmem, fed;        // fed: slots that copies were started into, where a wait ran out
+  int stalled, late, any_nan;
   float factor[kRows], base[kRows], row_top[8];
   float ref[2][kRows], down[2][kRows], top[2][4][kRows], sum[2][4][kRows], v_top[2][4], v_ref[2];
   int see[kRows];
@@ -153,13 +153,15 @@ __global__ void __launch_bounds__(kThreads, few_ctas(kDim, kRows)) kv8_attention
       bar_init(&sh.empty[i], 1);
     }
     bar_init(&sh.q_ready, kWorkers);
+    bar_init(&sh.drained, 1);
     for (int i = 0; i < 2; ++i) {
       bar_init(&sh.s_full[i], 1);
       bar_init(&sh.p_ready[i], kTeam);
       bar_init(&sh.pv_done[i], 1);
     }
-    sh.stalled = 0;
+    sh.stalled = sh.late = 0;
     sh.any_nan = 0;
+    sh.fed = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 9) {
@@ -236,7 +238,10 @@ __global__ void __launch_bounds__(kThreads, few_ctas(kDim, kRows)) kv8_attention
 #pragma unroll
           for (int of = 0; of < L::kKv; ++of) {
             const uint32_t i = L::kKv * at + of, slot = i % kSlots;
-            if (!(ok = bar_wait_warp(&sh.empty[slot], (i / kSlots & 1) ^ 1, &sh.stalled))) break;
+            if (!(ok = bar_wait_warp(&sh.empty[slot], (i / kSlots & 1) ^ 1, &sh.stalled))) {
+              sh.fed = i;
+              break;
+            }
             if (of == 0 && lane >= 16) sh.scale[at % kRing][kv][group] = now;
             __syncwarp();
             if (lane == 0)
@@ -593,12 +598,25 @@ __global__ void __launch_bounds__(kThreads, few_ctas(kDim, kRows)) kv8_attention
   // The tensor cores' last arrivals, at the slots that are not filled again, come before the block leaves.
   if (warp == 8 && ok)
     for (uint32_t i = L::kKv * n_tiles > (uint32_t)kSlots ? L::kKv * n_tiles - kSlots : 0; i < L::kKv * n_tiles && ok; ++i)
-      ok = bar_wait_warp(&sh.empty[i % kSlots], i / kSlots & 1, &sh.stalled);
+      if (!(ok = bar_wait_warp(&sh.empty[i % kSlots], i / kSlots & 1, &sh.stalled))) sh.fed = L::kKv * n_tiles;
   __syncwarp();
   fence_before();
   __syncthreads();
   fence_after();
-  if (sh.stalled && tid == 0) p.batch.report(PF_KV8_STALLED);
+  if (sh.stalled) {          // a wait ran out: what is still under way, copies and products, ends before the block does
+    if (tid == 0) p.batch.report(PF_KV8_STALLED);
+    if (warp == 8 && lane == 0) {
+      const uint32_t fed = sh.fed;
+      for (uint32_t i = fed > (uint32_t)kSlots ? fed - kSlots : 0; i < fed; ++i)
+        if (!bar_wait(&sh.full[i % kSlots], i / kSlots & 1, &sh.late)) break;
+    }
+    if (warp == 9 && lane == 0) {
+      commit(&sh.drained);
+      bar_wait(&sh.drained, 0, &sh.late);
+    }
+    __syncthreads();
+    fence_after();
+  }
   if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(L::kAlloc));
 }
 

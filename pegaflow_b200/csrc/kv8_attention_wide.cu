@@ -60,9 +60,9 @@ struct Part {
   int whole, slot;                       // all of the tile's tokens, or a partial result in this slot
 };
 struct Shared {
-  uint64_t q_full, full[2][2], empty[2][2], s_full[2], p_full[2], o_full[2], scales_full[kRing];
+  uint64_t q_full, full[2][2], empty[2][2], s_full[2], p_full[2], o_full[2], scales_full[kRing], drained;
   uint32_t tmem;
-  int stalled, any_nan;
+  int stalled, late, any_nan;
   Part part[2];
   float k_unit[kRing];       // 2^e_ref of K
   int v_ref[kRing];          // e_ref of V
@@ -118,7 +118,8 @@ __global__ void __launch_bounds__(threads_of(kDim), 1) kv8_attention_wide(AttnPa
       bar_init(&sh.o_full[i], 1);
     }
     for (int i = 0; i < kRing; ++i) bar_init(&sh.scales_full[i], 1);
-    sh.stalled = 0;
+    bar_init(&sh.drained, 1);
+    sh.stalled = sh.late = 0;
     sh.any_nan = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -572,7 +573,15 @@ __global__ void __launch_bounds__(threads_of(kDim), 1) kv8_attention_wide(AttnPa
   fence_before();
   __syncthreads();
   fence_after();
-  if (sh.stalled && tid == 0) p.batch.report(PF_KV8_STALLED);
+  if (sh.stalled) {          // a wait ran out: products that are still under way end before the block does
+    if (tid == 0) p.batch.report(PF_KV8_STALLED);
+    if (warp == kIssue && lane == 0) {
+      commit(&sh.drained);
+      bar_wait(&sh.drained, 0, &sh.late);
+    }
+    __syncthreads();
+    fence_after();
+  }
   if (warp == kIssue) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
 }
 
