@@ -568,8 +568,8 @@ enum pf_kv8_dtype { PF_KV8_BF16 = 0, PF_KV8_F16 = 1 };
 /* Bits of *status: what a kernel found and left out. */
 #define PF_KV8_BAD_BLOCK 1u   /* a block id outside the cache: its tokens are not written / not seen */
 #define PF_KV8_BAD_LENGTH 2u  /* a length below 0, or above what the block table or the weights hold: cut */
-#define PF_KV8_BAD_ROWS 4u    /* row starts that fall, leave the tensors, or give a sequence more than max_query rows: cut; where they
-                               claim more rows than the call can have, attention computes none */
+#define PF_KV8_BAD_ROWS 4u    /* row starts that fall, leave the tensors, or give a sequence more than max_query rows: cut; where one
+                               falls, attention computes no row of the call */
 #define PF_KV8_STALLED 8u     /* a wait inside a kernel ran out (two seconds): the outputs of the call are not valid */
 
 typedef struct pf_kv8_batch {

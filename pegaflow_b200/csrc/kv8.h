@@ -49,15 +49,17 @@ struct Kv8Batch {
   int n_rows;          // rows that the tensors of the call hold
   uint32_t *status;    // PF_KV8_* bits, or null
 
-  // Rows [lo, hi) of a sequence, within the tensors whatever `starts` holds.
-  __device__ void rows(int s, int &lo, int &hi) const {
+  // Rows [lo, hi) of a sequence, within the tensors whatever `starts` holds; false where its starts fall.
+  __device__ bool rows(int s, int &lo, int &hi) const {
     if (starts) {
-      lo = min(max(starts[s], 0), n_rows);
-      hi = min(max(starts[s + 1], lo), n_rows);
-    } else {
-      lo = s * rows_each;
-      hi = lo + rows_each;
+      const int a = starts[s], b = starts[s + 1];
+      lo = min(max(a, 0), n_rows);
+      hi = min(max(b, lo), n_rows);
+      return a <= b;
     }
+    lo = s * rows_each;
+    hi = lo + rows_each;
+    return true;
   }
   __device__ void report(uint32_t bits) const {
     if (status) atomicOr(status, bits);

@@ -21,34 +21,11 @@ __device__ __forceinline__ uint32_t narrow2(float lo, float hi) {
 // some 5 us behind the last CTA of the attention.
 constexpr int kJoinThreads = 256;
 template <int kDim, int kRows, int kUnits, bool kBf16>
-__global__ void __launch_bounds__(kJoinThreads) kv8_attention_join(AttnParams p, int team) {
+__device__ __forceinline__ void join(const AttnParams &p, const Work<kRows, kUnits> &work, int team) {
   constexpr int kSpan = kDim / 4, kDeep = 4;
   using SeqT = Seq<kRows, kUnits>;
-  extern __shared__ __align__(128) char smem[];
-  uint32_t *prefix = reinterpret_cast<uint32_t *>(smem);
   __shared__ float4 sh_a[kJoinThreads];
   __shared__ float sh_l[kJoinThreads], sh_top[kJoinThreads / 32];
-  const int n_seqs = p.batch.n_seqs;
-  const Work<kRows, kUnits> work(p, prefix);
-  after_previous();
-  const bool none = work.total() == 0;         // no rows, or row starts that claim more than there can be: no row is computed
-  if (p.clear_tail || (none && p.weights)) {   // rows [0, first) and [last, n_rows) belong to no sequence
-    int first = 0, last = 0, ignored;
-    if (!none) {
-      p.batch.rows(0, first, ignored);
-      p.batch.rows(n_seqs - 1, ignored, last);
-      first = min(first, last);
-    }
-    const int64_t per_row = (int64_t)p.q_heads * kDim, all = (first + p.batch.n_rows - last) * per_row;
-    const int64_t id = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * kJoinThreads + threadIdx.x;
-    for (int64_t e = id; e < all; e += (int64_t)gridDim.x * gridDim.y * kJoinThreads) {
-      int64_t row = e / per_row;
-      if (row >= first) row += last - first;
-      const int qh = (int)(e / kDim % p.q_heads), d = (int)(e % kDim);
-      if (p.clear_tail == PF_KV8_CLEAR_ALL) p.out[row * p.out_row + qh * p.out_head + d] = 0;
-      if (d == 0 && p.lse) p.lse[row * p.q_heads + qh] = -INFINITY;
-    }
-  }
   const Split split(work.total(), p.n_ctas);
   const int c0 = blockIdx.x;
   if (c0 + 1 >= split.n_ctas) return;
@@ -122,6 +99,38 @@ __global__ void __launch_bounds__(kJoinThreads) kv8_attention_join(AttnParams p,
   }
 }
 
+// Rows of no sequence, [0, first) and [last, n_rows), are cleared; all rows where none was computed, for the weights' sake too.
+template <int kDim>
+__device__ __forceinline__ void clear_rows(const AttnParams &p, bool none) {
+  int first = 0, last = 0, ignored;
+  if (!none) {
+    p.batch.rows(0, first, ignored);
+    p.batch.rows(p.batch.n_seqs - 1, ignored, last);
+  }
+#pragma unroll 1
+  for (uint32_t i = blockIdx.y * gridDim.x + blockIdx.x; i < (uint32_t)(first + p.batch.n_rows - last); i += gridDim.x * gridDim.y) {
+    const int64_t row = i < (uint32_t)first ? i : i - first + last;
+    if (p.clear_tail == PF_KV8_CLEAR_ALL) {
+#pragma unroll 1
+      for (int c = threadIdx.x; c < p.q_heads * kDim; c += kJoinThreads) p.out[row * p.out_row + c / kDim * p.out_head + c % kDim] = 0;
+    }
+    if (p.lse) {
+#pragma unroll 1
+      for (int c = threadIdx.x; c < p.q_heads; c += kJoinThreads) p.lse[row * p.q_heads + c] = -INFINITY;
+    }
+  }
+}
+
+template <int kDim, int kRows, int kUnits, bool kBf16>
+__global__ void __launch_bounds__(kJoinThreads) kv8_attention_join(AttnParams p, int team) {
+  extern __shared__ __align__(128) char smem[];
+  const Work<kRows, kUnits> work(p, reinterpret_cast<uint32_t *>(smem));
+  after_previous();
+  join<kDim, kRows, kUnits, kBf16>(p, work, team);
+  const bool none = work.total() == 0;
+  if (p.clear_tail || (none && p.weights)) clear_rows<kDim>(p, none);      // behind the join, which others may wait for
+}
+
 // Each token's probability from the scores that the attention kept, added to the weights: a thread a token, rows in order.
 // Bound by memory, 4 bytes for each score and 8 for each weight.
 constexpr int kAddThreads = 256;
@@ -143,6 +152,10 @@ __global__ void __launch_bounds__(kAddThreads) kv8_weights_add(AttnParams p) {
       if (lse != -INFINITY) base[r] = lse * kLog2e;
     }
   }
+  bool any = false;            // of rows that were not computed (a row start falls) there are no scores
+#pragma unroll
+  for (int r = 0; r < kRows; ++r) any |= base[r] != INFINITY;
+  if (!any) return;
   const float *scores = p.scores + (int64_t)blockIdx.x * p.score_tokens * kRows;
   float *weights = p.weights + s * p.w_seq + head * p.w_head;
   for (int tok = blockIdx.y * kAddThreads + threadIdx.x; tok < end; tok += gridDim.y * kAddThreads) {
@@ -165,7 +178,6 @@ struct Plan {
   size_t part_o, part_ml, lse, scores, bytes;   // offsets in the workspace
   int score_tokens;     // 0: scores are not kept
   int row_tiles;        // of a sequence, at most
-  uint32_t units;       // of all its rows, at most
 };
 
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
@@ -188,7 +200,6 @@ Plan make_plan(int device_id, const Kv8View &c, const Kv8Batch &b, const pf_kv8_
                          (((uint64_t)a.n_rows * group) / plan.rows + b.n_seqs) * c.heads;
   const uint64_t row_tiles = std::max<uint64_t>(1, (rows + plan.rows - 1) / plan.rows);
   if (units > 0xffffffffull || row_tiles * b.n_seqs > 1u << 29) throw Error::invalid("too many query rows for tables of this width: split the call");
-  plan.units = (uint32_t)units;
   plan.row_tiles = (int)row_tiles;
   plan.n_ctas = kv8_sm_count(device_id) * (plan.wide ? 1 : kv8_few_ctas(c.dim, plan.rows));
   const size_t slots = 2 * (size_t)plan.n_ctas * plan.rows;
@@ -348,7 +359,6 @@ int pf_kv8_attention(int device_id, const pf_kv8_cache *cache, const pf_kv8_batc
     p.group = (int)a.q_heads / c.heads;
     p.max_query = (int)std::min<size_t>(a.max_query, a.n_rows);
     p.row_tiles_most = plan.row_tiles;
-    p.units_most = plan.units;
     p.causal = a.causal != 0;
     p.clear_tail = a.clear_tail;
     p.vec_q = (uintptr_t)a.q % 16 == 0 && (a.q_row_stride | a.q_head_stride) % 8 == 0;

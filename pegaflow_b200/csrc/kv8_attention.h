@@ -23,7 +23,6 @@ struct AttnParams {
   int w_capacity;
   int q_heads, group, max_query;
   int row_tiles_most;   // of a sequence
-  uint32_t units_most;  // units (see Work) that n_rows rows can be, however they fall on the sequences
   int causal, clear_tail, vec_q, vec_out;
   float scale;
   // Partial results: slot 2 c + k of CTA c (k = 0: the segment that its range starts in, 1: the one that it ends in).
@@ -57,9 +56,10 @@ struct Split {
 template <int kRows, int kUnit, bool kWhole = false>
 struct Seq {
   int row0, rows, len, row_tiles;
+  bool rises;
   __device__ Seq(const AttnParams &p, int s) {
     int hi;
-    p.batch.rows(s, row0, hi);
+    rises = p.batch.rows(s, row0, hi);
     rows = min(hi - row0, p.max_query);
     len = p.batch.length(s, p.cache.block_log2);
     row_tiles = kWhole ? min(rows, 1) : (rows * p.group + kRows - 1) / kRows;     // kRows is a power of two
@@ -77,8 +77,8 @@ struct Seq {
 // The units of all (sequence, row tile) entries in order, kCost of them in front of each head's for what a segment costs at its
 // beginning and end, as sums before every chunk of entries (one, unless there are more
 // than kMost).  Every CTA of every kernel computes them for itself: lens stay on the device, and no launch and no
-// workspace is spent on it.  Row starts that fall and rise again can claim rows more than once: sums stay at the largest number
-// instead of wrapping, and where they exceed what the call's rows can be there is no work at all.
+// workspace is spent on it.  Where a row start falls there is no work at all: starts that fall and rise again claim rows more than
+// once, more of them together than the host has checked 32 bits for.
 template <int kRows, int kUnit, bool kWhole = false>
 struct Work {
   using SeqT = Seq<kRows, kUnit, kWhole>;
@@ -88,20 +88,22 @@ struct Work {
   static constexpr uint32_t kCost = 4;
   uint32_t *prefix;         // [chunks + 1] in shared memory
   int entries, chunk, chunks;
+  bool none;                // a row start falls
   static __host__ __device__ int chunk_of(int entries) { return max((entries + kMost - 1) / kMost, 1); }
   static __host__ size_t bytes(int n_seqs, int row_tiles_most) {
     const int entries = n_seqs * row_tiles_most, chunk = chunk_of(entries);
     return ((size_t)(entries + chunk - 1) / chunk + 1) * 4;
   }
-  static __device__ uint32_t add(uint32_t a, uint32_t b) {
-    const uint32_t sum = a + b;
-    return sum < a ? 0xffffffffu : sum;
-  }
   static __device__ int seq_of(const AttnParams &p, int e) { return p.row_tiles_most == 1 ? e : e / p.row_tiles_most; }
-  __device__ uint32_t units_of(const AttnParams &p, int e) const {       // of one head
+  __device__ uint32_t units_of(const AttnParams &p, int e, bool &falls) const {       // of one head
     const int s = seq_of(p, e), rt = e - s * p.row_tiles_most;
     const SeqT seq(p, s);
+    falls |= !seq.rises;
     return rt < seq.row_tiles ? seq.units(p, rt) + kCost : 0u;
+  }
+  __device__ uint32_t units_of(const AttnParams &p, int e) const {
+    bool ignored;
+    return units_of(p, e, ignored);
   }
   __device__ Work(const AttnParams &p, uint32_t *prefix) : prefix(prefix) {
     __shared__ uint32_t warp_sum[32];
@@ -110,31 +112,32 @@ struct Work {
     chunks = (entries + chunk - 1) / chunk;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n_warps = (blockDim.x + 31) >> 5;
     uint32_t base = 0;
+    bool falls = false;
     for (int c0 = 0; c0 < chunks; c0 += blockDim.x) {
       const int c = c0 + threadIdx.x;
       uint32_t mine = 0;
-      for (int e = c * chunk; c < chunks && e < min((c + 1) * chunk, entries); ++e) mine = add(mine, units_of(p, e) * (uint32_t)p.cache.heads);
+      for (int e = c * chunk; c < chunks && e < min((c + 1) * chunk, entries); ++e) mine += units_of(p, e, falls) * (uint32_t)p.cache.heads;
       uint32_t x = mine;
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) {
         const uint32_t y = __shfl_up_sync(0xffffffffu, x, d);
-        if (lane >= d) x = add(x, y);
+        if (lane >= d) x += y;
       }
       if (lane == 31) warp_sum[warp] = x;
       __syncthreads();
       uint32_t before = base, all = 0;
       for (int w = 0; w < n_warps; ++w) {
-        if (w < warp) before = add(before, warp_sum[w]);
-        all = add(all, warp_sum[w]);
+        if (w < warp) before += warp_sum[w];
+        all += warp_sum[w];
       }
       if (c < chunks) prefix[c] = before + x - mine;
-      base = add(base, all);
+      base += all;
       __syncthreads();
     }
-    if (threadIdx.x == 0) prefix[chunks] = base > p.units_most ? 0 : base;
-    __syncthreads();
+    if (threadIdx.x == 0) prefix[chunks] = base;
+    none = __syncthreads_or(falls);
   }
-  __device__ uint32_t total() const { return prefix[chunks]; }
+  __device__ uint32_t total() const { return none ? 0u : prefix[chunks]; }
 };
 
 // The segment in which unit u < total lies, at or behind `from`.
@@ -152,7 +155,7 @@ struct Segment {
     int e = lo * work.chunk;
     begin = work.prefix[lo];
     units = work.units_of(p, e);
-    while (e + 1 < work.entries && u - begin >= units * (uint32_t)p.cache.heads) {
+    while (u - begin >= units * (uint32_t)p.cache.heads) {
       begin += units * (uint32_t)p.cache.heads;
       units = work.units_of(p, ++e);
     }

@@ -217,6 +217,22 @@ def test_row_starts_that_fall_again_and_again_do_no_harm(pf, seqs, n, width, hea
     assert (out == 0).all() and torch.isneginf(lse).all()
 
 
+@pytest.mark.parametrize("rows", [1, 5, 40])
+def test_row_starts_that_fall_leave_weights_as_they_are(pf, rows):
+    """Whether scores would have been kept or taken again; without an lse of the call's own; a given out stays too."""
+    size, heads, dim = 16, 2, 128
+    blocks, tables = make_tables([100, 80, 60], size, 266)
+    cache = make_cache(pf, blocks, size, heads, dim, 267)
+    q = torch.randn((2 * rows, 4 * heads, dim), generator=gen(268), device="cuda").half()
+    w = torch.rand((3, heads, 100), generator=gen(269), device="cuda")
+    before, out = w.clone(), torch.full_like(q, 3.0)
+    starts = ints([0, 2 * rows, rows, 2 * rows])
+    cache.attention(q, tables.cuda(), ints([100, 80, 60]), starts=starts, max_query=rows, weights=w, out=out)
+    with pytest.raises(pf.PegaflowInvalidArgument, match="row starts"):
+        cache.check()
+    assert torch.equal(w, before) and (out == 3).all()
+
+
 def test_prompts_over_wide_tables_are_counted_by_their_own_tiles(pf):
     """8 prompts of 300 rows with tables for 2^24 tokens, of which they use 400."""
     size, heads, group, dim, rows = 16, 2, 16, 64, 300
