@@ -107,6 +107,8 @@ struct Work {
   }
   __device__ Work(const AttnParams &p, uint32_t *prefix) : prefix(prefix) {
     __shared__ uint32_t warp_sum[32];
+    __shared__ int sh_none;
+    if (threadIdx.x == 0) sh_none = 0;
     entries = p.batch.n_seqs * p.row_tiles_most;
     chunk = chunk_of(entries);
     chunks = (entries + chunk - 1) / chunk;
@@ -135,7 +137,9 @@ struct Work {
       __syncthreads();
     }
     if (threadIdx.x == 0) prefix[chunks] = base;
-    none = __syncthreads_or(falls);
+    if (falls) sh_none = 1;          // a vote of the barrier instead costs half a microsecond
+    __syncthreads();
+    none = sh_none;
   }
   __device__ uint32_t total() const { return none ? 0u : prefix[chunks]; }
 };
