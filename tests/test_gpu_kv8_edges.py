@@ -435,3 +435,101 @@ def test_outputs_that_overlap_themselves_or_the_queries_are_refused(pf):
     assert torch.equal(cache.attention(mine, t, n, out=mine), cache.attention(many, t, n))
     one = cache.attention(q[:1], t[:1], n[:1], out=q.new_zeros((1, 4, 64)).expand(1, 4, 64))      # of one row any stride
     assert torch.equal(one, want[:1])
+
+
+def test_all_three_in_one_graph_with_a_given_stream(pf):
+    """A step of append, attention and eviction captured together, on the capturing stream by name; replayed with other
+    lengths and rows, it gives what the calls give."""
+    size, heads, dim = 16, 2, 64
+    cache, same = make_cache(pf, 12, size, heads, dim, 235), make_cache(pf, 12, size, heads, dim, 235)
+    t, dst = ints([[1, 2, 3], [4, 5, 6]]), ints([[7], [8]])
+    x = torch.randn((2, heads, dim), generator=gen(236), device="cuda").half()
+    q = torch.randn((2, 2 * heads, dim), generator=gen(237), device="cuda").half()
+    lens, w = ints([20, 31]), torch.zeros((2, heads, 48), device="cuda")
+
+    def step(c, stream):
+        c.append(x, -x, t, lens, stream=stream)
+        out = c.attention(q, t, lens + 1, weights=w, stream=stream)
+        return (out, *c.evict(t, lens + 1, w, dst, 10, recent=3, stream=stream))
+
+    step(cache, None)
+    torch.cuda.synchronize()
+    cache.tensor.copy_(same.tensor)
+    graph, capturing = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph, stream=capturing):
+        got = step(cache, capturing.cuda_stream)
+    for lengths in ([20, 31], [0, 47], [15, 16]):
+        lens.copy_(ints(lengths))
+        x.copy_(torch.randn((2, heads, dim), generator=gen(238 + lengths[0]), device="cuda"))
+        w.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        weights = w.clone()
+        w.zero_()
+        want = step(same, None)
+        assert torch.equal(weights, w) and all(torch.equal(a, b) for a, b in zip(got, want))
+        assert torch.equal(cache.tensor, same.tensor)
+    cache.check()
+
+
+@pytest.mark.parametrize("kind", ["spread", "ties", "special"])
+@pytest.mark.parametrize("lens,keep,recent", [([12288, 12289, 40], 7000, 33), ([30001], 12300, 0), ([20000, 12287], 19999, 5000)])
+def test_evict_from_rows_longer_than_the_choice_holds_in_registers(pf, lens, keep, recent, kind):
+    size, heads, dim = 64, 1, 64
+    blocks, tables = make_tables(lens, size, 270)
+    n_dst = -(-keep // size)
+    cache = make_cache(pf, blocks + len(lens) * n_dst, size, heads, dim, 271, wide=5)
+    dst = torch.arange(blocks, blocks + len(lens) * n_dst, dtype=torch.int32).view(len(lens), n_dst)
+    w = torch.exp(2 * torch.randn((len(lens), heads, max(lens)), generator=gen(272), device="cuda"))
+    if kind == "ties":
+        w = torch.floor(w)
+    elif kind == "special":
+        w[..., ::3] = 0
+        w[..., 1::7] = math.nan
+        w[..., 2::11] = math.inf
+        w[..., 4::13] = -0.0
+    before, old, want = bytes_of(cache), ref.Cache(cache), ref.Cache(cache)
+    new_lens, new_w, kept = cache.evict(tables.cuda(), ints(lens), w, dst.cuda(), keep, recent=recent)
+    cache.check()
+    assert new_lens.tolist() == [min(n, keep) for n in lens]
+    w_ = w.cpu()
+    for s, n in enumerate(lens):
+        at = ref.choose(w_[s, 0].tolist(), n, keep, recent)
+        assert kept[s, 0].tolist() == at + [-1] * (keep - len(at))
+        want_w = torch.zeros(new_w.shape[2])
+        want_w[: len(at)] = w_[s, 0, at]
+        assert torch.equal(new_w[s, 0].cpu().nan_to_num(-7.0), want_w.nan_to_num(-7.0))
+        ids = tables[s].long()
+        for kv in range(2):
+            x = (old.values[kv, ids, 0] * old.scales[kv, ids, 0][:, None, None]).reshape(-1, dim)[at]
+            for b in range(-(-len(at) // size)):
+                want.store(kv, int(dst[s, b]), 0, {i: x[b * size + i] for i in range(min(size, len(at) - b * size))})
+    same_bytes(cache, want, before)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_weights_of_several_row_tiles_over_ranges_longer_than_a_pass(pf, dim):
+    """Eight requests whose tokens give each CTA more steps than it sums the weights of at a time."""
+    size, heads, group, rows, lens = 64, 8, 4, 20, [10240, 9000, 10240, 8111, 10240, 10001, 10240, 10240]
+    blocks, tables = make_tables(lens, size, 280)
+    cache = make_cache(pf, blocks, size, heads, dim, 281)
+    q = torch.randn((8 * rows, heads * group, dim), generator=gen(282), device="cuda").half()
+    w = torch.rand((8, heads, max(lens)), generator=gen(283), device="cuda")
+    before = w.clone()
+    out, lse = cache.attention(q, tables.cuda(), ints(lens), weights=w, lse=True)
+    cache.check()
+    for s, n in enumerate(lens):
+        a = slice(s * rows, (s + 1) * rows)
+        close(cache, q[a], out[a], lse[a], w[s, :, :n], before[s, :, :n], plain(cache, q[a], tables[s].tolist(), n, dim ** -0.5), n)
+        assert torch.equal(w[s, :, n:], before[s, :, n:])
+
+
+def test_the_largest_numbers_that_a_cache_holds(pf):
+    """2^120 is the largest scale: e4m3 values of 256 and more then stand for numbers that fp32 does not have."""
+    cache = pf.Kv8Cache(2, 16, 1, 64)
+    x = torch.zeros((1, 1, 64), dtype=torch.bfloat16, device="cuda")
+    x[0, 0, 0], x[0, 0, 1], x[0, 0, 2], x[0, 0, 3] = 3.3895313892515355e38, 3e38, -2.5e38, math.inf
+    cache.append(x, x, ints([[1]]), ints([0]))
+    assert (cache.scales[:, 1, 0] == 2.0 ** 120).all()
+    assert cache.values[0, 1, 0, 0, :4].float().tolist() == [256.0, 224.0, -192.0, 448.0]
+    cache.check()
