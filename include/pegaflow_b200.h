@@ -543,7 +543,7 @@ void pf_load_state_free(pf_load_state *state);                   /* unlinks when
  *    kv_heads x block_size x head_dim e4m3 values (head-major) and behind them one fp32 scale for
  *    each head, padded to 16 bytes: a value stands for itself times its head's scale.  Scales are
  *    powers of two, the least that brings the head's largest finite magnitude in that block within 448
- *    (exponents -110 to 120).  To the engine it is a layer of two segments of pf_kv8_record_bytes
+ *    (exponents -110 to 120; magnitudes above 2.97e38, which take the last one, may read back as infinity).  To the engine it is a layer of two segments of pf_kv8_record_bytes
  *    bytes: registration, save, load and peer copy move a block together with its scales.
  *
  *    All calls only enqueue work on `stream` (of the device `device_id`, which need not be the

@@ -20,7 +20,9 @@
 
 namespace pf {
 
-constexpr int kKv8MinExp = -110, kKv8MaxExp = 120;   // 2^e, 1 / 2^e and their products with e4m3 values stay normal
+// 2^e, 1 / 2^e and their products with e4m3 values stay normal, but for one thing: with e = 120, which only magnitudes above
+// 1.75 * 2^127 (2.97e38) ask for, values of 256 and more stand for numbers beyond fp32, which reads them as infinities.
+constexpr int kKv8MinExp = -110, kKv8MaxExp = 120;
 
 struct Kv8View {
   char *base;
