@@ -7,14 +7,6 @@
 namespace pf {
 namespace {
 
-template <bool kBf16>
-__device__ __forceinline__ uint32_t narrow2(float lo, float hi) {
-  if (!kBf16) return f16x2(lo, hi);
-  uint32_t d;
-  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
-  return d;
-}
-
 // Joins the parts of segments that several CTAs shared, in the order of the tokens.  CTA (b, y) looks at the boundary
 // between the ranges of CTAs b and b + 1: if it is the first one within a segment, it joins rows of it, a team of threads
 // for each.  kDim / 4 threads hold a row of a part as float4; a team of more reads several parts at once.  Bound by latency:

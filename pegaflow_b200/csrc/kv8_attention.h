@@ -224,7 +224,7 @@ void kv8_few_launch(const AttnParams &p, int rows, bool bf16, cudaStream_t strea
 void kv8_weights_launch(const AttnParams &p, bool bf16, int n_sms, cudaStream_t stream);
 // Query rows by the hundred (kv8_attention_wide.cu).
 struct WidePlan {
-  int rows, tokens, threads;
+  int rows, tokens;
   size_t smem;
 };
 WidePlan kv8_wide_plan(int dim);

@@ -365,13 +365,7 @@ __global__ void __launch_bounds__(threads_of(kDim), 1) kv8_attention_wide(AttnPa
               if (!whole) {
                 *reinterpret_cast<float4 *>(p.part_o + ((int64_t)slot * kRows + n - lane + t) * kDim + d) = y;
               } else {
-                uint2 w;
-                if (kBf16) {
-                  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w.x) : "f"(y.y), "f"(y.x));
-                  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w.y) : "f"(y.w), "f"(y.z));
-                } else {
-                  w = make_uint2(f16x2(y.x, y.y), f16x2(y.z, y.w));
-                }
+                const uint2 w = make_uint2(narrow2<kBf16>(y.x, y.y), narrow2<kBf16>(y.z, y.w));
                 if (p.vec_out) {
                   *reinterpret_cast<uint2 *>(dst) = w;
                 } else {
@@ -609,7 +603,7 @@ static_assert(Layout<256>::end <= Layout<128>::end && Layout<64>::end <= Layout<
 
 WidePlan kv8_wide_plan(int dim) {
   const int end = dim == 64 ? Layout<64>::end : dim == 128 ? Layout<128>::end : Layout<256>::end;
-  return WidePlan{kGroupRows * groups_of(dim), tokens_of(dim), threads_of(dim), 1024 + (size_t)end + sizeof(Shared)};
+  return WidePlan{kGroupRows * groups_of(dim), tokens_of(dim), 1024 + (size_t)end + sizeof(Shared)};
 }
 
 void kv8_wide_launch(const AttnParams &p, bool bf16, cudaStream_t stream) {
