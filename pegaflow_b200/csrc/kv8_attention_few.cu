@@ -17,7 +17,7 @@
 // instruction takes.
 //   q    scaled by a power of two for each row so that its largest element lies in [2^7, 2^8): its pieces hold a bf16 or an
 //        f16 exactly down to 2^-18 of the row's largest, and smaller elements to 2^-30 of it
-//   p    2^(6 + s - ref) rounded to f16 (2^-12 of p), ref following the row's running maximum in steps of 2^2; the pieces hold
+//   p    2^(6 + s - ref) rounded to f16 (2^-11 of p at most), ref following the row's running maximum in steps of 2^2; the pieces hold
 //        that exactly down to 2^-11, that is 2^-17 of the largest, and smaller ones to 2^-28 of it
 //   V's scale goes on p: 2^(e - e_ref), e_ref the largest so far, and the sums are in units of it; the row sum leaves it out
 //   sums fp32, the tensor cores' and the row sum's; it takes p before it is rounded

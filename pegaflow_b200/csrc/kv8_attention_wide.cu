@@ -12,8 +12,8 @@
 // products cost 4 * 256 * 128 * 128 flops at 8192 a cycle, the exponentials 256 * 128 at 16 a cycle and shared memory
 // (operands of the products and the converters' stores) 256 KB at 128 a cycle: 2048 cycles each.
 //
-// What it measured (bf16, 128 dimensions, blocks of 16): 2048 new rows of 32 query and 8 KV heads behind 10240 tokens take 524 us,
-// about 5500 cycles a step; without the exponentials 400 us, without the products 394 us, without the conversion 388 us, so
+// What it measured (bf16, 128 dimensions, blocks of 16): 2048 new rows of 32 query and 8 KV heads behind 10240 tokens take 527 to
+// 548 us on several boxes, about 5500 cycles a step; without the exponentials 400 us, without the products 394 us, without the conversion 388 us, so
 // that the three still wait for one another.  Four converter warps with half a step of loads in flight: 750 us.  One read of
 // the scores for the maximum and one for P: 623 us.  Sequence and tile in registers instead of shared memory: 600 us, by
 // spilled registers that the little L1 beside 227 KB of shared memory does not hold.
@@ -21,6 +21,9 @@
 // K and V have one layout in shared memory, rows of 128 bytes (64 dimensions) with 16-byte chunks swizzled over
 // eight rows: as the operand of the scores its contracted index runs along the row, as the operand of the output it runs
 // down the rows, which is the other of the two majors that a descriptor can name.
+//
+// Roundings to f16: P, by 2^-11 of itself at most (the row sums take it before that), because the tensor cores take no fp32; Q is
+// exact but for elements below 2^-28 of their row's largest.
 //
 // Scales, 2^e a block: the converters multiply K and V by 2^(e - e_ref) on the way, so that one unit holds for a step.  An e4m3
 // number is a multiple of 2^-9 and below 2^9: in f16 it stays exact for e - e_ref from -15 to 7, and what is lost further
