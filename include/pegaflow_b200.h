@@ -543,8 +543,9 @@ void pf_load_state_free(pf_load_state *state);                   /* unlinks when
  *    kv_heads x block_size x head_dim e4m3 values (head-major) and behind them one fp32 scale for
  *    each head, padded to 16 bytes: a value stands for itself times its head's scale.  Scales are
  *    powers of two, the least that brings the head's largest finite magnitude in that block within 448
- *    (exponents -110 to 120; magnitudes above 2.97e38, which take the last one, may read back as infinity).  To the engine it is a layer of two segments of pf_kv8_record_bytes
- *    bytes: registration, save, load and peer copy move a block together with its scales.
+ *    (exponents -110 to 120; magnitudes above 2.97e38, which take the last one, may read back as
+ *    infinity).  To the engine it is a layer of two segments of pf_kv8_record_bytes bytes:
+ *    registration, save, load and peer copy move a block together with its scales.
  *
  *    All calls only enqueue work on `stream` (of the device `device_id`, which need not be the
  *    current one), allocate nothing and may be captured.  Block tables, lengths and row starts
@@ -568,8 +569,8 @@ enum pf_kv8_dtype { PF_KV8_BF16 = 0, PF_KV8_F16 = 1 };
 /* Bits of *status: what a kernel found and left out. */
 #define PF_KV8_BAD_BLOCK 1u   /* a block id outside the cache: its tokens are not written / not seen */
 #define PF_KV8_BAD_LENGTH 2u  /* a length below 0, or above what the block table or the weights hold: cut */
-#define PF_KV8_BAD_ROWS 4u    /* row starts that fall, leave the tensors, or give a sequence more than max_query rows: cut; where one
-                               falls, attention computes no row of the call */
+#define PF_KV8_BAD_ROWS 4u    /* row starts that fall, leave the tensors, or give a sequence more than max_query rows: cut; where they
+                               claim more rows than the call can have, attention computes none */
 #define PF_KV8_STALLED 8u     /* a wait inside a kernel ran out (two seconds): the outputs of the call are not valid */
 
 typedef struct pf_kv8_batch {

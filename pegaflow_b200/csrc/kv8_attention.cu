@@ -91,11 +91,23 @@ __device__ __forceinline__ void join(const AttnParams &p, const Work<kRows, kUni
   }
 }
 
-// Rows of no sequence, [0, first) and [last, n_rows), are cleared; all rows where none was computed, for the weights' sake too.
+// Rows of no sequence, [0, first) and [last, n_rows), are cleared; where none was computed all rows, for the weights' sake too.  Where
+// a row start falls, any sequence may have the first and the last ones.
 template <int kDim>
-__device__ __forceinline__ void clear_rows(const AttnParams &p, bool none) {
+__device__ __forceinline__ void clear_rows(const AttnParams &p, bool none, bool falls) {
+  __shared__ int sh_first, sh_last;
   int first = 0, last = 0, ignored;
-  if (!none) {
+  if (falls && !none) {
+    if (threadIdx.x == 0) sh_first = p.batch.n_rows, sh_last = 0;
+    __syncthreads();
+#pragma unroll 1
+    for (int s = threadIdx.x; s < p.batch.n_seqs; s += kJoinThreads) {
+      p.batch.rows(s, first, last);
+      if (first < last) atomicMin(&sh_first, first), atomicMax(&sh_last, last);
+    }
+    __syncthreads();
+    first = min(sh_first, sh_last), last = sh_last;
+  } else if (!none) {
     p.batch.rows(0, first, ignored);
     p.batch.rows(p.batch.n_seqs - 1, ignored, last);
   }
@@ -113,14 +125,15 @@ __device__ __forceinline__ void clear_rows(const AttnParams &p, bool none) {
   }
 }
 
+// 40 registers: at 48 verify-16-ragged takes 58.0 us, at 40 57.4, at 64 59.3 (decode-1x131000 29.8, 29.7, 30.3).
 template <int kDim, int kRows, int kUnits, bool kBf16>
-__global__ void __launch_bounds__(kJoinThreads) kv8_attention_join(AttnParams p, int team) {
+__global__ void __launch_bounds__(kJoinThreads, 6) kv8_attention_join(AttnParams p, int team) {
   extern __shared__ __align__(128) char smem[];
   const Work<kRows, kUnits> work(p, reinterpret_cast<uint32_t *>(smem));
   after_previous();
   join<kDim, kRows, kUnits, kBf16>(p, work, team);
   const bool none = work.total() == 0;
-  if (p.clear_tail || (none && p.weights)) clear_rows<kDim>(p, none);      // behind the join, which others may wait for
+  if (p.clear_tail || (none && p.weights)) clear_rows<kDim>(p, none, work.falls);      // behind the join, which others may wait for
 }
 
 // Each token's probability from the scores that the attention kept, added to the weights: a thread a token, rows in order.
@@ -144,10 +157,6 @@ __global__ void __launch_bounds__(kAddThreads) kv8_weights_add(AttnParams p) {
       if (lse != -INFINITY) base[r] = lse * kLog2e;
     }
   }
-  bool any = false;            // of rows that were not computed (a row start falls) there are no scores
-#pragma unroll
-  for (int r = 0; r < kRows; ++r) any |= base[r] != INFINITY;
-  if (!any) return;
   const float *scores = p.scores + (int64_t)blockIdx.x * p.score_tokens * kRows;
   float *weights = p.weights + s * p.w_seq + head * p.w_head;
   for (int tok = blockIdx.y * kAddThreads + threadIdx.x; tok < end; tok += gridDim.y * kAddThreads) {
@@ -170,6 +179,7 @@ struct Plan {
   size_t part_o, part_ml, lse, scores, bytes;   // offsets in the workspace
   int score_tokens;     // 0: scores are not kept
   int row_tiles;        // of a sequence, at most
+  uint32_t units;       // of all its rows, at most
 };
 
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
@@ -192,6 +202,7 @@ Plan make_plan(int device_id, const Kv8View &c, const Kv8Batch &b, const pf_kv8_
                          (((uint64_t)a.n_rows * group) / plan.rows + b.n_seqs) * c.heads;
   const uint64_t row_tiles = std::max<uint64_t>(1, (rows + plan.rows - 1) / plan.rows);
   if (units > 0xffffffffull || row_tiles * b.n_seqs > 1u << 29) throw Error::invalid("too many query rows for tables of this width: split the call");
+  plan.units = (uint32_t)units;
   plan.row_tiles = (int)row_tiles;
   plan.n_ctas = kv8_sm_count(device_id) * (plan.wide ? 1 : kv8_few_ctas(c.dim, plan.rows));
   const size_t slots = 2 * (size_t)plan.n_ctas * plan.rows;
@@ -351,6 +362,7 @@ int pf_kv8_attention(int device_id, const pf_kv8_cache *cache, const pf_kv8_batc
     p.group = (int)a.q_heads / c.heads;
     p.max_query = (int)std::min<size_t>(a.max_query, a.n_rows);
     p.row_tiles_most = plan.row_tiles;
+    p.units_most = plan.units;
     p.causal = a.causal != 0;
     p.clear_tail = a.clear_tail;
     p.vec_q = (uintptr_t)a.q % 16 == 0 && (a.q_row_stride | a.q_head_stride) % 8 == 0;

@@ -23,6 +23,7 @@ struct AttnParams {
   int w_capacity;
   int q_heads, group, max_query;
   int row_tiles_most;   // of a sequence
+  uint32_t units_most;  // units (see Work) that n_rows rows can be, however they fall on the sequences
   int causal, clear_tail, vec_q, vec_out;
   float scale;
   // Partial results: slot 2 c + k of CTA c (k = 0: the segment that its range starts in, 1: the one that it ends in).
@@ -77,8 +78,8 @@ struct Seq {
 // The units of all (sequence, row tile) entries in order, kCost of them in front of each head's for what a segment costs at its
 // beginning and end, as sums before every chunk of entries (one, unless there are more
 // than kMost).  Every CTA of every kernel computes them for itself: lens stay on the device, and no launch and no
-// workspace is spent on it.  Where a row start falls there is no work at all: starts that fall and rise again claim rows more than
-// once, more of them together than the host has checked 32 bits for.
+// workspace is spent on it.  Starts that fall and rise again claim rows more than once: where one falls the units are counted
+// once more, in 64 bits, and if they are more than the host has checked 32 bits for, there is no work at all.
 template <int kRows, int kUnit, bool kWhole = false>
 struct Work {
   using SeqT = Seq<kRows, kUnit, kWhole>;
@@ -88,7 +89,7 @@ struct Work {
   static constexpr uint32_t kCost = 4;
   uint32_t *prefix;         // [chunks + 1] in shared memory
   int entries, chunk, chunks;
-  bool none;                // a row start falls
+  bool falls, none;         // a row start falls; and there is no work for that
   static __host__ __device__ int chunk_of(int entries) { return max((entries + kMost - 1) / kMost, 1); }
   static __host__ size_t bytes(int n_seqs, int row_tiles_most) {
     const int entries = n_seqs * row_tiles_most, chunk = chunk_of(entries);
@@ -105,16 +106,16 @@ struct Work {
     bool ignored;
     return units_of(p, e, ignored);
   }
-  __device__ Work(const AttnParams &p, uint32_t *prefix) : prefix(prefix) {
+  __device__ Work(const AttnParams &p, uint32_t *prefix) : prefix(prefix), falls(false) {
     __shared__ uint32_t warp_sum[32];
-    __shared__ int sh_none;
-    if (threadIdx.x == 0) sh_none = 0;
+    __shared__ int sh_falls;
+    __shared__ unsigned long long sh_units;
+    if (threadIdx.x == 0) sh_falls = 0;
     entries = p.batch.n_seqs * p.row_tiles_most;
     chunk = chunk_of(entries);
     chunks = (entries + chunk - 1) / chunk;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n_warps = (blockDim.x + 31) >> 5;
     uint32_t base = 0;
-    bool falls = false;
     for (int c0 = 0; c0 < chunks; c0 += blockDim.x) {
       const int c = c0 + threadIdx.x;
       uint32_t mine = 0;
@@ -137,9 +138,19 @@ struct Work {
       __syncthreads();
     }
     if (threadIdx.x == 0) prefix[chunks] = base;
-    if (falls) sh_none = 1;          // a vote of the barrier instead costs half a microsecond
+    if (falls) sh_falls = 1;         // a vote of the barrier instead costs half a microsecond
     __syncthreads();
-    none = sh_none;
+    none = falls = sh_falls;
+    if (falls) {
+      if (threadIdx.x == 0) sh_units = 0;
+      __syncthreads();
+      unsigned long long mine = 0;
+#pragma unroll 1
+      for (int e = threadIdx.x; e < entries; e += blockDim.x) mine += (unsigned long long)units_of(p, e) * (uint32_t)p.cache.heads;
+      atomicAdd(&sh_units, mine);
+      __syncthreads();
+      none = sh_units > p.units_most;
+    }
   }
   __device__ uint32_t total() const { return none ? 0u : prefix[chunks]; }
 };

@@ -217,20 +217,38 @@ def test_row_starts_that_fall_again_and_again_do_no_harm(pf, seqs, n, width, hea
     assert (out == 0).all() and torch.isneginf(lse).all()
 
 
-@pytest.mark.parametrize("rows", [1, 5, 40])
-def test_row_starts_that_fall_leave_weights_as_they_are(pf, rows):
-    """Whether scores would have been kept or taken again; without an lse of the call's own; a given out stays too."""
-    size, heads, dim = 16, 2, 128
-    blocks, tables = make_tables([100, 80, 60], size, 266)
-    cache = make_cache(pf, blocks, size, heads, dim, 267)
-    q = torch.randn((2 * rows, 4 * heads, dim), generator=gen(268), device="cuda").half()
-    w = torch.rand((3, heads, 100), generator=gen(269), device="cuda")
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_row_starts_that_fall_again_and_again_leave_weights_as_they_are(pf, dim):
+    """Without an lse of the call's own; a given out stays too."""
+    size, heads, seqs, rows = 16, 2, 400, 200
+    cache = make_cache(pf, 8, size, heads, dim, 267)
+    q = torch.randn((rows, 4 * heads, dim), generator=gen(268), device="cuda").half()
+    tables, lens = ints([[1, 2, 3, 4]]).expand(seqs, 4), torch.full((seqs,), 64, dtype=torch.int32, device="cuda")
+    w = torch.rand((seqs, heads, 64), generator=gen(269), device="cuda")
     before, out = w.clone(), torch.full_like(q, 3.0)
-    starts = ints([0, 2 * rows, rows, 2 * rows])
-    cache.attention(q, tables.cuda(), ints([100, 80, 60]), starts=starts, max_query=rows, weights=w, out=out)
+    cache.attention(q, tables, lens, starts=ints([0, rows] * (seqs // 2) + [0]), max_query=rows, weights=w, out=out)
     with pytest.raises(pf.PegaflowInvalidArgument, match="row starts"):
         cache.check()
     assert torch.equal(w, before) and (out == 3).all()
+
+
+@pytest.mark.parametrize("rows", [1, 5, 40])
+def test_a_row_start_that_falls_behind_the_sequences_cuts_those_rows_alone(pf, rows):
+    """A batch padded with sequences whose starts are 0: reported, and the others' rows are computed as ever."""
+    size, heads, dim, n = 16, 2, 128, 100
+    blocks, tables = make_tables([n, n - 10], size, 266)
+    cache = make_cache(pf, blocks, size, heads, dim, 267)
+    q = torch.randn((2 * rows + 3, 4 * heads, dim), generator=gen(268), device="cuda").half()
+    t = torch.cat([tables, torch.zeros((2, tables.shape[1]), dtype=torch.int32)]).cuda()
+    w = torch.rand((4, heads, n), generator=gen(269), device="cuda")
+    before = w.clone()
+    out, lse = cache.attention(q, t, ints([n, n - 10, 0, 0]), starts=ints([0, rows, 2 * rows, 0, 0]), max_query=rows, weights=w, lse=True)
+    with pytest.raises(pf.PegaflowInvalidArgument, match="row starts"):
+        cache.check()
+    for s in range(2):
+        a, m = slice(s * rows, (s + 1) * rows), n - 10 * s
+        close(cache, q[a], out[a], lse[a], w[s, :, :m], before[s, :, :m], plain(cache, q[a], tables[s].tolist(), m, dim ** -0.5), m)
+    assert torch.equal(w[2:], before[2:])
 
 
 def test_prompts_over_wide_tables_are_counted_by_their_own_tiles(pf):
