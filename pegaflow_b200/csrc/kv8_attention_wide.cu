@@ -13,7 +13,7 @@
 // (operands of the products and the converters' stores) 256 KB at 128 a cycle: 2048 cycles each.
 //
 // What it measured (bf16, 128 dimensions, blocks of 16): 2048 new rows of 32 query and 8 KV heads behind 10240 tokens take 527 to
-// 548 us on several boxes, about 5500 cycles a step; without the exponentials 400 us, without the products 394 us, without the conversion 388 us, so
+// 548 us on several GPUs, about 5500 cycles a step; without the exponentials 400 us, without the products 394 us, without the conversion 388 us, so
 // that the three still wait for one another.  Four converter warps with half a step of loads in flight: 750 us.  One read of
 // the scores for the maximum and one for P: 623 us.  Sequence and tile in registers instead of shared memory: 600 us, by
 // spilled registers that the little L1 beside 227 KB of shared memory does not hold.
