@@ -597,6 +597,7 @@ int pf_kv8_append(int device_id, const pf_kv8_cache *cache, const pf_kv8_batch *
 /* Attention of n_rows query rows over the cache.  lens include the rows' own tokens: row i of a sequence with n rows
  * is token lens - n + i and sees, with `causal`, the tokens up to itself, otherwise all.  out = sum p * V with
  * p = exp(scale * q.K - lse) over the visible tokens; a row that sees nothing gives out = 0, lse = -infinity.
+ * The sums are fp32 and hold up to 64 times V for each token before they are divided: V above 2^104 (2e31) may overflow.
  * weights (may be NULL) [n_seqs][kv_heads][weights_capacity]: the sum of p over the sequence's rows and the
  * query heads of the group is added for each token, in an order that does not vary. */
 enum { PF_KV8_CLEAR_ALL = 1, PF_KV8_CLEAR_LSE = 2 };
